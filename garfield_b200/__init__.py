@@ -28,6 +28,7 @@ __all__ = [
     "GarfieldError", "lib", "lib_path", "SearchParams", "Index", "Plan", "NO_ID", "schedule_batches",
     "read_fvecs", "write_fvecs", "read_attrs", "write_attrs", "read_u32mat", "write_u32mat",
     "read_ranges", "write_ranges", "read_labels", "read_grid",
+    "Fp4Rows", "quantize_fp4", "dequantize_fp4", "quantize_fp4_host", "dequantize_fp4_host",
 ]
 
 NO_ID = 0xFFFFFFFF
@@ -139,6 +140,11 @@ def lib() -> C.CDLL:
         "gf_write_q": (C.c_int, [C.c_char_p, _P, _P, _P, _U32, _U32]),
         "gf_quantize_i8": (C.c_int, [_P, _U32, _U32, C.c_float, _P, _P, _P, _P]),
         "gf_quantize_i8_host": (C.c_int, [_P, _U32, _U32, C.c_float, _P, _P, _P]),
+        "gf_fp4_bytes": (C.c_uint64, [_U32, _U32, _U32]),
+        "gf_quantize_fp4": (C.c_int, [_P, _U32, C.c_uint64, _U32, _U32, C.c_float, _U32, _P, _P]),
+        "gf_dequantize_fp4": (C.c_int, [_P, _U32, _U32, _U32, C.c_float, _P, _U32, C.c_uint64, _P]),
+        "gf_quantize_fp4_host": (C.c_int, [_P, _U32, _U32, C.c_float, _U32, _P]),
+        "gf_dequantize_fp4_host": (C.c_int, [_P, _U32, _U32, _U32, C.c_float, _P]),
         "gf_write_attrs": (C.c_int, [C.c_char_p, _P, _U32, _U32]),
         "gf_read_u32mat": (C.c_int, [C.c_char_p, _PTR(_P), _PTR(_U32), _PTR(_U32)]),
         "gf_write_u32mat": (C.c_int, [C.c_char_p, _P, _U32, _U32]),
@@ -541,6 +547,139 @@ def quantize_i8(data, alpha: float = 1.0, stream=None):
     _check(lib().gf_quantize_i8(_dev_ptr(data), n, dim, alpha, _dev_ptr(q), _dev_ptr(sc), _dev_ptr(zp),
                                 _stream_ptr(stream)), "gf_quantize_i8")
     return q, sc, zp
+
+
+# ------------------------------------------------- 4-bit block floating point
+
+@dataclass
+class Fp4Rows:
+    """n x dim rows held in 4 bits (the packed form that include/garfield.h describes): codes with one
+    scale per `block` elements of a row, standing for the data multiplied by alpha.  packed is a uint8
+    CUDA tensor, or a numpy array from quantize_fp4_host."""
+    packed: object
+    n: int
+    dim: int
+    block: int
+    alpha: float
+
+
+def _fp4_need(ok: bool, what: str, msg: str) -> None:
+    if not ok:
+        raise GarfieldError(1, what, msg)
+
+
+def _fp4_dtype(dtype, what: str) -> int:
+    import torch
+    kinds = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    _fp4_need(dtype in kinds, what, f"dtype {dtype} is not float32, float16 or bfloat16")
+    return kinds[dtype]
+
+
+def _fp4_matrix(t, what: str, name: str):
+    """(rows, columns, row stride) of a CUDA matrix whose rows are each without gaps."""
+    import torch
+    _fp4_need(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2, what, f"{name}: expected a 2-D CUDA tensor")
+    n, dim = t.shape
+    _fp4_need(0 < dim < 2 ** 32 and n < 2 ** 32, what, f"{name}: shape {tuple(t.shape)} out of range")
+    _fp4_need(dim == 1 or n == 0 or t.stride(1) == 1, what, f"{name}: the elements of a row must be adjacent")
+    ld = t.stride(0) if n > 1 else dim
+    _fp4_need(ld >= dim, what, f"{name}: rows overlap (stride {ld} below {dim})")
+    return n, dim, ld
+
+
+def _fp4_rows(rows, what: str):
+    import torch
+    _fp4_need(isinstance(rows, Fp4Rows), what, "expected Fp4Rows")
+    p = rows.packed
+    _fp4_need(isinstance(p, torch.Tensor) and p.is_cuda and p.dtype == torch.uint8 and p.is_contiguous(), what,
+              "Fp4Rows.packed: expected a contiguous uint8 CUDA tensor")
+    need = lib().gf_fp4_bytes(rows.n, rows.dim, rows.block)
+    _fp4_need(rows.dim > 0 and rows.block in (16, 32), what, f"dim {rows.dim}, block {rows.block}")
+    _fp4_need(p.numel() >= need, what, f"Fp4Rows.packed holds {p.numel()} bytes, {need} needed")
+    return p
+
+
+class _on_stream:
+    """Makes a tensor's device current, and the given stream of it (None: the device's current one),
+    so that what is allocated inside belongs to the stream that the kernels run on."""
+
+    def __init__(self, device, stream):
+        import torch
+        if stream is not None and not hasattr(stream, "cuda_stream"):
+            stream = torch.cuda.ExternalStream(int(stream), device=device)
+        self.stream = stream if stream is not None else torch.cuda.current_stream(device)
+        self.device, self.ctx = torch.cuda.device(device), torch.cuda.stream(self.stream)
+
+    def __enter__(self):
+        self.device.__enter__()
+        self.ctx.__enter__()
+        return C.c_void_p(self.stream.cuda_stream)
+
+    def __exit__(self, *exc):
+        self.ctx.__exit__(*exc)
+        self.device.__exit__(*exc)
+
+
+def quantize_fp4(data, alpha: float = 1.0, block: int = 32, stream=None) -> Fp4Rows:
+    """gf_quantize_fp4: the rows of a float32, float16 or bfloat16 CUDA matrix, held in 4 bits."""
+    import torch
+    what = "gf_quantize_fp4"
+    n, dim, ld = _fp4_matrix(data, what, "data")
+    dt = _fp4_dtype(data.dtype, what)
+    _fp4_need(block in (16, 32), what, f"block {block} is not 16 or 32")
+    with _on_stream(data.device, stream) as s:
+        packed = torch.empty(lib().gf_fp4_bytes(n, dim, block), dtype=torch.uint8, device=data.device)
+        _check(lib().gf_quantize_fp4(C.c_void_p(data.data_ptr()), dt, ld, n, dim, alpha, block,
+                                     C.c_void_p(packed.data_ptr()), s), what)
+    return Fp4Rows(packed, n, dim, block, float(alpha))
+
+
+def dequantize_fp4(rows: Fp4Rows, dtype=None, out=None, stream=None):
+    """gf_dequantize_fp4: the values that rows are held as (n x dim, float32 unless dtype or out say
+    otherwise)."""
+    import torch
+    what = "gf_dequantize_fp4"
+    p = _fp4_rows(rows, what)
+    dtype = dtype or (out.dtype if out is not None else torch.float32)
+    dt = _fp4_dtype(dtype, what)
+    with _on_stream(p.device, stream) as s:
+        out = _fp4_out(out, (rows.n, rows.dim), dtype, p.device, what)
+        _check(lib().gf_dequantize_fp4(C.c_void_p(p.data_ptr()), rows.n, rows.dim, rows.block, rows.alpha,
+                                       C.c_void_p(out.data_ptr()), dt, max(out.stride(0), rows.dim), s), what)
+    return out
+
+
+def _fp4_out(out, shape, dtype, device, what: str):
+    import torch
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    _fp4_need(isinstance(out, torch.Tensor) and out.is_cuda and tuple(out.shape) == shape and out.dtype == dtype
+              and out.device == device, what, f"out: expected a {dtype} tensor of shape {shape} on {device}")
+    if out.numel():
+        _fp4_matrix(out, what, "out")
+    return out
+
+
+def quantize_fp4_host(data: np.ndarray, alpha: float = 1.0, block: int = 32) -> Fp4Rows:
+    """gf_quantize_fp4_host on a float32 array: the same bytes as quantize_fp4."""
+    data = np.ascontiguousarray(data, dtype=np.float32)
+    n, dim = data.shape
+    _fp4_need(dim > 0 and block in (16, 32), "gf_quantize_fp4_host", f"dim {dim}, block {block}")
+    packed = np.empty(lib().gf_fp4_bytes(n, dim, block), np.uint8)
+    _check(lib().gf_quantize_fp4_host(_np_ptr(data), n, dim, alpha, block, _np_ptr(packed)), "gf_quantize_fp4_host")
+    return Fp4Rows(packed, n, dim, block, float(alpha))
+
+
+def dequantize_fp4_host(rows: Fp4Rows) -> np.ndarray:
+    """gf_dequantize_fp4_host: the float32 values that rows with a host array are held as."""
+    what = "gf_dequantize_fp4_host"
+    p = rows.packed
+    _fp4_need(isinstance(p, np.ndarray) and p.dtype == np.uint8 and p.flags["C_CONTIGUOUS"], what,
+              "Fp4Rows.packed: expected a contiguous uint8 array")
+    _fp4_need(p.size >= lib().gf_fp4_bytes(rows.n, rows.dim, rows.block), what, "Fp4Rows.packed is too short")
+    out = np.empty((rows.n, rows.dim), np.float32)
+    _check(lib().gf_dequantize_fp4_host(_np_ptr(p), rows.n, rows.dim, rows.block, rows.alpha, _np_ptr(out)), what)
+    return out
 
 
 def read_q(path):

@@ -446,6 +446,50 @@ gf_status gf_quantize_i8(const float* data, uint32_t n, uint32_t dim, float alph
                          int32_t* zero_points_out, void* stream);
 gf_status gf_quantize_i8_host(const float* data, uint32_t n, uint32_t dim, float alpha, int8_t* q_out,
                               float* scales_out, int32_t* zero_points_out);
+/* -------------------------------------- 4-bit block floating point (device) */
+
+/* Element types of the arrays that the calls below read and write. */
+typedef enum { GF_F32 = 0, GF_F16 = 1, GF_BF16 = 2 } gf_dtype;
+
+/*
+ * Rows held in 4 bits, beside the byte codecs above.  No counterpart in the reference.  A row is cut
+ * into blocks of 32 or 16 consecutive elements (the last may be short).  With x = data *
+ * alpha (fp32, rounded) and amax = max |x| over a block, the block's scale s and the codes are
+ *   block 32: s = 2^(floor(log2 amax) - 2), exponent at least -127 (E8M0)
+ *   block 16: s = amax / 6 rounded to E4M3 (nearest, ties to even, at most 448)
+ *   code = x / s rounded to E2M1 -- 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives -- nearest,
+ *          ties to the even code, at most 6 in size; 0 where s = 0
+ * and an element is held as code * s / alpha.  Block 32 covers fp32's range with alpha = 1; its
+ * largest elements saturate when amax is above 1.5 of its binade.  Block 16 is the more accurate;
+ * alpha has to bring amax / 6 into E4M3's range, 2^-9 to 448 (larger data saturate, smaller
+ * become 0).  A block with an infinity or a NaN after the multiplication is held as NaN.
+ *
+ * The held form ("packed") is one array of gf_fp4_bytes(n, dim, block) bytes, 16-byte aligned:
+ * panels of 128 rows, in a panel groups of 128 elements, in a group the scales and then
+ * columns of 32 elements (only those the row has, in its last group).
+ *   scales:  for every 4 blocks 512 bytes; block b (of 4) of row r at (r % 32) * 16 + (r / 32) * 4 + b
+ *   column:  2048 bytes, row r at r * 16, element 2i in the low half of byte i, 2i + 1 in the high
+ * r being the row in its panel.  Scales and codes past a row's end are 0; the bytes of rows
+ * that the last panel lacks are neither written nor used.  gf_fp4_bytes is 0 for a bad shape
+ * (dim = 0, or a block other than 16 and 32).
+ *
+ * Device calls take device pointers on the current device, enqueue one kernel on `stream`,
+ * allocate nothing and can be captured into a graph; n = 0 does nothing.  dtype is a gf_dtype;
+ * ld is the distance between rows in elements, at least dim.  alpha is positive and finite.
+ * _host: host arrays, fp32 rows without gaps; gf_quantize_fp4_host writes the same bytes as
+ * gf_quantize_fp4, and 0 in the rows that the last panel lacks.
+ * gf_dequantize_fp4 multiplies each code with the rounded s / alpha and rounds to dtype: exact
+ * in fp32 when alpha is a power of two, else within 2^-23 of the held value.
+ */
+uint64_t gf_fp4_bytes(uint32_t n, uint32_t dim, uint32_t block);
+gf_status gf_quantize_fp4(const void* data, uint32_t dtype, uint64_t ld, uint32_t n, uint32_t dim, float alpha,
+                          uint32_t block, void* packed_out, void* stream);
+gf_status gf_dequantize_fp4(const void* packed, uint32_t n, uint32_t dim, uint32_t block, float alpha, void* out,
+                            uint32_t dtype, uint64_t ld, void* stream);
+gf_status gf_quantize_fp4_host(const float* data, uint32_t n, uint32_t dim, float alpha, uint32_t block,
+                               void* packed_out);
+gf_status gf_dequantize_fp4_host(const void* packed, uint32_t n, uint32_t dim, uint32_t block, float alpha, float* out);
+
 /* attrs.bin: uint32 n, uint32 a, n*a int32 (tools.cuh:747-765). */
 gf_status gf_read_attrs(const char* path, int32_t** attrs, uint32_t* n, uint32_t* a);
 gf_status gf_write_attrs(const char* path, const int32_t* attrs, uint32_t n, uint32_t a);

@@ -1,0 +1,181 @@
+"""4-bit block floating point on the host: the held values against the format's definition in 64
+bits, the packed byte positions, non-finite blocks and refusals."""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+
+import garfield_b200 as gf
+
+MAGS = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+
+
+def e4m3_values():
+    """All finite non-negative E4M3 values by code."""
+    v = [m / 8 * 2.0 ** -6 for m in range(8)]
+    v += [(1 + m / 8) * 2.0 ** (e - 7) for e in range(1, 16) for m in range(8)]
+    return np.array(v[:127])
+
+
+def nearest_even(x, table):
+    """Index of the table value nearest to x (x >= 0, ascending table), ties to the even index."""
+    hi = np.clip(np.searchsorted(table, x), 1, len(table) - 1)
+    lo = hi - 1
+    dl, dh = x - table[lo], table[hi] - x
+    return np.where((dl < dh) | ((dl == dh) & (lo % 2 == 0)), lo, hi)
+
+
+def held(x, alpha, block):
+    """codes (signed values), scales and held values of float32 rows, from the definition in 64 bits."""
+    n, dim = x.shape
+    nb = -(-dim // block)
+    v = np.zeros((n, nb * block))
+    v[:, :dim] = (x.astype(np.float32) * np.float32(alpha)).astype(np.float64)
+    v = v.reshape(n, nb, block)
+    amax = np.abs(v).max(2)
+    if block == 32:
+        e = np.where(amax > 0, np.frexp(amax)[1] - 3, -127)
+        s = 2.0 ** np.clip(e, -127, 127)
+    else:
+        t = e4m3_values()
+        s = t[nearest_even(np.minimum(amax / 6, 448.0), t)]
+    with np.errstate(divide="ignore", invalid="ignore"):
+        y = np.where(s[:, :, None] > 0, np.abs(v) / s[:, :, None], 0.0)
+    code = np.copysign(MAGS[nearest_even(np.minimum(y, 6.0), MAGS)], v)
+    return code.reshape(n, -1), s, ((code * s[:, :, None]).reshape(n, -1)[:, :dim]) / alpha
+
+
+def data(n, dim, seed, kind):
+    rng = np.random.default_rng(seed)
+    if kind == "normal":
+        return rng.standard_normal((n, dim)).astype(np.float32)
+    if kind == "wide":  # magnitudes over many binades, both signs, some zeros and whole zero rows
+        x = rng.standard_normal((n, dim)) * 2.0 ** rng.uniform(-20, 8, (n, dim))
+        x[rng.random((n, dim)) < 0.1] = 0.0
+        x[::7] = 0.0
+        return x.astype(np.float32)
+    # values on and next to the borders between codes: border * scale, one ulp below and above
+    b = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 0.5, 4.0])
+    x = (rng.choice(b, (n, dim)) * rng.choice([-1.0, 1.0], (n, dim))).astype(np.float32)
+    x[:, 0] = 6.0
+    y = np.nextafter(x, np.float32(0.0))
+    z = np.nextafter(x, np.float32(9.0) * np.sign(x))
+    pick = rng.integers(0, 3, (n, dim))
+    return np.where(pick == 0, x, np.where(pick == 1, y, z)).astype(np.float32)
+
+
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("alpha", [1.0, 16.0, 0.3])
+@pytest.mark.parametrize("kind", ["normal", "wide", "borders"])
+@pytest.mark.parametrize("n,dim", [(1, 1), (3, 96), (130, 33), (5, 300), (129, 128)])
+def test_host_values_match_definition(n, dim, kind, alpha, block):
+    x = data(n, dim, n * 1000 + dim, kind)
+    got = gf.dequantize_fp4_host(gf.quantize_fp4_host(x, alpha, block))
+    _, _, want = held(x, alpha, block)
+    if alpha == 0.3:  # s / alpha and its product with the code are each rounded: 2 * 2^-24, and alpha itself
+        a32 = float(np.float32(alpha))
+        want = want * alpha / a32
+        assert np.all(np.abs(got - want) <= 2.0 ** -23 * np.abs(want) + 1e-45)
+    else:
+        assert np.array_equal(got, want.astype(np.float32))
+
+
+@pytest.mark.parametrize("block", [16, 32])
+def test_packed_positions(block):
+    """Each code and scale stands where the header says."""
+    n, dim = 200, 300
+    x = data(n, dim, 5, "wide")
+    rows = gf.quantize_fp4_host(x, 1.0, block)
+    code, s, _ = held(x, 1.0, block)
+    sub = 512 * (32 // block)
+    full = sub + 4 * 2048
+    panel = 2 * full + sub + 2 * 2048  # 300 = 128 + 128 + 44: the last group has 2 columns
+    assert rows.packed.size == gf.lib().gf_fp4_bytes(n, dim, block) == 2 * panel
+    t = e4m3_values()
+    for i in (0, 1, 31, 32, 100, 127, 128, 199):
+        for k in (0, 1, 15, 16, 31, 32, 97, 127, 128, 255, 256, 299):
+            base = (i // 128) * panel + (k // 128) * full
+            r, kg = i % 128, k % 128
+            byte = rows.packed[base + sub + (kg // 32) * 2048 + r * 16 + (kg % 32) // 2]
+            nib = (byte >> (4 * (k & 1))) & 15
+            c = code[i, k]
+            assert MAGS[nib & 7] == abs(c) and bool(nib & 8) == bool(np.signbit(c))
+            b = kg // block
+            s8 = rows.packed[base + (b // 4) * 512 + (r % 32) * 16 + (r // 32) * 4 + b % 4]
+            assert (t[s8] if block == 16 else 2.0 ** (int(s8) - 127)) == s[i, k // block]
+    assert not rows.packed[panel + sub + (200 - 128) * 16:panel + sub + 2048].any()  # rows past n
+
+
+def test_extremes():
+    """The ends of fp32's range hold in blocks of 32; E4M3's range bounds blocks of 16."""
+    x = np.zeros((4, 32), np.float32)
+    x[0, :2] = [np.finfo(np.float32).max, -1e38]
+    x[1, :2] = [2.0 ** -126, 2.0 ** -128]
+    x[2, :2] = [1e-45, -1e-45]
+    x[3, :2] = [1e5, 10.0]
+    got = gf.dequantize_fp4_host(gf.quantize_fp4_host(x, 1.0, 32))
+    assert np.array_equal(got, held(x, 1.0, 32)[2].astype(np.float32))
+    got = gf.dequantize_fp4_host(gf.quantize_fp4_host(x, 1.0, 16))
+    assert got[3, 0] == 6 * 448 and got[3, 1] == 0.0 and not got[1].any()
+
+
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_non_finite_block_reads_nan(block, bad):
+    x = np.ones((3, 80), np.float32)
+    x[1, 35] = bad
+    got = gf.dequantize_fp4_host(gf.quantize_fp4_host(x, 1.0, block))
+    want = np.ones((3, 80), bool)
+    want[1, 32:32 + block] = False
+    assert np.array_equal(np.isfinite(got), want)
+    assert np.isnan(got[1, 32:32 + block]).all()
+
+
+def test_empty():
+    r = gf.quantize_fp4_host(np.zeros((0, 7), np.float32))
+    assert r.packed.size == 0 and gf.dequantize_fp4_host(r).shape == (0, 7)
+
+
+def test_size_of_bad_shapes():
+    L = gf.lib()
+    assert L.gf_fp4_bytes(5, 0, 32) == 0 and L.gf_fp4_bytes(5, 8, 8) == 0
+    assert L.gf_fp4_bytes(2 ** 32 - 1, 2 ** 32 - 1, 32) > 2 ** 62
+
+
+@pytest.mark.parametrize("args,word", [
+    (dict(dim=0), b"dim"), (dict(block=64), b"block"), (dict(alpha=0.0), b"alpha"), (dict(alpha=float("nan")), b"alpha"),
+    (dict(alpha=float("inf")), b"alpha"), (dict(alpha=-1.0), b"alpha"), (dict(dtype=3), b"dtype"), (dict(ld=7), b"stride"),
+    (dict(data=0), b"null"), (dict(packed=0), b"null"), (dict(data=64 + 2), b"misaligned"), (dict(packed=64 + 8), b"misaligned"),
+])
+def test_refusals(args, word):
+    """Refused before anything is launched: the pointers are never followed."""
+    a = dict(data=64, dtype=0, ld=8, n=4, dim=8, alpha=1.0, block=32, packed=64)
+    a.update(args)
+    L, P = gf.lib(), ctypes.c_void_p
+    assert L.gf_quantize_fp4(P(a["data"]), a["dtype"], a["ld"], a["n"], a["dim"], a["alpha"], a["block"], P(a["packed"]),
+                             None) == 1
+    assert word in L.gf_last_error()
+    assert L.gf_dequantize_fp4(P(a["packed"]), a["n"], a["dim"], a["block"], a["alpha"], P(a["data"]), a["dtype"], a["ld"],
+                               None) == 1
+    assert word in L.gf_last_error()
+    if {"dim", "block", "alpha"} & set(args):
+        buf = np.zeros(4096 * 4, np.uint8)
+        p = P(buf.ctypes.data)
+        assert L.gf_quantize_fp4_host(p, a["n"], a["dim"], a["alpha"], a["block"], p) == 1
+        assert L.gf_dequantize_fp4_host(p, a["n"], a["dim"], a["block"], a["alpha"], p) == 1
+
+
+def test_python_refusals():
+    import torch
+    with pytest.raises(gf.GarfieldError):
+        gf.quantize_fp4(torch.zeros(4, 8))  # not on a GPU
+    with pytest.raises(gf.GarfieldError):
+        gf.quantize_fp4_host(np.zeros((4, 8), np.float32), block=8)
+    with pytest.raises(gf.GarfieldError):
+        gf.dequantize_fp4(gf.quantize_fp4_host(np.zeros((4, 8), np.float32)))
+    r = gf.quantize_fp4_host(np.zeros((4, 8), np.float32))
+    r.n = 400
+    with pytest.raises(gf.GarfieldError):
+        gf.dequantize_fp4_host(r)

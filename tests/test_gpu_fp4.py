@@ -1,0 +1,149 @@
+"""4-bit block floating point on the GPU: the device quantiser's bytes against the host form's, the values
+read back against the definition in 64 bits, strides, alignments, streams and graphs."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import garfield_b200 as gf
+from test_fp4 import data, held
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def valid_bytes(packed, n, dim, block):
+    """Packed bytes of the rows that exist, as (scales, codes) lists in panel order."""
+    sub = 512 * (32 // block)
+    out = []
+    at = 0
+    for p in range(-(-n // 128)):
+        rows = min(128, n - p * 128)
+        for k in range(0, dim, 128):
+            cols = min(4, -(-(dim - k) // 32))
+            sc = packed[at:at + sub].reshape(-1, 32, 4, 4).transpose(0, 2, 1, 3).reshape(-1, 128, 4)
+            out.append(sc[:, :rows].ravel())
+            out.append(packed[at + sub:at + sub + cols * 2048].reshape(cols, 128, 16)[:, :rows].ravel())
+            at += sub + cols * 2048
+    assert at == packed.size
+    return np.concatenate(out)
+
+
+def same_bytes(rows, ref):
+    assert (rows.n, rows.dim, rows.block) == (ref.n, ref.dim, ref.block)
+    a = valid_bytes(rows.packed.cpu().numpy(), rows.n, rows.dim, rows.block)
+    b = valid_bytes(ref.packed, ref.n, ref.dim, ref.block)
+    assert np.array_equal(a, b), np.flatnonzero(a != b)[:10]
+
+
+SHAPES = [(1, 1), (1, 8192), (3, 96), (64, 31), (127, 32), (128, 128), (130, 33), (300, 300), (1000, 65), (513, 1000)]
+
+
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,dim", SHAPES)
+def test_device_matches_host(n, dim, dtype, block):
+    for kind, alpha in (("normal", 16.0), ("wide", 1.0), ("borders", 1.0), ("normal", 0.3)):
+        x = torch.from_numpy(data(n, dim, n + dim, kind)).to(dtype)
+        same_bytes(gf.quantize_fp4(x.cuda(), alpha, block), gf.quantize_fp4_host(x.float().numpy(), alpha, block))
+
+
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,dim", SHAPES)
+def test_read_back(n, dim, dtype, block):
+    for kind, alpha in (("normal", 16.0), ("wide", 1.0)):
+        x = data(n, dim, n + 3 * dim, kind)
+        got = gf.dequantize_fp4(gf.quantize_fp4(torch.from_numpy(x).cuda(), alpha, block), dtype)
+        want = torch.from_numpy(held(x, alpha, block)[2]).to(torch.float32).to(dtype)  # exact in fp32: alpha is 2^k
+        assert torch.equal(got.cpu(), want)
+    x = data(n, dim, 1, "normal")
+    r = gf.quantize_fp4(torch.from_numpy(x).cuda(), 0.3, block)
+    ref = gf.Fp4Rows(r.packed.cpu().numpy(), n, dim, block, 0.3)
+    assert torch.equal(gf.dequantize_fp4(r, dtype).cpu(), torch.from_numpy(gf.dequantize_fp4_host(ref)).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [33, 96])
+@pytest.mark.parametrize("offset,gap", [(0, 0), (1, 0), (4, 4), (3, 5), (0, 1)])
+def test_strided_rows(dtype, dim, offset, gap):
+    """Rows inside a wider matrix, at any element offset; what lies beside the output is left as it was."""
+    n = 140
+    x = torch.from_numpy(data(n, dim, 9, "normal")).to(dtype).cuda()
+    buf = torch.full((n, offset + dim + gap), float("nan"), dtype=dtype, device="cuda")
+    view = buf[:, offset:offset + dim]
+    view.copy_(x)
+    r = gf.quantize_fp4(view, 1.0, 32)
+    same_bytes(r, gf.quantize_fp4_host(x.float().cpu().numpy(), 1.0, 32))
+    out = torch.full_like(buf, 7.0)
+    got = gf.dequantize_fp4(r, out=out[:, offset:offset + dim])
+    assert torch.equal(got, gf.dequantize_fp4(r, dtype))
+    assert (out[:, :offset] == 7.0).all() and (out[:, offset + dim:] == 7.0).all()
+
+
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan"), -float("inf")])
+def test_non_finite_block_reads_nan(block, bad):
+    x = torch.ones(200, 80, device="cuda")
+    x[131, 35] = bad
+    r = gf.quantize_fp4(x, 1.0, block)
+    same_bytes(r, gf.quantize_fp4_host(x.cpu().numpy(), 1.0, block))
+    got = gf.dequantize_fp4(r)
+    want = torch.ones(200, 80, dtype=torch.bool, device="cuda")
+    want[131, 32:32 + block] = False
+    assert torch.equal(torch.isfinite(got), want)
+
+
+def test_rows_past_the_last_are_left():
+    n, dim = 130, 96
+    x = torch.from_numpy(data(n, dim, 2, "normal")).cuda()
+    size = gf.lib().gf_fp4_bytes(n, dim, 32)
+    packed = torch.full((size + 64,), 0xA5, dtype=torch.uint8, device="cuda")
+    import ctypes
+    gf._check(gf.lib().gf_quantize_fp4(ctypes.c_void_p(x.data_ptr()), 0, dim, n, dim, 1.0, 32,
+                                       ctypes.c_void_p(packed.data_ptr()), gf._stream_ptr(None)), "gf_quantize_fp4")
+    p = packed.cpu().numpy()
+    assert (p[size:] == 0xA5).all()
+    codes = p[size // 2 + 512:size].reshape(3, 128, 16)
+    assert (codes[:, 2:] == 0xA5).all()
+
+
+def test_empty_and_refused():
+    r = gf.quantize_fp4(torch.empty(0, 16, device="cuda"))
+    assert gf.dequantize_fp4(r).shape == (0, 16)
+    x = torch.zeros(8, 16, device="cuda")
+    for bad in (x.t(), x[0], x.double(), x.expand(8, 16)[:, ::2], x[:1].expand(8, 16)):
+        with pytest.raises(gf.GarfieldError):
+            gf.quantize_fp4(bad)
+    with pytest.raises(gf.GarfieldError):
+        gf.quantize_fp4(x, block=64)
+    with pytest.raises(gf.GarfieldError):
+        gf.quantize_fp4(x, alpha=0.0)
+    r = gf.quantize_fp4(x)
+    with pytest.raises(gf.GarfieldError):
+        gf.dequantize_fp4(r, out=torch.zeros(7, 16, device="cuda"))
+    with pytest.raises(gf.GarfieldError):
+        gf.dequantize_fp4(r, dtype=torch.float64)
+    with pytest.raises(gf.GarfieldError):
+        gf.dequantize_fp4(gf.Fp4Rows(r.packed, 400, 16, 32, 1.0))
+
+
+def test_streams_and_graph():
+    x = torch.from_numpy(data(500, 200, 4, "normal")).cuda()
+    want = gf.dequantize_fp4(gf.quantize_fp4(x))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = gf.dequantize_fp4(gf.quantize_fp4(x, stream=side), stream=side)
+    got2 = gf.dequantize_fp4(gf.quantize_fp4(x, stream=side.cuda_stream), stream=side.cuda_stream)
+    side.synchronize()
+    assert torch.equal(got, want) and torch.equal(got2, want)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = gf.dequantize_fp4(gf.quantize_fp4(x))
+    x.mul_(-3.0)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, gf.dequantize_fp4(gf.quantize_fp4(x)))
