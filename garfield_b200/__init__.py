@@ -28,7 +28,7 @@ __all__ = [
     "GarfieldError", "lib", "lib_path", "SearchParams", "Index", "Plan", "NO_ID", "schedule_batches",
     "read_fvecs", "write_fvecs", "read_attrs", "write_attrs", "read_u32mat", "write_u32mat",
     "read_ranges", "write_ranges", "read_labels", "read_grid",
-    "Fp4Rows", "quantize_fp4", "dequantize_fp4", "quantize_fp4_host", "dequantize_fp4_host",
+    "Fp4Rows", "quantize_fp4", "dequantize_fp4", "product_fp4", "quantize_fp4_host", "dequantize_fp4_host",
 ]
 
 NO_ID = 0xFFFFFFFF
@@ -143,6 +143,7 @@ def lib() -> C.CDLL:
         "gf_fp4_bytes": (C.c_uint64, [_U32, _U32, _U32]),
         "gf_quantize_fp4": (C.c_int, [_P, _U32, C.c_uint64, _U32, _U32, C.c_float, _U32, _P, _P]),
         "gf_dequantize_fp4": (C.c_int, [_P, _U32, _U32, _U32, C.c_float, _P, _U32, C.c_uint64, _P]),
+        "gf_product_fp4": (C.c_int, [_P, _U32, _P, _U32, _U32, _U32, C.c_float, _P, _U32, C.c_uint64, _U32, _P]),
         "gf_quantize_fp4_host": (C.c_int, [_P, _U32, _U32, C.c_float, _U32, _P]),
         "gf_dequantize_fp4_host": (C.c_int, [_P, _U32, _U32, _U32, C.c_float, _P]),
         "gf_write_attrs": (C.c_int, [C.c_char_p, _P, _U32, _U32]),
@@ -645,7 +646,33 @@ def dequantize_fp4(rows: Fp4Rows, dtype=None, out=None, stream=None):
     with _on_stream(p.device, stream) as s:
         out = _fp4_out(out, (rows.n, rows.dim), dtype, p.device, what)
         _check(lib().gf_dequantize_fp4(C.c_void_p(p.data_ptr()), rows.n, rows.dim, rows.block, rows.alpha,
-                                       C.c_void_p(out.data_ptr()), dt, max(out.stride(0), rows.dim), s), what)
+                                       C.c_void_p(out.data_ptr()), dt, out.stride(0) if rows.n > 1 else rows.dim, s), what)
+    return out
+
+
+def product_fp4(queries, rows: Fp4Rows, dtype=None, out=None, query_alpha: float = 1.0, stream=None,
+                test_wait: int = 0):
+    """gf_product_fp4: the inner products of every query with every row (m x n, float32 unless dtype or
+    out say otherwise).  queries: Fp4Rows of the same dim and block, or a float32, float16 or
+    bfloat16 CUDA matrix, which is held in 4 bits (quantize_fp4 with query_alpha and the rows'
+    block) for the call."""
+    import torch
+    what = "gf_product_fp4"
+    p = _fp4_rows(rows, what)
+    dtype = dtype or (out.dtype if out is not None else torch.float32)
+    dt = _fp4_dtype(dtype, what)
+    with _on_stream(p.device, stream) as s:
+        if isinstance(queries, torch.Tensor):
+            _fp4_need(queries.device == p.device, what, f"queries on {queries.device}, rows on {p.device}")
+            queries = quantize_fp4(queries, query_alpha, rows.block)
+        qp = _fp4_rows(queries, what)
+        _fp4_need(qp.device == p.device, what, f"queries on {qp.device}, rows on {p.device}")
+        _fp4_need((queries.dim, queries.block) == (rows.dim, rows.block), what,
+                  f"queries of dim {queries.dim}, block {queries.block}; rows of dim {rows.dim}, block {rows.block}")
+        out = _fp4_out(out, (queries.n, rows.n), dtype, p.device, what)
+        _check(lib().gf_product_fp4(C.c_void_p(qp.data_ptr()), queries.n, C.c_void_p(p.data_ptr()), rows.n, rows.dim,
+                                    rows.block, 1.0 / (queries.alpha * rows.alpha), C.c_void_p(out.data_ptr()), dt,
+                                    out.stride(0) if queries.n > 1 and rows.n else rows.n, test_wait, s), what)
     return out
 
 

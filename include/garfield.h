@@ -489,6 +489,19 @@ gf_status gf_dequantize_fp4(const void* packed, uint32_t n, uint32_t dim, uint32
 gf_status gf_quantize_fp4_host(const float* data, uint32_t n, uint32_t dim, float alpha, uint32_t block,
                                void* packed_out);
 gf_status gf_dequantize_fp4_host(const void* packed, uint32_t n, uint32_t dim, uint32_t block, float alpha, float* out);
+/*
+ * Products of rows held in 4 bits: out[i * ld + j] = scale * <q_i, r_j> for the m rows of q_packed and
+ * the n rows of r_packed (same dim and block), the codes and block scales multiplied as they
+ * are held, summed in fp32 on the tensor cores, multiplied by scale in fp32 and rounded to dtype.
+ * scale = 1 / (alpha of q * alpha of r) gives the products of the data; it is finite.  The same
+ * call gives the same bits every time.  out must not overlap the inputs.  Whichever of the two has more rows is best passed as r.
+ * test_wait: 0 in normal use.  Test hook for the timeout path: every wait of the kernel gives up
+ * after test_wait polls and every load expects 16 bytes more than it copies; what a CTA then still
+ * owes of out becomes NaN.
+ */
+gf_status gf_product_fp4(const void* q_packed, uint32_t m, const void* r_packed, uint32_t n, uint32_t dim,
+                         uint32_t block, float scale, void* out, uint32_t dtype, uint64_t ld, uint32_t test_wait,
+                         void* stream);
 
 /* attrs.bin: uint32 n, uint32 a, n*a int32 (tools.cuh:747-765). */
 gf_status gf_read_attrs(const char* path, int32_t** attrs, uint32_t* n, uint32_t* a);

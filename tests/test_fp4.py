@@ -179,3 +179,18 @@ def test_python_refusals():
     r.n = 400
     with pytest.raises(gf.GarfieldError):
         gf.dequantize_fp4_host(r)
+
+
+@pytest.mark.parametrize("args,word", [
+    (dict(dim=0), b"dim"), (dict(block=8), b"block"), (dict(scale=float("nan")), b"scale"),
+    (dict(scale=float("inf")), b"scale"), (dict(dtype=7), b"dtype"), (dict(ld=4), b"stride"), (dict(q=0), b"null"),
+    (dict(r=0), b"null"), (dict(out=0), b"null"), (dict(q=72), b"misaligned"), (dict(r=72), b"misaligned"),
+    (dict(out=66), b"misaligned"),
+])
+def test_product_refusals(args, word):
+    a = dict(q=64, m=3, r=64, n=5, dim=8, block=32, scale=1.0, out=64, dtype=0, ld=5)
+    a.update(args)
+    L, P = gf.lib(), ctypes.c_void_p
+    assert L.gf_product_fp4(P(a["q"]), a["m"], P(a["r"]), a["n"], a["dim"], a["block"], a["scale"], P(a["out"]), a["dtype"],
+                            a["ld"], 0, None) == 1
+    assert word in L.gf_last_error()
