@@ -98,6 +98,13 @@ __device__ __forceinline__ void tmem_wait_ld16(uint32_t* v) {
                  :
                  : "memory");
 }
+// True in one lane of the warp.  Loops and addresses around it stay warp-uniform, so the compiler
+// keeps them in uniform registers, which is what the asynchronous instructions read.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
+}
 // Bounded wait on a phase; false when it ran out or the CTA is stopping.
 __device__ __forceinline__ bool bwait(uint64_t* bar, uint32_t par, const volatile uint32_t* stop, uint32_t polls) {
     for (uint32_t p = 0; p < polls; ++p) {
@@ -168,23 +175,21 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
                 const uint32_t a_bytes = A.Lo.scale_bytes + cols * kFp4ColBytes;
                 const uint32_t pad = cols & 1u;
                 const uint64_t at = (uint64_t)g * A.Lo.group_bytes;
-                if (lane == 0)
+                if (elect_one()) {
                     mbar_arrive_expect_tx(&full[st], a_bytes + np * A.Lo.scale_bytes + cols * rows * 16 + pad * ntc + A.extra_tx);
-                __syncwarp();
-                // lane 0: the panel's group; then one lane per query scale run, per query column piece, and the zeros
-                if (lane == 0) {
                     bulk_g2s(stg, src_r + at, a_bytes, &full[st]);
-                } else if (lane <= np) {
-                    bulk_g2s(stg + A.sfb_off + (lane - 1) * A.Lo.scale_bytes, A.q + (uint64_t)(pq0 + lane - 1) * A.Lo.panel_bytes + at,
-                             A.Lo.scale_bytes, &full[st]);
-                } else if (lane <= np + cols * np) {
-                    const uint32_t j = (lane - np - 1) % np, c = (lane - np - 1) / np;
-                    const uint32_t a = max(q0, (pq0 + j) * kFp4Rows), b = min(q0 + rows, (pq0 + j + 1) * kFp4Rows);
-                    bulk_g2s(stg + A.b_off + c * ntc + (a - q0) * 16,
-                             A.q + (uint64_t)(pq0 + j) * A.Lo.panel_bytes + at + A.Lo.scale_bytes + c * kFp4ColBytes + (a % kFp4Rows) * 16,
-                             (b - a) * 16, &full[st]);
-                } else if (pad && lane == 31) {
-                    bulk_g2s(stg + A.b_off + cols * ntc, g_zero, ntc, &full[st]);
+                    for (uint32_t j = 0; j < np; ++j) {
+                        // the tile's rows of query panel pq0 + j: its scales, then a run of each column
+                        const uint8_t* src = A.q + (uint64_t)(pq0 + j) * A.Lo.panel_bytes + at;
+                        const uint32_t a = max(q0, (pq0 + j) * kFp4Rows), b = min(q0 + rows, (pq0 + j + 1) * kFp4Rows);
+                        bulk_g2s(stg + A.sfb_off + j * A.Lo.scale_bytes, src, A.Lo.scale_bytes, &full[st]);
+                        src += A.Lo.scale_bytes + (a % kFp4Rows) * 16;
+                        unsigned char* dst = stg + A.b_off + (a - q0) * 16;
+#pragma unroll
+                        for (uint32_t c = 0; c < 4; ++c)
+                            if (c < cols) bulk_g2s(dst + c * ntc, src + c * kFp4ColBytes, (b - a) * 16, &full[st]);
+                    }
+                    if (pad) bulk_g2s(stg + A.b_off + cols * ntc, g_zero, ntc, &full[st]);
                 }
                 __syncwarp();
             }
@@ -201,35 +206,38 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         __syncwarp();
     } else if (warp == 1) {
         // -------------------------------------------------------------- MMA warp
-        if (lane == 0) {
-            // E2M1 x E2M1, K-major, N = nt, M = 128, scales UE8M0 (block 32) or UE4M3 (block 16)
-            const uint32_t idesc = (1u << 7) | (1u << 10) | ((A.nt >> 3) << 17) | ((BLOCK == 32 ? 1u : 0u) << 23) | ((128u >> 4) << 24);
-            const uint32_t sf0 = tmem + A.acc * A.nt;
-            bool ok = true;
-            uint32_t i = 0, u = 0;  // stages consumed, tiles done
-            for (uint64_t t = blockIdx.x; t < A.tiles; t += gridDim.x, ++u) {
-                const uint32_t b = u % A.acc;
-                const uint32_t q0 = (uint32_t)(t % A.qtiles) * A.nt, rows = min(A.nt, A.m - q0);
-                const uint32_t np = (q0 + rows - 1) / kFp4Rows - q0 / kFp4Rows + 1;
-                const uint32_t lead = (q0 % kFp4Rows) / 32;  // the tile's first row in its first panel's scales
-                if (u >= A.acc && !(ok = bwait(&tempty[b], ((u / A.acc) - 1) & 1u, stop, A.polls))) break;
+        // E2M1 x E2M1, K-major, N = nt, M = 128, scales UE8M0 (block 32) or UE4M3 (block 16)
+        const uint32_t idesc = (1u << 7) | (1u << 10) | ((A.nt >> 3) << 17) | ((BLOCK == 32 ? 1u : 0u) << 23) | ((128u >> 4) << 24);
+        const uint32_t sf0 = tmem + A.acc * A.nt;
+        constexpr uint32_t kSub = BLOCK == 16 ? 2 : 1;  // scale sub-blocks of a group
+        bool ok = true;
+        uint32_t i = 0, u = 0;  // stages consumed, tiles done
+        for (uint64_t t = blockIdx.x; t < A.tiles; t += gridDim.x, ++u) {
+            const uint32_t b = u % A.acc;
+            const uint32_t q0 = (uint32_t)(t % A.qtiles) * A.nt, rows = min(A.nt, A.m - q0);
+            const uint32_t np = (q0 + rows - 1) / kFp4Rows - q0 / kFp4Rows + 1;
+            const uint32_t lead = (q0 % kFp4Rows) / 32;  // the tile's first row in its first panel's scales
+            if (u >= A.acc && !(ok = __all_sync(kFull, bwait(&tempty[b], ((u / A.acc) - 1) & 1u, stop, A.polls)))) break;
+            tc_fence_after();
+            for (uint32_t g = 0; g < G; ++g, ++i) {
+                const uint32_t st = i % A.stages;
+                if (!(ok = __all_sync(kFull, bwait(&full[st], (i / A.stages) & 1u, stop, A.polls)))) break;
                 tc_fence_after();
-                for (uint32_t g = 0; g < G; ++g, ++i) {
-                    const uint32_t st = i % A.stages;
-                    if (!(ok = bwait(&full[st], (i / A.stages) & 1u, stop, A.polls))) break;
-                    tc_fence_after();
-                    const uint32_t stg = smem_u32(sm + st * A.stage_bytes);
-                    const uint32_t steps = ((g + 1 == G ? A.Lo.last_cols : 4u) + 1) / 2;
-                    constexpr uint32_t kSub = BLOCK == 16 ? 2 : 1;  // scale sub-blocks of a group
-                    // this stage's scales; its slot was last read by MMAs that the stage's empty barrier covers
-                    const uint32_t sfa = sf0 + st * A.sf_cols, sfb = sfa + 4 * kSub;
+                const uint32_t stg = smem_u32(sm + st * A.stage_bytes);
+                const uint32_t cols = g + 1 == G ? A.Lo.last_cols : 4u;
+                // this stage's scales; their slot was last read by MMAs that the stage's empty barrier covers
+                const uint32_t sfa = sf0 + st * A.sf_cols, sfb = sfa + 4 * kSub;
+                const uint32_t a0 = stg + A.Lo.scale_bytes, b0 = stg + A.b_off;
+                if (elect_one()) {
+#pragma unroll
                     for (uint32_t h = 0; h < kSub; ++h) {
                         scales_to_tmem(sfa + h * 4, stg + h * kFp4ScaleSub);
                         for (uint32_t j = 0; j < np; ++j)
                             scales_to_tmem(sfb + (h * A.npan + j) * 4, stg + A.sfb_off + j * A.Lo.scale_bytes + h * kFp4ScaleSub);
                     }
-                    const uint32_t a0 = stg + A.Lo.scale_bytes, b0 = stg + A.b_off;
-                    for (uint32_t s = 0; s < steps; ++s) {
+#pragma unroll
+                    for (uint32_t s = 0; s < 2; ++s) {
+                        if (s * 2 >= cols) break;
                         const uint64_t ad = smem_desc(a0 + s * 2 * kFp4ColBytes, kFp4ColBytes, 128);
                         const uint64_t bd = smem_desc(b0 + s * 2 * ntc, ntc, 128);
                         // block 16: step s uses sub-block s; block 32: bytes 2s, 2s + 1 of the one sub-block
@@ -238,18 +246,20 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
                         mma_fp4<BLOCK>(tmem + b * A.nt, ad, bd, id, sfa + h * 4, sfb + h * A.npan * 4 + lead, (g | s) ? 1u : 0u);
                     }
                     mma_commit(&empty[st]);  // the stage is free once these MMAs have read it
+                    if (g + 1 == G) mma_commit(&tfull[b]);
                 }
-                if (!ok) break;
-                mma_commit(&tfull[b]);
+                __syncwarp();
             }
-            if (!ok) *stop = 1u;
-            // every MMA has completed before TMEM is released
-            mma_commit(drain);
-            uint32_t p = 0;
-            while (!mbar_try_wait(drain, 0, 1000) && ++p < A.polls) {
-            }
-            if (p >= A.polls) *stop = 1u;
+            if (!ok) break;
         }
+        if (!ok) *stop = 1u;
+        // every MMA has completed before TMEM is released
+        if (elect_one()) mma_commit(drain);
+        __syncwarp();
+        uint32_t p = 0;
+        while (!mbar_try_wait(drain, 0, 1000) && ++p < A.polls) {
+        }
+        if (p >= A.polls) *stop = 1u;
         __syncwarp();
     } else {
         // -------------------------------------------------------------- epilogue warps
