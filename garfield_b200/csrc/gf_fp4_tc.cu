@@ -114,6 +114,17 @@ __device__ __forceinline__ bool bwait(uint64_t* bar, uint32_t par, const volatil
     return false;
 }
 
+// Position in a ring of barriers: slot and the parity of its current use.
+struct Ring {
+    uint32_t i = 0, par = 0;
+    __device__ __forceinline__ void next(uint32_t n) {
+        if (++i == n) {
+            i = 0;
+            par ^= 1u;
+        }
+    }
+};
+
 __device__ __forceinline__ void store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
@@ -158,18 +169,17 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
     if (warp == 0) {
         // -------------------------------------------------------------- producer warp
         bool ok = true;
-        uint32_t i = 0;  // stages filled
+        Ring ring;
+        uint64_t filled = 0;
         for (uint64_t t = blockIdx.x; ok && t < A.tiles; t += gridDim.x) {
             const uint32_t panel = (uint32_t)(t / A.qtiles), q0 = (uint32_t)(t % A.qtiles) * A.nt;
             const uint32_t rows = min(A.nt, A.m - q0);
             const uint32_t pq0 = q0 / kFp4Rows, np = (q0 + rows - 1) / kFp4Rows - pq0 + 1;  // query panels of the tile
             const uint8_t* src_r = A.r + panel * A.Lo.panel_bytes;
-            for (uint32_t g = 0; g < G; ++g, ++i) {
-                const uint32_t st = i % A.stages;
-                if (i >= A.stages) {
-                    ok = __all_sync(kFull, bwait(&empty[st], ((i / A.stages) - 1) & 1u, stop, A.polls));
-                    if (!ok) break;
-                }
+            for (uint32_t g = 0; g < G; ++g, ring.next(A.stages), ++filled) {
+                const uint32_t st = ring.i;
+                // (a barrier's first wait, for the use before its first, returns at once)
+                if (!(ok = __all_sync(kFull, bwait(&empty[st], ring.par ^ 1u, stop, A.polls)))) break;
                 unsigned char* stg = sm + st * A.stage_bytes;
                 const uint32_t cols = g + 1 == G ? A.Lo.last_cols : 4u;
                 const uint32_t a_bytes = A.Lo.scale_bytes + cols * kFp4ColBytes;
@@ -197,10 +207,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         if (!ok) *stop = 1u;
         // every copy issued lands before the CTA exits (in normal operation they completed long ago)
         if (lane == 0)
-            for (uint32_t st = 0; st < A.stages && st < i; ++st) {
-                const uint32_t last = st + ((i - 1 - st) / A.stages) * A.stages;
+            for (uint32_t st = 0; st < A.stages && st < filled; ++st) {
+                const uint32_t use = (uint32_t)((filled - 1 - st) / A.stages);  // the slot's last
                 uint32_t p = 0;
-                while (!mbar_try_wait(&full[st], (last / A.stages) & 1u, 1000) && ++p < A.polls) {
+                while (!mbar_try_wait(&full[st], use & 1u, 1000) && ++p < A.polls) {
                 }
             }
         __syncwarp();
@@ -211,17 +221,17 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         const uint32_t sf0 = tmem + A.acc * A.nt;
         constexpr uint32_t kSub = BLOCK == 16 ? 2 : 1;  // scale sub-blocks of a group
         bool ok = true;
-        uint32_t i = 0, u = 0;  // stages consumed, tiles done
-        for (uint64_t t = blockIdx.x; t < A.tiles; t += gridDim.x, ++u) {
-            const uint32_t b = u % A.acc;
+        Ring ring, accs;
+        for (uint64_t t = blockIdx.x; t < A.tiles; t += gridDim.x, accs.next(A.acc)) {
+            const uint32_t b = accs.i;
             const uint32_t q0 = (uint32_t)(t % A.qtiles) * A.nt, rows = min(A.nt, A.m - q0);
             const uint32_t np = (q0 + rows - 1) / kFp4Rows - q0 / kFp4Rows + 1;
             const uint32_t lead = (q0 % kFp4Rows) / 32;  // the tile's first row in its first panel's scales
-            if (u >= A.acc && !(ok = __all_sync(kFull, bwait(&tempty[b], ((u / A.acc) - 1) & 1u, stop, A.polls)))) break;
+            if (!(ok = __all_sync(kFull, bwait(&tempty[b], accs.par ^ 1u, stop, A.polls)))) break;
             tc_fence_after();
-            for (uint32_t g = 0; g < G; ++g, ++i) {
-                const uint32_t st = i % A.stages;
-                if (!(ok = __all_sync(kFull, bwait(&full[st], (i / A.stages) & 1u, stop, A.polls)))) break;
+            for (uint32_t g = 0; g < G; ++g, ring.next(A.stages)) {
+                const uint32_t st = ring.i;
+                if (!(ok = __all_sync(kFull, bwait(&full[st], ring.par, stop, A.polls)))) break;
                 tc_fence_after();
                 const uint32_t stg = smem_u32(sm + st * A.stage_bytes);
                 const uint32_t cols = g + 1 == G ? A.Lo.last_cols : 4u;
@@ -267,14 +277,15 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         T* out = static_cast<T*>(A.out);
         bool ok = true;
         uint32_t u = 0;
-        for (uint64_t t = blockIdx.x; t < A.tiles; t += gridDim.x, ++u) {
+        Ring accs;
+        for (uint64_t t = blockIdx.x; t < A.tiles; t += gridDim.x, ++u, accs.next(A.acc)) {
             if (!split && (u & 1u) != h) continue;
-            const uint32_t b = u % A.acc;
+            const uint32_t b = accs.i;
             const uint32_t panel = (uint32_t)(t / A.qtiles), q0 = (uint32_t)(t % A.qtiles) * A.nt;
             const uint32_t rows = min(A.nt, A.m - q0);
             const uint64_t j = (uint64_t)panel * kFp4Rows + qq * 32 + lane;
             if (ok) {
-                ok = __all_sync(kFull, bwait(&tfull[b], (u / A.acc) & 1u, stop, A.polls));
+                ok = __all_sync(kFull, bwait(&tfull[b], accs.par, stop, A.polls));
                 tc_fence_after();
             }
             T* dst = out + q0 * A.ld + j;
