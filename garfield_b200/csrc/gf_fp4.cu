@@ -154,7 +154,8 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const T* __restr
         for (uint32_t i = threadIdx.x; i < cols * kFp4Rows; i += kThreads) {
             const uint32_t c = i / kFp4Rows, r = i % kFp4Rows;
             if (r < valid)
-                reinterpret_cast<uint4*>(dst + kSb)[i] = *reinterpret_cast<const uint4*>(codes_s + c * kColPitch + r * 16);
+                *reinterpret_cast<uint4*>(dst + kSb + c * Lo.col_bytes + r * 16) =
+                    *reinterpret_cast<const uint4*>(codes_s + c * kColPitch + r * 16);
         }
         __syncthreads();
     }
@@ -183,7 +184,8 @@ __global__ void __launch_bounds__(kThreads) fp4_dequantize_kernel(const uint8_t*
         for (uint32_t i = threadIdx.x; i < cols * kFp4Rows; i += kThreads) {
             const uint32_t c = i / kFp4Rows, r = i % kFp4Rows;
             if (r < valid)
-                *reinterpret_cast<uint4*>(codes_s + c * kColPitch + r * 16) = reinterpret_cast<const uint4*>(src + kSb)[i];
+                *reinterpret_cast<uint4*>(codes_s + c * kColPitch + r * 16) =
+                    *reinterpret_cast<const uint4*>(src + kSb + c * Lo.col_bytes + r * 16);
         }
         __syncthreads();
         if (k < dim) {
@@ -243,7 +245,7 @@ float scale_host(uint32_t b, uint32_t block) {
 }
 
 void quantize_host(const float* data, uint32_t n, uint32_t dim, float alpha, uint32_t block, uint8_t* packed) {
-    const Fp4Layout Lo = fp4_layout(dim, block);
+    const Fp4Layout Lo = fp4_layout(n, dim, block);
     std::memset(packed, 0, Lo.panel_bytes * fp4_panels(n));
     for (uint32_t i = 0; i < n; ++i)
         for (uint32_t k0 = 0; k0 < dim; k0 += block) {
@@ -274,19 +276,19 @@ void quantize_host(const float* data, uint32_t n, uint32_t dim, float alpha, uin
                 // block 32: multiplied by 1 / s, a power of two that fp32 holds for every s
                 const float y = block == 16 ? x[k] * alpha / s : std::ldexp(x[k] * alpha, 127 - (int)s8);
                 const uint32_t kg = k % kFp4Group;
-                uint8_t* b = grp + Lo.scale_bytes + (kg / kFp4Col) * kFp4ColBytes + r * 16 + (kg % kFp4Col) / 2;
+                uint8_t* b = grp + Lo.scale_bytes + (kg / kFp4Col) * Lo.col_bytes + r * 16 + (kg % kFp4Col) / 2;
                 *b = (uint8_t)(*b | e2m1_host(y) << (4 * (k & 1u)));
             }
         }
 }
 
 void dequantize_host(const uint8_t* packed, uint32_t n, uint32_t dim, uint32_t block, float alpha, float* out) {
-    const Fp4Layout Lo = fp4_layout(dim, block);
+    const Fp4Layout Lo = fp4_layout(n, dim, block);
     for (uint32_t i = 0; i < n; ++i)
         for (uint32_t k = 0; k < dim; ++k) {
             const uint32_t r = i % kFp4Rows, kg = k % kFp4Group;
             const uint8_t* grp = packed + (i / kFp4Rows) * Lo.panel_bytes + (uint64_t)(k / kFp4Group) * Lo.group_bytes;
-            const uint32_t b = grp[Lo.scale_bytes + (kg / kFp4Col) * kFp4ColBytes + r * 16 + (kg % kFp4Col) / 2];
+            const uint32_t b = grp[Lo.scale_bytes + (kg / kFp4Col) * Lo.col_bytes + r * 16 + (kg % kFp4Col) / 2];
             const uint32_t c = (b >> (4 * (k & 1u))) & 15u;
             const float s = scale_host(grp[fp4_scale_at(r, kg / block)], block) / alpha;
             out[(uint64_t)i * dim + k] = (c & 8u ? -kMags[c & 7u] : kMags[c & 7u]) * s;
@@ -301,7 +303,7 @@ unsigned grid_of(uint64_t tiles) { return (unsigned)std::min<uint64_t>(tiles, 0x
 
 template <typename T, uint32_t BLOCK>
 void launch_quantize(const void* data, uint64_t ld, uint32_t n, uint32_t dim, float alpha, uint8_t* packed, cudaStream_t s) {
-    const Fp4Layout Lo = fp4_layout(dim, BLOCK);
+    const Fp4Layout Lo = fp4_layout(n, dim, BLOCK);
     const uint64_t tiles = (uint64_t)fp4_panels(n) * Lo.groups;
     const T* x = static_cast<const T*>(data);
     if (aligned(data, 4 * sizeof(T)) && ld % 4 == 0 && dim % 4 == 0)
@@ -311,7 +313,7 @@ void launch_quantize(const void* data, uint64_t ld, uint32_t n, uint32_t dim, fl
 }
 template <typename T, uint32_t BLOCK>
 void launch_dequantize(const uint8_t* packed, uint32_t n, uint32_t dim, float alpha, void* out, uint64_t ld, cudaStream_t s) {
-    const Fp4Layout Lo = fp4_layout(dim, BLOCK);
+    const Fp4Layout Lo = fp4_layout(n, dim, BLOCK);
     const uint64_t tiles = (uint64_t)fp4_panels(n) * Lo.groups;
     T* y = static_cast<T*>(out);
     if (aligned(out, 4 * sizeof(T)) && ld % 4 == 0 && dim % 4 == 0)
@@ -328,7 +330,7 @@ using namespace gf;
 
 extern "C" uint64_t gf_fp4_bytes(uint32_t n, uint32_t dim, uint32_t block) {
     if (!fp4_shape(dim, block)) return 0;
-    return fp4_layout(dim, block).panel_bytes * fp4_panels(n);
+    return fp4_layout(n, dim, block).panel_bytes * fp4_panels(n);
 }
 
 extern "C" gf_status gf_quantize_fp4(const void* data, uint32_t dtype, uint64_t ld, uint32_t n, uint32_t dim, float alpha,

@@ -1,16 +1,16 @@
 // Layout of rows held in 4-bit block floating point (gf_fp4.cu, gf_fp4_tc.cu).
 //
-// Rows are cut into panels of 128 and their elements into groups of 128.  A panel holds its
-// groups in order; a group is
+// Rows are cut into panels of 128 (fewer than 128 rows: one panel of their number rounded up to 16)
+// and their elements into groups of 128.  A panel of h rows holds its groups in order; a group is
 //   scales   128 rows x (128 / block) bytes, as `128 / (4 block)` sub-blocks of 512 bytes: byte b
 //            of row r in a sub-block (4 consecutive blocks b of the row) is at
 //            (r % 32) * 16 + (r / 32) * 4 + b -- the order in which one tcgen05.cp (32x128b,
 //            warpx4) spreads the scales of 128 rows over 4 TMEM columns
-//   codes    columns of 32 elements; a column is 128 rows x 16 bytes, row r at r * 16, element
+//   codes    columns of 32 elements; a column is h rows x 16 bytes, row r at r * 16, element
 //            2i in the low half of byte i -- 8 rows of a column are one tcgen05 core matrix
 //            (K-major, no swizzle), so a column needs no rearranging between HBM and the MMA
-// The last group of a row holds only the columns that have elements.  Every byte of a group is
-// contiguous, so one bulk copy brings a group of a panel into shared memory.  Codes and scales
+// The last group of a row holds only the columns that have elements.  Every byte of a panel is
+// contiguous, so one bulk copy brings a group, or several, into shared memory.  Codes and scales
 // past the end of a row are 0; what stands in the rows past n of the last panel is unspecified
 // (a row's bytes reach only that row's outputs).
 #pragma once
@@ -24,20 +24,22 @@ namespace gf {
 constexpr uint32_t kFp4Rows = 128;              // rows of a panel
 constexpr uint32_t kFp4Group = 128;             // elements of a group
 constexpr uint32_t kFp4Col = 32;                // elements of a column
-constexpr uint32_t kFp4ColBytes = kFp4Rows * 16;
+constexpr uint32_t kFp4ColBytes = kFp4Rows * 16;  // a column of a full panel
 constexpr uint32_t kFp4ScaleSub = 512;          // bytes of one scale sub-block
 
 struct Fp4Layout {
-    uint32_t groups, last_cols, scale_bytes, group_bytes;
+    uint32_t groups, last_cols, scale_bytes, col_bytes, group_bytes, last_bytes;
     uint64_t panel_bytes;
 };
-__host__ __device__ inline Fp4Layout fp4_layout(uint32_t dim, uint32_t block) {
+__host__ __device__ inline Fp4Layout fp4_layout(uint32_t n, uint32_t dim, uint32_t block) {
     Fp4Layout L;
+    L.col_bytes = (n < kFp4Rows ? (n + 15) / 16 * 16 : kFp4Rows) * 16;
     L.groups = (uint32_t)(((uint64_t)dim + kFp4Group - 1) / kFp4Group);
     L.last_cols = (uint32_t)((dim - (uint64_t)(L.groups - 1) * kFp4Group + kFp4Col - 1) / kFp4Col);
     L.scale_bytes = block == 16 ? 2 * kFp4ScaleSub : kFp4ScaleSub;
-    L.group_bytes = L.scale_bytes + kFp4Group / kFp4Col * kFp4ColBytes;
-    L.panel_bytes = (uint64_t)(L.groups - 1) * L.group_bytes + L.scale_bytes + (uint64_t)L.last_cols * kFp4ColBytes;
+    L.group_bytes = L.scale_bytes + kFp4Group / kFp4Col * L.col_bytes;
+    L.last_bytes = L.scale_bytes + L.last_cols * L.col_bytes;
+    L.panel_bytes = (uint64_t)(L.groups - 1) * L.group_bytes + L.last_bytes;
     return L;
 }
 __host__ __device__ inline uint32_t fp4_panels(uint32_t n) { return (uint32_t)(((uint64_t)n + kFp4Rows - 1) / kFp4Rows); }

@@ -6,10 +6,12 @@
 // The rows r are the M side (128 rows of a panel = 128 TMEM lanes), the queries q the N side, so
 // an accumulator's lanes are consecutive j: a warp's store of one column is a contiguous
 // run of out, whatever the number of queries, and few queries cost few columns.  A CTA walks tiles
-// (panel, nt queries), queries fastest, so a panel's bytes leave HBM once.  Warp 0 copies, per group of
-// 128 elements, the panel's group (one run) and the query columns and scales into a ring of stages;
-// one thread of warp 1 spreads the scales into TMEM (tcgen05.cp) and issues the
-// group's two MMAs (64 elements each); eight warps read finished accumulators and write out.
+// (pb panels, a panel of queries), queries fastest, so a panel's bytes leave HBM once.  Warp 0
+// copies the panels' groups and the query panel's, one run each, into a ring of stages; warp 1
+// spreads the scales into TMEM (tcgen05.cp) and issues two MMAs of 64 elements per panel and
+// group; eight warps read finished accumulators and write out.  A stage holds two groups of a
+// panel or, for rows of one group, up to four panels: an asynchronous copy costs its issuing warp some 80
+// cycles, and at the HBM rate a group of a panel passes in 200.
 //
 // Every wait is bounded.  When one runs out the CTA stops and the outputs it still owes become NaN.
 #include <cuda_bf16.h>
@@ -28,22 +30,23 @@ using namespace dev;
 constexpr uint32_t kThreads = 320;    // producer warp, MMA warp, 8 epilogue warps
 constexpr uint32_t kMaxStages = 8;
 constexpr uint32_t kMaxAcc = 8;
-constexpr uint32_t kMaxNt = 256;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kPolls = 1u << 20;
 constexpr uint32_t kSmemLimit = 227 * 1024;
 
-// Zeros for the second column of an MMA step that the row's last group lacks: with zero codes on the
-// query side, what the other side's column holds from earlier stages adds nothing.
-__device__ __align__(16) uint8_t g_zero[kMaxNt * 16];
+// Zeros for the second column of an MMA step that the rows' last group lacks: with zero codes on the
+// query side, whatever codes stand in the other side's place add nothing.
+__device__ __align__(16) uint8_t g_zero[kFp4ColBytes];
 
 struct ProdArgs {
     const uint8_t *r, *q;
-    Fp4Layout Lo;
-    uint32_t m, n, nt, acc, stages, qtiles;
-    uint32_t stage_bytes, b_off, sfb_off;  // within a stage: query columns, query scales (the panel's group is at 0)
-    uint32_t npan;                         // query panels a tile can touch
-    uint32_t sf_cols;                      // TMEM columns of one stage's scales
+    Fp4Layout Lr, Lq;
+    uint32_t m, n, panels, qtiles;
+    uint32_t nt;                        // columns of an accumulator: the rows of a query panel
+    uint32_t pb, gs;                    // panels of a tile and groups of a stage (one of them 1)
+    uint32_t acc, stages, stage_bytes;
+    uint32_t b_off;                     // within a stage: the query panel's groups (the row panels' are at 0)
+    uint32_t sf_cols;                   // TMEM columns of one stage's scales
     uint64_t tiles;
     void* out;
     uint64_t ld;
@@ -132,6 +135,8 @@ __device__ __forceinline__ void store(__nv_bfloat16* p, float v) { *p = __float2
 template <typename T, uint32_t BLOCK>
 __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_constant__ ProdArgs A) {
     extern __shared__ __align__(1024) unsigned char sm[];
+    constexpr uint32_t kSub = BLOCK == 16 ? 2 : 1;  // scale sub-blocks of a group
+    constexpr uint32_t kItems = 4;                  // (panel, group) pairs of a stage, at most
     uint64_t* full = reinterpret_cast<uint64_t*>(sm + A.stages * A.stage_bytes);
     uint64_t* empty = full + kMaxStages;
     uint64_t* tfull = empty + kMaxStages;
@@ -140,7 +145,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile uint32_t* stop = tmem_slot + 1;
     const uint32_t warp = threadIdx.x >> 5, lane = lane_id();
-    const bool split = A.nt >= 64;  // both epilogue halves share a tile's columns, else they take alternate tiles
+    const uint32_t cpp = A.nt / 16;     // 16-column chunks of a panel's accumulator
+    const bool split = A.pb * cpp > 1;  // both epilogue halves share a tile's chunks, else they take alternate tiles
 
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
@@ -164,44 +170,37 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const uint32_t G = A.Lo.groups, ntc = A.nt * 16;
+    const uint32_t G = A.Lr.groups;
 
     if (warp == 0) {
         // -------------------------------------------------------------- producer warp
         bool ok = true;
         Ring ring;
         uint64_t filled = 0;
+        const uint32_t pad = (A.Lq.last_cols & 1u) * A.nt * 16;  // bytes of the zero column of the last group
         for (uint64_t t = blockIdx.x; ok && t < A.tiles; t += gridDim.x) {
-            const uint32_t panel = (uint32_t)(t / A.qtiles), q0 = (uint32_t)(t % A.qtiles) * A.nt;
-            const uint32_t rows = min(A.nt, A.m - q0);
-            const uint32_t pq0 = q0 / kFp4Rows, np = (q0 + rows - 1) / kFp4Rows - pq0 + 1;  // query panels of the tile
-            const uint8_t* src_r = A.r + panel * A.Lo.panel_bytes;
-            for (uint32_t g = 0; g < G; ++g, ring.next(A.stages), ++filled) {
-                const uint32_t st = ring.i;
+            const uint32_t p0 = (uint32_t)(t / A.qtiles) * A.pb, qt = (uint32_t)(t % A.qtiles);
+            const uint32_t np = min(A.pb, A.panels - p0);
+            const uint8_t* src_r = A.r + p0 * A.Lr.panel_bytes;
+            const uint8_t* src_q = A.q + qt * A.Lq.panel_bytes;
+            for (uint32_t g = 0; g < G; g += A.gs, ring.next(A.stages), ++filled) {
                 // (a barrier's first wait, for the use before its first, returns at once)
-                if (!(ok = __all_sync(kFull, bwait(&empty[st], ring.par ^ 1u, stop, A.polls)))) break;
-                unsigned char* stg = sm + st * A.stage_bytes;
-                const uint32_t cols = g + 1 == G ? A.Lo.last_cols : 4u;
-                const uint32_t a_bytes = A.Lo.scale_bytes + cols * kFp4ColBytes;
-                const uint32_t pad = cols & 1u;
-                const uint64_t at = (uint64_t)g * A.Lo.group_bytes;
+                if (!(ok = __all_sync(kFull, bwait(&empty[ring.i], ring.par ^ 1u, stop, A.polls)))) break;
+                unsigned char* stg = sm + ring.i * A.stage_bytes;
+                uint64_t* bar = &full[ring.i];
+                const bool last = g + A.gs >= G;
+                const uint32_t whole = last ? G - 1 - g : A.gs;  // full groups of the stage
+                const uint32_t a_bytes = (whole * A.Lr.group_bytes + (last ? A.Lr.last_bytes : 0u)) * np;
+                const uint32_t b_bytes = whole * A.Lq.group_bytes + (last ? A.Lq.last_bytes : 0u);
                 if (elect_one()) {
-                    mbar_arrive_expect_tx(&full[st], a_bytes + np * A.Lo.scale_bytes + cols * rows * 16 + pad * ntc + A.extra_tx);
-                    bulk_g2s(stg, src_r + at, a_bytes, &full[st]);
-                    for (uint32_t j = 0; j < np; ++j) {
-                        // the tile's rows of query panel pq0 + j: its scales, then a run of each column
-                        const uint8_t* src = A.q + (uint64_t)(pq0 + j) * A.Lo.panel_bytes + at;
-                        const uint32_t a = max(q0, (pq0 + j) * kFp4Rows), b = min(q0 + rows, (pq0 + j + 1) * kFp4Rows);
-                        bulk_g2s(stg + A.sfb_off + j * A.Lo.scale_bytes, src, A.Lo.scale_bytes, &full[st]);
-                        src += A.Lo.scale_bytes + (a % kFp4Rows) * 16;
-                        unsigned char* dst = stg + A.b_off + (a - q0) * 16;
-#pragma unroll
-                        for (uint32_t c = 0; c < 4; ++c)
-                            if (c < cols) bulk_g2s(dst + c * ntc, src + c * kFp4ColBytes, (b - a) * 16, &full[st]);
-                    }
-                    if (pad) bulk_g2s(stg + A.b_off + cols * ntc, g_zero, ntc, &full[st]);
+                    mbar_arrive_expect_tx(bar, a_bytes + b_bytes + (last ? pad : 0u) + A.extra_tx);
+                    bulk_g2s(stg, src_r, a_bytes, bar);
+                    bulk_g2s(stg + A.b_off, src_q, b_bytes, bar);
+                    if (last && pad) bulk_g2s(stg + A.b_off + b_bytes, g_zero, pad, bar);
                 }
                 __syncwarp();
+                src_r += a_bytes;
+                src_q += b_bytes;
             }
         }
         if (!ok) *stop = 1u;
@@ -218,45 +217,50 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         // -------------------------------------------------------------- MMA warp
         // E2M1 x E2M1, K-major, N = nt, M = 128, scales UE8M0 (block 32) or UE4M3 (block 16)
         const uint32_t idesc = (1u << 7) | (1u << 10) | ((A.nt >> 3) << 17) | ((BLOCK == 32 ? 1u : 0u) << 23) | ((128u >> 4) << 24);
-        const uint32_t sf0 = tmem + A.acc * A.nt;
-        constexpr uint32_t kSub = BLOCK == 16 ? 2 : 1;  // scale sub-blocks of a group
+        const uint32_t acc_cols = A.pb * A.nt, sf0 = tmem + A.acc * acc_cols;
+        const uint32_t a_item = A.pb > 1 ? (uint32_t)A.Lr.panel_bytes : A.Lr.group_bytes;
+        const uint64_t ad0 = smem_desc(0, A.Lr.col_bytes, 128), bd0 = smem_desc(0, A.Lq.col_bytes, 128);
         bool ok = true;
         Ring ring, accs;
         for (uint64_t t = blockIdx.x; t < A.tiles; t += gridDim.x, accs.next(A.acc)) {
-            const uint32_t b = accs.i;
-            const uint32_t q0 = (uint32_t)(t % A.qtiles) * A.nt, rows = min(A.nt, A.m - q0);
-            const uint32_t np = (q0 + rows - 1) / kFp4Rows - q0 / kFp4Rows + 1;
-            const uint32_t lead = (q0 % kFp4Rows) / 32;  // the tile's first row in its first panel's scales
-            if (!(ok = __all_sync(kFull, bwait(&tempty[b], accs.par ^ 1u, stop, A.polls)))) break;
+            const uint32_t np = min(A.pb, A.panels - (uint32_t)(t / A.qtiles) * A.pb);
+            const uint32_t d0 = tmem + accs.i * acc_cols;
+            if (!(ok = __all_sync(kFull, bwait(&tempty[accs.i], accs.par ^ 1u, stop, A.polls)))) break;
             tc_fence_after();
-            for (uint32_t g = 0; g < G; ++g, ring.next(A.stages)) {
-                const uint32_t st = ring.i;
-                if (!(ok = __all_sync(kFull, bwait(&full[st], ring.par, stop, A.polls)))) break;
+            for (uint32_t g = 0; g < G; g += A.gs, ring.next(A.stages)) {
+                if (!(ok = __all_sync(kFull, bwait(&full[ring.i], ring.par, stop, A.polls)))) break;
                 tc_fence_after();
-                const uint32_t stg = smem_u32(sm + st * A.stage_bytes);
-                const uint32_t cols = g + 1 == G ? A.Lo.last_cols : 4u;
+                const uint32_t stg = smem_u32(sm) + ring.i * A.stage_bytes;
+                const uint32_t items = A.pb > 1 ? np : min(A.gs, G - g);
                 // this stage's scales; their slot was last read by MMAs that the stage's empty barrier covers
-                const uint32_t sfa = sf0 + st * A.sf_cols, sfb = sfa + 4 * kSub;
-                const uint32_t a0 = stg + A.Lo.scale_bytes, b0 = stg + A.b_off;
+                const uint32_t sfa = sf0 + ring.i * A.sf_cols, sfb = sfa + A.pb * A.gs * 4 * kSub;
                 if (elect_one()) {
 #pragma unroll
-                    for (uint32_t h = 0; h < kSub; ++h) {
-                        scales_to_tmem(sfa + h * 4, stg + h * kFp4ScaleSub);
-                        for (uint32_t j = 0; j < np; ++j)
-                            scales_to_tmem(sfb + (h * A.npan + j) * 4, stg + A.sfb_off + j * A.Lo.scale_bytes + h * kFp4ScaleSub);
-                    }
+                    for (uint32_t x = 0; x < kItems; ++x) {
+                        if (x >= items) break;
+                        const uint32_t gx = A.pb > 1 ? 0 : x;  // group of the stage
+                        const uint32_t as = stg + x * a_item, bs = stg + A.b_off + gx * A.Lq.group_bytes;
+                        const uint32_t sa = sfa + x * 4 * kSub, sb = sfb + gx * 4 * kSub;
 #pragma unroll
-                    for (uint32_t s = 0; s < 2; ++s) {
-                        if (s * 2 >= cols) break;
-                        const uint64_t ad = smem_desc(a0 + s * 2 * kFp4ColBytes, kFp4ColBytes, 128);
-                        const uint64_t bd = smem_desc(b0 + s * 2 * ntc, ntc, 128);
-                        // block 16: step s uses sub-block s; block 32: bytes 2s, 2s + 1 of the one sub-block
-                        const uint32_t id = BLOCK == 16 ? idesc : idesc | (2 * s) << 4 | (2 * s) << 29;
-                        const uint32_t h = BLOCK == 16 ? s : 0;
-                        mma_fp4<BLOCK>(tmem + b * A.nt, ad, bd, id, sfa + h * 4, sfb + h * A.npan * 4 + lead, (g | s) ? 1u : 0u);
+                        for (uint32_t h = 0; h < kSub; ++h) {
+                            scales_to_tmem(sa + h * 4, as + h * kFp4ScaleSub);
+                            if (x == 0 || A.pb == 1) scales_to_tmem(sb + h * 4, bs + h * kFp4ScaleSub);
+                        }
+                        const uint32_t cols = g + gx + 1 == G ? A.Lr.last_cols : 4u;
+                        const uint32_t d = A.pb > 1 ? d0 + x * A.nt : d0;
+#pragma unroll
+                        for (uint32_t s = 0; s < 2; ++s) {
+                            if (s * 2 >= cols) break;
+                            const uint64_t ad = ad0 + ((as + kSub * kFp4ScaleSub + s * 2 * A.Lr.col_bytes) >> 4);
+                            const uint64_t bd = bd0 + ((bs + kSub * kFp4ScaleSub + s * 2 * A.Lq.col_bytes) >> 4);
+                            // block 16: step s uses sub-block s; block 32: bytes 2s, 2s + 1 of the one sub-block
+                            const uint32_t id = BLOCK == 16 ? idesc : idesc | (2 * s) << 4 | (2 * s) << 29;
+                            const uint32_t h = BLOCK == 16 ? s * 4 : 0;
+                            mma_fp4<BLOCK>(d, ad, bd, id, sa + h, sb + h, (g + gx) | s ? 1u : 0u);
+                        }
                     }
-                    mma_commit(&empty[st]);  // the stage is free once these MMAs have read it
-                    if (g + 1 == G) mma_commit(&tfull[b]);
+                    mma_commit(&empty[ring.i]);  // the stage is free once these MMAs have read it
+                    if (g + A.gs >= G) mma_commit(&tfull[accs.i]);
                 }
                 __syncwarp();
             }
@@ -273,37 +277,52 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         __syncwarp();
     } else {
         // -------------------------------------------------------------- epilogue warps
+        constexpr uint32_t kBatch = 4;  // chunks read before any is stored
         const uint32_t qq = warp & 3u, h = (warp - 2) >> 2;  // lane quarter, half
+        const uint32_t acc_cols = A.pb * A.nt;
         T* out = static_cast<T*>(A.out);
         bool ok = true;
         uint32_t u = 0;
         Ring accs;
         for (uint64_t t = blockIdx.x; t < A.tiles; t += gridDim.x, ++u, accs.next(A.acc)) {
             if (!split && (u & 1u) != h) continue;
-            const uint32_t b = accs.i;
-            const uint32_t panel = (uint32_t)(t / A.qtiles), q0 = (uint32_t)(t % A.qtiles) * A.nt;
+            const uint32_t p0 = (uint32_t)(t / A.qtiles) * A.pb, q0 = (uint32_t)(t % A.qtiles) * A.nt;
             const uint32_t rows = min(A.nt, A.m - q0);
-            const uint64_t j = (uint64_t)panel * kFp4Rows + qq * 32 + lane;
+            const uint32_t chunks = min(A.pb, A.panels - p0) * cpp, x0 = split ? h : 0, dx = split ? 2 : 1;
+            const uint32_t addr = tmem + (qq * 32 << 16) + accs.i * acc_cols;
             if (ok) {
-                ok = __all_sync(kFull, bwait(&tfull[b], accs.par, stop, A.polls));
+                ok = __all_sync(kFull, bwait(&tfull[accs.i], accs.par, stop, A.polls));
                 tc_fence_after();
             }
-            T* dst = out + q0 * A.ld + j;
-            for (uint32_t c = split ? h * 16 : 0; c < rows; c += split ? 32 : 16) {
-                uint32_t v[16];
+            for (uint32_t x = x0; x < chunks || x == x0; x += kBatch * dx) {
+                uint32_t v[kBatch][16];
                 __syncwarp();  // tcgen05.ld is warp-collective
                 if (ok) {
-                    tmem_ld16(tmem + (qq * 32 << 16) + b * A.nt + c, v);
-                    tmem_wait_ld16(v);
-                }
-                if (j < A.n)
 #pragma unroll
-                    for (uint32_t e = 0; e < 16; ++e)
-                        if (c + e < rows) store(dst + (uint64_t)(c + e) * A.ld, ok ? __uint_as_float(v[e]) * A.scale : __int_as_float(0x7FC00000));
+                    for (uint32_t y = 0; y < kBatch; ++y)
+                        if (x + y * dx < chunks) tmem_ld16(addr + (x + y * dx) * 16, v[y]);
+#pragma unroll
+                    for (uint32_t y = 0; y < kBatch; ++y) tmem_wait_ld16(v[y]);
+                    if (x + kBatch * dx >= chunks) {  // the accumulator's last read by this warp
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&tempty[accs.i]);
+                    }
+                }
+#pragma unroll
+                for (uint32_t y = 0; y < kBatch; ++y) {
+                    const uint32_t xy = x + y * dx;
+                    if (xy >= chunks) break;
+                    const uint32_t p = xy / cpp, c = (xy - p * cpp) * 16;
+                    const uint64_t j = (uint64_t)(p0 + p) * kFp4Rows + qq * 32 + lane;
+                    T* dst = out + (uint64_t)(q0 + c) * A.ld + j;
+                    if (j < A.n)
+#pragma unroll
+                        for (uint32_t e = 0; e < 16; ++e)
+                            if (c + e < rows)
+                                store(dst + e * A.ld, ok ? __uint_as_float(v[y][e]) * A.scale : __int_as_float(0x7FC00000));
+                }
             }
-            tc_fence_before();
-            __syncwarp();
-            if (ok && lane == 0) mbar_arrive(&tempty[b]);
         }
         if (!ok) *stop = 1u;
     }
@@ -329,29 +348,31 @@ gf_status product(const void* q, uint32_t m, const void* r, uint32_t n, uint32_t
     ProdArgs A = {};
     A.r = static_cast<const uint8_t*>(r);
     A.q = static_cast<const uint8_t*>(q);
-    A.Lo = fp4_layout(dim, block);
+    A.Lr = fp4_layout(n, dim, block);
+    A.Lq = fp4_layout(m, dim, block);
     A.m = m;
     A.n = n;
+    A.panels = fp4_panels(n);
+    A.qtiles = fp4_panels(m);
     A.out = out;
     A.ld = ld;
     A.scale = scale;
     A.polls = test_wait ? test_wait : kPolls;
     A.extra_tx = test_wait ? 16u : 0u;
-    // queries of a tile: all of them up to 256, else equal tiles of a multiple of 64 (a tile then starts
-    // at the first or the middle of the 4 TMEM columns of its panel's scales)
-    const uint32_t nq = (uint32_t)(((uint64_t)m + kMaxNt - 1) / kMaxNt);
-    const uint32_t per = (uint32_t)(((uint64_t)m + nq - 1) / nq), step = nq > 1 ? 64 : 16;
-    A.nt = (per + step - 1) / step * step;
-    A.qtiles = (uint32_t)(((uint64_t)m + A.nt - 1) / A.nt);
-    A.npan = A.qtiles == 1 ? fp4_panels(A.nt) : (A.nt + (A.nt % kFp4Rows ? 64 : 0) + kFp4Rows - 1) / kFp4Rows;
-    A.tiles = (uint64_t)fp4_panels(n) * A.qtiles;
-    A.b_off = A.Lo.group_bytes;
-    A.sfb_off = A.b_off + 4 * A.nt * 16;
-    A.stage_bytes = A.sfb_off + A.npan * A.Lo.scale_bytes;
-    A.sf_cols = (1 + A.npan) * 4 * (block == 16 ? 2 : 1);
-    // two accumulators or more when they leave room for four stages' scales; then as many stages as fit
-    A.acc = std::min(kMaxAcc, std::max(1u, (kTmemCols - 4 * A.sf_cols) / A.nt));
-    A.stages = std::min({kMaxStages, (kSmemLimit - 1024) / A.stage_bytes, (kTmemCols - A.acc * A.nt) / A.sf_cols});
+    A.nt = A.Lq.col_bytes / 16;
+    A.pb = A.gs = 1;
+    if (A.Lr.groups > 1)
+        A.gs = 2;
+    else  // several panels to a tile while two accumulators fit and every SM still has a tile
+        while (A.pb < 4 && 2 * A.pb * A.nt <= 128 && (uint64_t)A.panels * A.qtiles >= 2ull * A.pb * sms) A.pb *= 2;
+    const uint32_t sub = block == 16 ? 2 : 1;
+    A.tiles = ((uint64_t)A.panels + A.pb - 1) / A.pb * A.qtiles;
+    // the panels' part has room for whole groups: an MMA reads 128 rows of two columns whatever the panel has
+    A.b_off = A.pb * A.gs * (sub * kFp4ScaleSub + kFp4Group / kFp4Col * kFp4ColBytes);
+    A.stage_bytes = A.b_off + A.gs * A.Lq.group_bytes;
+    A.sf_cols = (A.pb + 1) * A.gs * 4 * sub;
+    A.stages = std::min(kMaxStages, (kSmemLimit - 1024) / A.stage_bytes);
+    A.acc = std::min(kMaxAcc, (kTmemCols - A.stages * A.sf_cols) / (A.pb * A.nt));
     const uint32_t smem = A.stages * A.stage_bytes + (2 * kMaxStages + 2 * kMaxAcc + 1) * 8 + 16;
     const uint32_t grid = (uint32_t)std::min<uint64_t>(A.tiles, (uint64_t)sms);
     auto go = [&](auto tag) {

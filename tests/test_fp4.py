@@ -108,6 +108,20 @@ def test_packed_positions(block):
     assert not rows.packed[panel + sub + (200 - 128) * 16:panel + sub + 2048].any()  # rows past n
 
 
+@pytest.mark.parametrize("n,h", [(1, 16), (16, 16), (17, 32), (100, 112), (113, 128), (127, 128)])
+def test_short_panel(n, h):
+    """Fewer than 128 rows make one panel of their number rounded up to 16."""
+    x = data(n, 70, n, "normal")
+    rows = gf.quantize_fp4_host(x)
+    assert rows.packed.size == 512 + 3 * h * 16
+    code, _, _ = held(x, 1.0, 32)
+    for k in (0, 31, 40, 69):
+        byte = rows.packed[512 + (k // 32) * h * 16 + (n - 1) * 16 + (k % 32) // 2]
+        nib = (byte >> (4 * (k & 1))) & 15
+        assert MAGS[nib & 7] == abs(code[n - 1, k])
+    assert np.array_equal(gf.dequantize_fp4_host(rows), held(x, 1.0, 32)[2].astype(np.float32))
+
+
 def test_extremes():
     """The ends of fp32's range hold in blocks of 32; E4M3's range bounds blocks of 16."""
     x = np.zeros((4, 32), np.float32)

@@ -18,6 +18,7 @@ DTYPES = [torch.float32, torch.float16, torch.bfloat16]
 def valid_bytes(packed, n, dim, block):
     """Packed bytes of the rows that exist, as (scales, codes) lists in panel order."""
     sub = 512 * (32 // block)
+    h = 128 if n >= 128 else -(-n // 16) * 16
     out = []
     at = 0
     for p in range(-(-n // 128)):
@@ -26,8 +27,8 @@ def valid_bytes(packed, n, dim, block):
             cols = min(4, -(-(dim - k) // 32))
             sc = packed[at:at + sub].reshape(-1, 32, 4, 4).transpose(0, 2, 1, 3).reshape(-1, 128, 4)
             out.append(sc[:, :rows].ravel())
-            out.append(packed[at + sub:at + sub + cols * 2048].reshape(cols, 128, 16)[:, :rows].ravel())
-            at += sub + cols * 2048
+            out.append(packed[at + sub:at + sub + cols * h * 16].reshape(cols, h, 16)[:, :rows].ravel())
+            at += sub + cols * h * 16
     assert at == packed.size
     return np.concatenate(out)
 
