@@ -41,13 +41,12 @@ __device__ __align__(16) uint8_t g_zero[kFp4ColBytes];
 struct ProdArgs {
     const uint8_t *r, *q;
     Fp4Layout Lr, Lq;
-    uint32_t m, n, panels, qtiles;
+    uint32_t m, n, panels, batches, qtiles;  // batches: tiles along the rows
     uint32_t nt;                        // columns of an accumulator: the rows of a query panel
     uint32_t pb, gs;                    // panels of a tile and groups of a stage (one of them 1)
     uint32_t acc, stages, stage_bytes;
     uint32_t b_off;                     // within a stage: the query panel's groups (the row panels' are at 0)
     uint32_t sf_cols;                   // TMEM columns of one stage's scales
-    uint64_t tiles;
     void* out;
     uint64_t ld;
     float scale;
@@ -62,8 +61,8 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo, uint
 }
 // 32 rows x 16 bytes of scales from shared memory (four 128-byte core matrices) to 4 TMEM
 // columns, repeated in each quarter of the lanes.
-__device__ __forceinline__ void scales_to_tmem(uint32_t tmem, uint32_t saddr) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(smem_desc(saddr, 128, 128)) : "memory");
+__device__ __forceinline__ void scales_to_tmem(uint32_t tmem, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
 template <uint32_t BLOCK>
 __device__ __forceinline__ void mma_fp4(uint32_t tmem, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t sfa, uint32_t sfb,
@@ -109,7 +108,17 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 // Bounded wait on a phase; false when it ran out or the CTA is stopping.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t par) {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok)
+                 : "r"(smem_u32(bar)), "r"(par)
+                 : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ bool bwait(uint64_t* bar, uint32_t par, const volatile uint32_t* stop, uint32_t polls) {
+    for (uint32_t p = 0; p < 16; ++p)
+        if (mbar_test(bar, par)) return true;
     for (uint32_t p = 0; p < polls; ++p) {
         if (mbar_try_wait(bar, par, 1000)) return true;
         if (*stop) return false;
@@ -128,6 +137,23 @@ struct Ring {
     }
 };
 
+// This CTA's tiles: blockIdx.x, + gridDim.x, ...; query tiles vary fastest.
+struct Tiles {
+    uint32_t p, q, dp, dq, qtiles, batches;
+    __device__ __forceinline__ Tiles(uint32_t batches_, uint32_t qtiles_)
+        : p(blockIdx.x / qtiles_), q(blockIdx.x % qtiles_), dp(gridDim.x / qtiles_), dq(gridDim.x % qtiles_), qtiles(qtiles_),
+          batches(batches_) {}
+    __device__ __forceinline__ bool more() const { return p < batches; }
+    __device__ __forceinline__ void next() {
+        p += dp;
+        q += dq;
+        if (q >= qtiles) {
+            q -= qtiles;
+            ++p;
+        }
+    }
+};
+
 __device__ __forceinline__ void store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
@@ -136,7 +162,6 @@ template <typename T, uint32_t BLOCK>
 __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_constant__ ProdArgs A) {
     extern __shared__ __align__(1024) unsigned char sm[];
     constexpr uint32_t kSub = BLOCK == 16 ? 2 : 1;  // scale sub-blocks of a group
-    constexpr uint32_t kItems = 4;                  // (panel, group) pairs of a stage, at most
     uint64_t* full = reinterpret_cast<uint64_t*>(sm + A.stages * A.stage_bytes);
     uint64_t* empty = full + kMaxStages;
     uint64_t* tfull = empty + kMaxStages;
@@ -178,11 +203,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         Ring ring;
         uint64_t filled = 0;
         const uint32_t pad = (A.Lq.last_cols & 1u) * A.nt * 16;  // bytes of the zero column of the last group
-        for (uint64_t t = blockIdx.x; ok && t < A.tiles; t += gridDim.x) {
-            const uint32_t p0 = (uint32_t)(t / A.qtiles) * A.pb, qt = (uint32_t)(t % A.qtiles);
-            const uint32_t np = min(A.pb, A.panels - p0);
+        for (Tiles t(A.batches, A.qtiles); ok && t.more(); t.next()) {
+            const uint32_t p0 = t.p * A.pb, np = min(A.pb, A.panels - p0);
             const uint8_t* src_r = A.r + p0 * A.Lr.panel_bytes;
-            const uint8_t* src_q = A.q + qt * A.Lq.panel_bytes;
+            const uint8_t* src_q = A.q + t.q * A.Lq.panel_bytes;
             for (uint32_t g = 0; g < G; g += A.gs, ring.next(A.stages), ++filled) {
                 // (a barrier's first wait, for the use before its first, returns at once)
                 if (!(ok = __all_sync(kFull, bwait(&empty[ring.i], ring.par ^ 1u, stop, A.polls)))) break;
@@ -218,49 +242,70 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         // E2M1 x E2M1, K-major, N = nt, M = 128, scales UE8M0 (block 32) or UE4M3 (block 16)
         const uint32_t idesc = (1u << 7) | (1u << 10) | ((A.nt >> 3) << 17) | ((BLOCK == 32 ? 1u : 0u) << 23) | ((128u >> 4) << 24);
         const uint32_t acc_cols = A.pb * A.nt, sf0 = tmem + A.acc * acc_cols;
-        const uint32_t a_item = A.pb > 1 ? (uint32_t)A.Lr.panel_bytes : A.Lr.group_bytes;
-        const uint64_t ad0 = smem_desc(0, A.Lr.col_bytes, 128), bd0 = smem_desc(0, A.Lq.col_bytes, 128);
+        // everything below in 16-byte units of shared memory, added to a descriptor's address field
+        constexpr uint32_t kScales = kSub * kFp4ScaleSub / 16;
+        const uint32_t a_item = (A.pb > 1 ? (uint32_t)A.Lr.panel_bytes : A.Lr.group_bytes) / 16, b_item = A.Lq.group_bytes / 16;
+        const uint32_t a_step = A.Lr.col_bytes / 8, b_step = A.Lq.col_bytes / 8;
+        const uint32_t sm0 = smem_u32(sm) / 16, st16 = A.stage_bytes / 16, b_off = A.b_off / 16;
+        const uint64_t ad0 = smem_desc(0, A.Lr.col_bytes, 128) + kScales, bd0 = smem_desc(0, A.Lq.col_bytes, 128) + kScales;
+        const uint64_t cd0 = smem_desc(0, 128, 128);
+        const uint32_t sfb_off = A.pb * A.gs * 4 * kSub;
         bool ok = true;
         Ring ring, accs;
-        for (uint64_t t = blockIdx.x; t < A.tiles; t += gridDim.x, accs.next(A.acc)) {
-            const uint32_t np = min(A.pb, A.panels - (uint32_t)(t / A.qtiles) * A.pb);
+        for (Tiles t(A.batches, A.qtiles); t.more(); t.next(), accs.next(A.acc)) {
+            const uint32_t np = min(A.pb, A.panels - t.p * A.pb);
             const uint32_t d0 = tmem + accs.i * acc_cols;
             if (!(ok = __all_sync(kFull, bwait(&tempty[accs.i], accs.par ^ 1u, stop, A.polls)))) break;
             tc_fence_after();
             for (uint32_t g = 0; g < G; g += A.gs, ring.next(A.stages)) {
                 if (!(ok = __all_sync(kFull, bwait(&full[ring.i], ring.par, stop, A.polls)))) break;
                 tc_fence_after();
-                const uint32_t stg = smem_u32(sm) + ring.i * A.stage_bytes;
-                const uint32_t items = A.pb > 1 ? np : min(A.gs, G - g);
+                const uint32_t as = sm0 + ring.i * st16, bs = as + b_off;
                 // this stage's scales; their slot was last read by MMAs that the stage's empty barrier covers
-                const uint32_t sfa = sf0 + ring.i * A.sf_cols, sfb = sfa + A.pb * A.gs * 4 * kSub;
+                const uint32_t sfa = sf0 + ring.i * A.sf_cols, sfb = sfa + sfb_off;
+                const bool last = g + A.gs >= G;
+                const uint32_t items = A.pb > 1 ? np : min(A.gs, G - g);
+                // (panel, group) pair x of the stage: its scales, and its MMA step s of 64 elements
+                auto scales = [&](uint32_t x, bool q) {
+#pragma unroll
+                    for (uint32_t h = 0; h < kSub; ++h) {
+                        scales_to_tmem(sfa + (x * kSub + h) * 4, cd0 + (as + x * a_item + h * (kFp4ScaleSub / 16)));
+                        if (q) scales_to_tmem(sfb + (x * kSub + h) * 4, cd0 + (bs + x * b_item + h * (kFp4ScaleSub / 16)));
+                    }
+                };
+                auto step = [&](uint32_t x, uint32_t s, uint32_t gx, uint32_t d, uint32_t acc) {
+                    // block 16: step s uses sub-block s; block 32: bytes 2s, 2s + 1 of the one sub-block
+                    const uint32_t h = BLOCK == 16 ? s * 4 : 0;
+                    mma_fp4<BLOCK>(d, ad0 + (as + x * a_item + s * a_step), bd0 + (bs + gx * b_item + s * b_step),
+                                   BLOCK == 16 ? idesc : idesc | (2 * s) << 4 | (2 * s) << 29, sfa + x * 4 * kSub + h,
+                                   sfb + gx * 4 * kSub + h, acc);
+                };
                 if (elect_one()) {
+                    if (A.pb == 1 && (!last || (items == 2 && A.Lr.last_cols > 2))) {  // two groups, both steps
+                        scales(0, true);
+                        scales(1, true);
+                        step(0, 0, 0, d0, g);
+                        step(0, 1, 0, d0, 1);
+                        step(1, 0, 1, d0, 1);
+                        step(1, 1, 1, d0, 1);
+                    } else if (items == 4 && A.Lr.last_cols > 2) {  // four panels, both steps
 #pragma unroll
-                    for (uint32_t x = 0; x < kItems; ++x) {
-                        if (x >= items) break;
-                        const uint32_t gx = A.pb > 1 ? 0 : x;  // group of the stage
-                        const uint32_t as = stg + x * a_item, bs = stg + A.b_off + gx * A.Lq.group_bytes;
-                        const uint32_t sa = sfa + x * 4 * kSub, sb = sfb + gx * 4 * kSub;
+                        for (uint32_t x = 0; x < 4; ++x) scales(x, x == 0);
 #pragma unroll
-                        for (uint32_t h = 0; h < kSub; ++h) {
-                            scales_to_tmem(sa + h * 4, as + h * kFp4ScaleSub);
-                            if (x == 0 || A.pb == 1) scales_to_tmem(sb + h * 4, bs + h * kFp4ScaleSub);
+                        for (uint32_t x = 0; x < 4; ++x) {
+                            step(x, 0, 0, d0 + x * A.nt, 0);
+                            step(x, 1, 0, d0 + x * A.nt, 1);
                         }
-                        const uint32_t cols = g + gx + 1 == G ? A.Lr.last_cols : 4u;
-                        const uint32_t d = A.pb > 1 ? d0 + x * A.nt : d0;
-#pragma unroll
-                        for (uint32_t s = 0; s < 2; ++s) {
-                            if (s * 2 >= cols) break;
-                            const uint64_t ad = ad0 + ((as + kSub * kFp4ScaleSub + s * 2 * A.Lr.col_bytes) >> 4);
-                            const uint64_t bd = bd0 + ((bs + kSub * kFp4ScaleSub + s * 2 * A.Lq.col_bytes) >> 4);
-                            // block 16: step s uses sub-block s; block 32: bytes 2s, 2s + 1 of the one sub-block
-                            const uint32_t id = BLOCK == 16 ? idesc : idesc | (2 * s) << 4 | (2 * s) << 29;
-                            const uint32_t h = BLOCK == 16 ? s * 4 : 0;
-                            mma_fp4<BLOCK>(d, ad, bd, id, sa + h, sb + h, (g + gx) | s ? 1u : 0u);
+                    } else {
+                        for (uint32_t x = 0; x < items; ++x) {
+                            const uint32_t gx = A.pb > 1 ? 0 : x, d = A.pb > 1 ? d0 + x * A.nt : d0;
+                            scales(x, x == 0 || A.pb == 1);
+                            step(x, 0, gx, d, g + gx);
+                            if (g + gx + 1 < G || A.Lr.last_cols > 2) step(x, 1, gx, d, 1);
                         }
                     }
                     mma_commit(&empty[ring.i]);  // the stage is free once these MMAs have read it
-                    if (g + A.gs >= G) mma_commit(&tfull[accs.i]);
+                    if (last) mma_commit(&tfull[accs.i]);
                 }
                 __syncwarp();
             }
@@ -284,9 +329,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         bool ok = true;
         uint32_t u = 0;
         Ring accs;
-        for (uint64_t t = blockIdx.x; t < A.tiles; t += gridDim.x, ++u, accs.next(A.acc)) {
+        for (Tiles t(A.batches, A.qtiles); t.more(); t.next(), ++u, accs.next(A.acc)) {
             if (!split && (u & 1u) != h) continue;
-            const uint32_t p0 = (uint32_t)(t / A.qtiles) * A.pb, q0 = (uint32_t)(t % A.qtiles) * A.nt;
+            const uint32_t p0 = t.p * A.pb, q0 = t.q * A.nt;
             const uint32_t rows = min(A.nt, A.m - q0);
             const uint32_t chunks = min(A.pb, A.panels - p0) * cpp, x0 = split ? h : 0, dx = split ? 2 : 1;
             const uint32_t addr = tmem + (qq * 32 << 16) + accs.i * acc_cols;
@@ -366,7 +411,8 @@ gf_status product(const void* q, uint32_t m, const void* r, uint32_t n, uint32_t
     else  // several panels to a tile while two accumulators fit and every SM still has a tile
         while (A.pb < 4 && 2 * A.pb * A.nt <= 128 && (uint64_t)A.panels * A.qtiles >= 2ull * A.pb * sms) A.pb *= 2;
     const uint32_t sub = block == 16 ? 2 : 1;
-    A.tiles = ((uint64_t)A.panels + A.pb - 1) / A.pb * A.qtiles;
+    A.batches = (A.panels + A.pb - 1) / A.pb;
+    const uint64_t tiles = (uint64_t)A.batches * A.qtiles;
     // the panels' part has room for whole groups: an MMA reads 128 rows of two columns whatever the panel has
     A.b_off = A.pb * A.gs * (sub * kFp4ScaleSub + kFp4Group / kFp4Col * kFp4ColBytes);
     A.stage_bytes = A.b_off + A.gs * A.Lq.group_bytes;
@@ -374,7 +420,7 @@ gf_status product(const void* q, uint32_t m, const void* r, uint32_t n, uint32_t
     A.stages = std::min(kMaxStages, (kSmemLimit - 1024) / A.stage_bytes);
     A.acc = std::min(kMaxAcc, (kTmemCols - A.stages * A.sf_cols) / (A.pb * A.nt));
     const uint32_t smem = A.stages * A.stage_bytes + (2 * kMaxStages + 2 * kMaxAcc + 1) * 8 + 16;
-    const uint32_t grid = (uint32_t)std::min<uint64_t>(A.tiles, (uint64_t)sms);
+    const uint32_t grid = (uint32_t)std::min<uint64_t>(tiles, (uint64_t)sms);
     auto go = [&](auto tag) {
         using T = decltype(tag);
         return block == 16 ? launch_product<T, 16>(A, grid, smem, s) : launch_product<T, 32>(A, grid, smem, s);
