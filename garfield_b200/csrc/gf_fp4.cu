@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const T* __restr
     for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
         const uint32_t p = (uint32_t)(t / Lo.groups), g = (uint32_t)(t % Lo.groups);
         const uint32_t row0 = p * kFp4Rows, valid = min(kFp4Rows, n - row0);
-        const uint32_t cols = g + 1 == Lo.groups ? Lo.last_cols : 4u;
+        const uint32_t cols = min(4u, Lo.cols - 4 * g);
         const uint32_t k = g * kFp4Group + lane * 4;
         for (uint32_t r0 = warp; r0 < valid; r0 += kWarps * U) {
             float x[U][4];
@@ -146,15 +146,16 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const T* __restr
             }
         }
         __syncthreads();
-        uint8_t* dst = packed + p * Lo.panel_bytes + (uint64_t)g * Lo.group_bytes;
+        uint32_t* dst_s = reinterpret_cast<uint32_t*>(packed + Lo.scales_at(p, g));
+        uint8_t* dst = packed + Lo.col_at(p, 4 * g);
         for (uint32_t i = threadIdx.x; i < kSb / 4; i += kThreads) {
             const uint32_t r = (i & 3u) * 32 + ((i >> 2) & 31u);
-            if (r < valid) reinterpret_cast<uint32_t*>(dst)[i] = reinterpret_cast<const uint32_t*>(scales_s)[i];
+            if (r < valid) dst_s[i] = reinterpret_cast<const uint32_t*>(scales_s)[i];
         }
         for (uint32_t i = threadIdx.x; i < cols * kFp4Rows; i += kThreads) {
             const uint32_t c = i / kFp4Rows, r = i % kFp4Rows;
             if (r < valid)
-                *reinterpret_cast<uint4*>(dst + kSb + c * Lo.col_bytes + r * 16) =
+                *reinterpret_cast<uint4*>(dst + c * Lo.col_bytes + r * 16) =
                     *reinterpret_cast<const uint4*>(codes_s + c * kColPitch + r * 16);
         }
         __syncthreads();
@@ -176,16 +177,16 @@ __global__ void __launch_bounds__(kThreads) fp4_dequantize_kernel(const uint8_t*
     for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
         const uint32_t p = (uint32_t)(t / Lo.groups), g = (uint32_t)(t % Lo.groups);
         const uint32_t row0 = p * kFp4Rows, valid = min(kFp4Rows, n - row0);
-        const uint32_t cols = g + 1 == Lo.groups ? Lo.last_cols : 4u;
+        const uint32_t cols = min(4u, Lo.cols - 4 * g);
         const uint32_t k = g * kFp4Group + lane * 4;
-        const uint8_t* src = packed + p * Lo.panel_bytes + (uint64_t)g * Lo.group_bytes;
-        for (uint32_t i = threadIdx.x; i < kSb / 16; i += kThreads)
-            reinterpret_cast<uint4*>(scales_s)[i] = reinterpret_cast<const uint4*>(src)[i];
+        const uint4* src_s = reinterpret_cast<const uint4*>(packed + Lo.scales_at(p, g));
+        const uint8_t* src = packed + Lo.col_at(p, 4 * g);
+        for (uint32_t i = threadIdx.x; i < kSb / 16; i += kThreads) reinterpret_cast<uint4*>(scales_s)[i] = src_s[i];
         for (uint32_t i = threadIdx.x; i < cols * kFp4Rows; i += kThreads) {
             const uint32_t c = i / kFp4Rows, r = i % kFp4Rows;
             if (r < valid)
                 *reinterpret_cast<uint4*>(codes_s + c * kColPitch + r * 16) =
-                    *reinterpret_cast<const uint4*>(src + kSb + c * Lo.col_bytes + r * 16);
+                    *reinterpret_cast<const uint4*>(src + c * Lo.col_bytes + r * 16);
         }
         __syncthreads();
         if (k < dim) {
@@ -268,15 +269,13 @@ void quantize_host(const float* data, uint32_t n, uint32_t dim, float alpha, uin
                 std::frexp(amax, &e);  // amax in [2^(e-1), 2^e)
                 s8 = amax > 0.0f ? (uint32_t)std::max(e - 3 + 127, 0) : 0u;
             }
-            uint8_t* grp = packed + (i / kFp4Rows) * Lo.panel_bytes + (uint64_t)(k0 / kFp4Group) * Lo.group_bytes;
-            grp[fp4_scale_at(r, (k0 % kFp4Group) / block)] = (uint8_t)s8;
+            packed[Lo.scales_at(i / kFp4Rows, k0 / kFp4Group) + fp4_scale_at(r, (k0 % kFp4Group) / block)] = (uint8_t)s8;
             if (bad || (block == 16 && s8 == 0)) continue;
             const float s = scale_host(s8, block);
             for (uint32_t k = k0; k < k1; ++k) {
                 // block 32: multiplied by 1 / s, a power of two that fp32 holds for every s
                 const float y = block == 16 ? x[k] * alpha / s : std::ldexp(x[k] * alpha, 127 - (int)s8);
-                const uint32_t kg = k % kFp4Group;
-                uint8_t* b = grp + Lo.scale_bytes + (kg / kFp4Col) * Lo.col_bytes + r * 16 + (kg % kFp4Col) / 2;
+                uint8_t* b = packed + Lo.col_at(i / kFp4Rows, k / kFp4Col) + r * 16 + (k % kFp4Col) / 2;
                 *b = (uint8_t)(*b | e2m1_host(y) << (4 * (k & 1u)));
             }
         }
@@ -286,11 +285,10 @@ void dequantize_host(const uint8_t* packed, uint32_t n, uint32_t dim, uint32_t b
     const Fp4Layout Lo = fp4_layout(n, dim, block);
     for (uint32_t i = 0; i < n; ++i)
         for (uint32_t k = 0; k < dim; ++k) {
-            const uint32_t r = i % kFp4Rows, kg = k % kFp4Group;
-            const uint8_t* grp = packed + (i / kFp4Rows) * Lo.panel_bytes + (uint64_t)(k / kFp4Group) * Lo.group_bytes;
-            const uint32_t b = grp[Lo.scale_bytes + (kg / kFp4Col) * Lo.col_bytes + r * 16 + (kg % kFp4Col) / 2];
-            const uint32_t c = (b >> (4 * (k & 1u))) & 15u;
-            const float s = scale_host(grp[fp4_scale_at(r, kg / block)], block) / alpha;
+            const uint32_t r = i % kFp4Rows, p = i / kFp4Rows;
+            const uint32_t c = (packed[Lo.col_at(p, k / kFp4Col) + r * 16 + (k % kFp4Col) / 2] >> (4 * (k & 1u))) & 15u;
+            const uint32_t s8 = packed[Lo.scales_at(p, k / kFp4Group) + fp4_scale_at(r, k % kFp4Group / block)];
+            const float s = scale_host(s8, block) / alpha;
             out[(uint64_t)i * dim + k] = (c & 8u ? -kMags[c & 7u] : kMags[c & 7u]) * s;
         }
 }

@@ -1,16 +1,16 @@
 // Layout of rows held in 4-bit block floating point (gf_fp4.cu, gf_fp4_tc.cu).
 //
-// Rows are cut into panels of 128 (fewer than 128 rows: one panel of their number rounded up to 16)
-// and their elements into groups of 128.  A panel of h rows holds its groups in order; a group is
-//   scales   128 rows x (128 / block) bytes, as `128 / (4 block)` sub-blocks of 512 bytes: byte b
-//            of row r in a sub-block (4 consecutive blocks b of the row) is at
+// Rows are cut into panels of 128 (fewer than 128 rows: one panel of their number rounded up to 16),
+// their elements into groups of 128 and columns of 32.  A panel of h rows holds
+//   scales   for each group, 128 rows x (128 / block) bytes, as `128 / (4 block)` sub-blocks of 512
+//            bytes: byte b of row r in a sub-block (4 consecutive blocks b of the row) is at
 //            (r % 32) * 16 + (r / 32) * 4 + b -- the order in which one tcgen05.cp (32x128b,
 //            warpx4) spreads the scales of 128 rows over 4 TMEM columns
-//   codes    columns of 32 elements; a column is h rows x 16 bytes, row r at r * 16, element
-//            2i in the low half of byte i -- 8 rows of a column are one tcgen05 core matrix
-//            (K-major, no swizzle), so a column needs no rearranging between HBM and the MMA
-// The last group of a row holds only the columns that have elements.  Every byte of a panel is
-// contiguous, so one bulk copy brings a group, or several, into shared memory.  Codes and scales
+//   codes    for each column that has elements, h rows x 16 bytes, row r at r * 16, element 2i in
+//            the low half of byte i -- 8 rows of a column are one tcgen05 core matrix (K-major,
+//            no swizzle), so a column needs no rearranging between HBM and the MMA
+// The scales of consecutive groups and the codes of consecutive columns are one run each: two bulk
+// copies bring any number of groups into shared memory, one a whole panel.  Codes and scales
 // past the end of a row are 0; what stands in the rows past n of the last panel is unspecified
 // (a row's bytes reach only that row's outputs).
 #pragma once
@@ -28,18 +28,20 @@ constexpr uint32_t kFp4ColBytes = kFp4Rows * 16;  // a column of a full panel
 constexpr uint32_t kFp4ScaleSub = 512;          // bytes of one scale sub-block
 
 struct Fp4Layout {
-    uint32_t groups, last_cols, scale_bytes, col_bytes, group_bytes, last_bytes;
+    uint32_t groups, cols, scale_bytes, col_bytes;  // groups and columns of a row, bytes of a group's scales and of a column
     uint64_t panel_bytes;
+    __host__ __device__ uint64_t scales_at(uint32_t p, uint32_t g) const { return p * panel_bytes + (uint64_t)g * scale_bytes; }
+    __host__ __device__ uint64_t col_at(uint32_t p, uint32_t c) const {
+        return p * panel_bytes + (uint64_t)groups * scale_bytes + (uint64_t)c * col_bytes;
+    }
 };
 __host__ __device__ inline Fp4Layout fp4_layout(uint32_t n, uint32_t dim, uint32_t block) {
     Fp4Layout L;
     L.col_bytes = (n < kFp4Rows ? (n + 15) / 16 * 16 : kFp4Rows) * 16;
     L.groups = (uint32_t)(((uint64_t)dim + kFp4Group - 1) / kFp4Group);
-    L.last_cols = (uint32_t)((dim - (uint64_t)(L.groups - 1) * kFp4Group + kFp4Col - 1) / kFp4Col);
+    L.cols = (uint32_t)(((uint64_t)dim + kFp4Col - 1) / kFp4Col);
     L.scale_bytes = block == 16 ? 2 * kFp4ScaleSub : kFp4ScaleSub;
-    L.group_bytes = L.scale_bytes + kFp4Group / kFp4Col * L.col_bytes;
-    L.last_bytes = L.scale_bytes + L.last_cols * L.col_bytes;
-    L.panel_bytes = (uint64_t)(L.groups - 1) * L.group_bytes + L.last_bytes;
+    L.panel_bytes = (uint64_t)L.groups * L.scale_bytes + (uint64_t)L.cols * L.col_bytes;
     return L;
 }
 __host__ __device__ inline uint32_t fp4_panels(uint32_t n) { return (uint32_t)(((uint64_t)n + kFp4Rows - 1) / kFp4Rows); }

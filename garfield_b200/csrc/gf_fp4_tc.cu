@@ -5,13 +5,20 @@
 //
 // The rows r are the M side (128 rows of a panel = 128 TMEM lanes), the queries q the N side, so
 // an accumulator's lanes are consecutive j: a warp's store of one column is a contiguous
-// run of out, whatever the number of queries, and few queries cost few columns.  A CTA walks tiles
-// (pb panels, a panel of queries), queries fastest, so a panel's bytes leave HBM once.  Warp 0
-// copies the panels' groups and the query panel's, one run each, into a ring of stages; warp 1
-// spreads the scales into TMEM (tcgen05.cp) and issues two MMAs of 64 elements per panel and
-// group; eight warps read finished accumulators and write out.  A stage holds two groups of a
-// panel or, for rows of one group, up to four panels: an asynchronous copy costs its issuing warp some 80
-// cycles, and at the HBM rate a group of a panel passes in 200.
+// run of out, whatever the number of queries, and few queries cost few columns.
+//
+// One kernel in two widths.  CTAS = 1: a CTA walks tiles of pb row panels by one query panel (up to
+// 128 queries).  CTAS = 2: a cluster of two CTAs walks tiles of two row panels by two query panels,
+// each CTA holding one of either and the tcgen05.mma of the pair (M = N = 256) reading both, so
+// that a byte copied into shared memory feeds twice the products.  Query tiles vary fastest: a
+// panel's bytes leave HBM once.
+//
+// Warp 0 copies scales and codes, one run each, into a ring of stages of up to four groups (of a
+// panel, or of several panels that fit whole); warp 1 spreads the stage's scales into TMEM
+// (tcgen05.cp) and issues two MMAs of 64 elements per panel and group; eight warps read
+// finished accumulators and write out.  The stages are this long because a warp pays some 450
+// cycles a stage whatever it holds (waiting, committing, the first instruction's way), while a group's
+// MMAs take 128 cycles at N = 128 and its panel's bytes 200 at the HBM rate.
 //
 // Every wait is bounded.  When one runs out the CTA stops and the outputs it still owes become NaN.
 #include <cuda_bf16.h>
@@ -38,14 +45,18 @@ constexpr uint32_t kSmemLimit = 227 * 1024;
 // query side, whatever codes stand in the other side's place add nothing.
 __device__ __align__(16) uint8_t g_zero[kFp4ColBytes];
 
+// Groups of a full stage: four, or three where two query panels' scales of 16-element blocks would leave
+// TMEM no room for a third stage beside an accumulator of 256 columns.
+constexpr uint32_t stage_groups(uint32_t block, uint32_t ctas) { return ctas == 2 && block == 16 ? 3 : 4; }
+
 struct ProdArgs {
     const uint8_t *r, *q;
     Fp4Layout Lr, Lq;
-    uint32_t m, n, panels, batches, qtiles;  // batches: tiles along the rows
-    uint32_t nt;                        // columns of an accumulator: the rows of a query panel
-    uint32_t pb, gs;                    // panels of a tile and groups of a stage (one of them 1)
+    uint32_t m, n, panels, qpanels, batches, qtiles;  // batches: tiles along the rows
+    uint32_t nt;                        // columns of an accumulator
+    uint32_t pb, gs;                    // row panels of a CTA's tile and groups of a stage (pb > 1: gs is all groups)
     uint32_t acc, stages, stage_bytes;
-    uint32_t b_off;                     // within a stage: the query panel's groups (the row panels' are at 0)
+    uint32_t b_off, bc_off;             // within a stage: the query panels' scales, and the query panel's codes
     uint32_t sf_cols;                   // TMEM columns of one stage's scales
     void* out;
     uint64_t ld;
@@ -60,29 +71,74 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo, uint
            (uint64_t)((sbo >> 4) & 0x3FFFu) << 32 | (uint64_t)1 << 46;
 }
 // 32 rows x 16 bytes of scales from shared memory (four 128-byte core matrices) to 4 TMEM
-// columns, repeated in each quarter of the lanes.
+// columns, repeated in each quarter of the lanes (of both CTAs of a pair, each from its own).
+template <uint32_t CTAS>
 __device__ __forceinline__ void scales_to_tmem(uint32_t tmem, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+    if (CTAS == 1)
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
-template <uint32_t BLOCK>
+#define GF_MMA_FP4(group, kind)                                                                                 \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\ttcgen05.mma.cta_group::" group ".kind::" kind  \
+                 " [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(tmem),                                        \
+                 "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc))
+template <uint32_t BLOCK, uint32_t CTAS>
 __device__ __forceinline__ void mma_fp4(uint32_t tmem, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                         uint32_t acc) {
-    if (BLOCK == 16)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(tmem),
-            "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc));
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(tmem),
-            "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc));
+    if (BLOCK == 16 && CTAS == 1) GF_MMA_FP4("1", "mxf4nvf4.block_scale.scale_vec::4X");
+    if (BLOCK == 32 && CTAS == 1) GF_MMA_FP4("1", "mxf4.block_scale.scale_vec::2X");
+    if (BLOCK == 16 && CTAS == 2) GF_MMA_FP4("2", "mxf4nvf4.block_scale.scale_vec::4X");
+    if (BLOCK == 32 && CTAS == 2) GF_MMA_FP4("2", "mxf4.block_scale.scale_vec::2X");
 }
+#undef GF_MMA_FP4
+// Arrival on the barrier (of both CTAs of a pair, at the same offset) once the MMAs issued so far are done.
+template <uint32_t CTAS>
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    if (CTAS == 1)
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                         smem_u32(bar)),
+                     "h"((uint16_t)3)
+                     : "memory");
+}
+template <uint32_t CTAS>
+__device__ __forceinline__ void tmem_alloc(uint32_t* slot) {
+    if (CTAS == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(kTmemCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(kTmemCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+    }
+}
+template <uint32_t CTAS>
+__device__ __forceinline__ void tmem_free(uint32_t tmem) {
+    if (CTAS == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+    else
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// Arrival on the same barrier of the cluster's CTA 0, ordered after this thread's earlier accesses.
+__device__ __forceinline__ void arrive_at_leader(uint64_t* bar) {
+    asm volatile(
+        "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, 0;\n mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n}\n" ::"r"(
+            smem_u32(bar))
+        : "memory");
+}
+// Every thread of the CTA, or of the pair, has arrived.
+template <uint32_t CTAS>
+__device__ __forceinline__ void sync_all() {
+    tc_fence_before();
+    if (CTAS == 1)
+        __syncthreads();
+    else
+        asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory");
+    tc_fence_after();
 }
 // 16 consecutive TMEM columns of this warp's 32 lanes, and the wait that orders their use.
 __device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* v) {
@@ -107,20 +163,33 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
     return p != 0;
 }
-// Bounded wait on a phase; false when it ran out or the CTA is stopping.
+// Bounded wait on a phase; false when it ran out or the CTA is stopping.  (The suspending form of
+// the test takes longer to answer than the plain one, so a few of those come first.)  Arrivals may
+// come from the pair's other CTA, hence the cluster scope.
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t par) {
     uint32_t ok;
-    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-                 : "=r"(ok)
-                 : "r"(smem_u32(bar)), "r"(par)
-                 : "memory");
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(par)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t par) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, "
+        "p;\n}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(par), "r"(1000u)
+        : "memory");
     return ok != 0;
 }
 __device__ __forceinline__ bool bwait(uint64_t* bar, uint32_t par, const volatile uint32_t* stop, uint32_t polls) {
     for (uint32_t p = 0; p < 16; ++p)
         if (mbar_test(bar, par)) return true;
     for (uint32_t p = 0; p < polls; ++p) {
-        if (mbar_try_wait(bar, par, 1000)) return true;
+        if (mbar_try(bar, par)) return true;
         if (*stop) return false;
     }
     return false;
@@ -137,12 +206,11 @@ struct Ring {
     }
 };
 
-// This CTA's tiles: blockIdx.x, + gridDim.x, ...; query tiles vary fastest.
+// The tiles of worker i of w: i, i + w, ...; query tiles vary fastest.
 struct Tiles {
     uint32_t p, q, dp, dq, qtiles, batches;
-    __device__ __forceinline__ Tiles(uint32_t batches_, uint32_t qtiles_)
-        : p(blockIdx.x / qtiles_), q(blockIdx.x % qtiles_), dp(gridDim.x / qtiles_), dq(gridDim.x % qtiles_), qtiles(qtiles_),
-          batches(batches_) {}
+    __device__ __forceinline__ Tiles(uint32_t i, uint32_t w, uint32_t batches_, uint32_t qtiles_)
+        : p(i / qtiles_), q(i % qtiles_), dp(w / qtiles_), dq(w % qtiles_), qtiles(qtiles_), batches(batches_) {}
     __device__ __forceinline__ bool more() const { return p < batches; }
     __device__ __forceinline__ void next() {
         p += dp;
@@ -158,42 +226,41 @@ __device__ __forceinline__ void store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-template <typename T, uint32_t BLOCK>
+template <typename T, uint32_t BLOCK, uint32_t CTAS>
 __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_constant__ ProdArgs A) {
     extern __shared__ __align__(1024) unsigned char sm[];
     constexpr uint32_t kSub = BLOCK == 16 ? 2 : 1;  // scale sub-blocks of a group
+    constexpr uint32_t kGs = stage_groups(BLOCK, CTAS);
     uint64_t* full = reinterpret_cast<uint64_t*>(sm + A.stages * A.stage_bytes);
-    uint64_t* empty = full + kMaxStages;
+    uint64_t* pfull = full + kMaxStages;  // CTA 0 of a pair: the other CTA's stage is full
+    uint64_t* empty = pfull + kMaxStages;
     uint64_t* tfull = empty + kMaxStages;
     uint64_t* tempty = tfull + kMaxAcc;
     uint64_t* drain = tempty + kMaxAcc;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile uint32_t* stop = tmem_slot + 1;
     const uint32_t warp = threadIdx.x >> 5, lane = lane_id();
+    const uint32_t rank = CTAS == 2 ? (blockIdx.x & 1u) : 0u;  // in the pair (clusters are consecutive blocks)
+    const uint32_t worker = blockIdx.x / CTAS, workers = gridDim.x / CTAS;
     const uint32_t cpp = A.nt / 16;     // 16-column chunks of a panel's accumulator
     const bool split = A.pb * cpp > 1;  // both epilogue halves share a tile's chunks, else they take alternate tiles
 
-    if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                     "r"(kTmemCols));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
-    }
+    if (warp == 0) tmem_alloc<CTAS>(tmem_slot);
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kMaxStages; ++i) {
             mbar_init(&full[i], 1);
+            mbar_init(&pfull[i], 1);
             mbar_init(&empty[i], 1);
         }
         for (uint32_t i = 0; i < kMaxAcc; ++i) {
             mbar_init(&tfull[i], 1);
-            mbar_init(&tempty[i], split ? 8 : 4);
+            mbar_init(&tempty[i], (split ? 8 : 4) * CTAS);
         }
         mbar_init(drain, 1);
         *stop = 0;
         fence_mbar_init();
     }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
+    sync_all<CTAS>();
     const uint32_t tmem = *tmem_slot;
     const uint32_t G = A.Lr.groups;
 
@@ -202,29 +269,39 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         bool ok = true;
         Ring ring;
         uint64_t filled = 0;
-        const uint32_t pad = (A.Lq.last_cols & 1u) * A.nt * 16;  // bytes of the zero column of the last group
-        for (Tiles t(A.batches, A.qtiles); ok && t.more(); t.next()) {
-            const uint32_t p0 = t.p * A.pb, np = min(A.pb, A.panels - p0);
-            const uint8_t* src_r = A.r + p0 * A.Lr.panel_bytes;
-            const uint8_t* src_q = A.q + t.q * A.Lq.panel_bytes;
+        const uint32_t pad = A.Lq.cols & 1u;  // the last group lacks the second column of an MMA step
+        for (Tiles t(worker, workers, A.batches, A.qtiles); ok && t.more(); t.next()) {
+            const uint32_t p0 = t.p * A.pb * CTAS + rank, np = p0 < A.panels ? min(A.pb, A.panels - p0) : 0u;
+            const uint32_t qp = t.q * CTAS + rank;
             for (uint32_t g = 0; g < G; g += A.gs, ring.next(A.stages), ++filled) {
                 // (a barrier's first wait, for the use before its first, returns at once)
                 if (!(ok = __all_sync(kFull, bwait(&empty[ring.i], ring.par ^ 1u, stop, A.polls)))) break;
                 unsigned char* stg = sm + ring.i * A.stage_bytes;
                 uint64_t* bar = &full[ring.i];
-                const bool last = g + A.gs >= G;
-                const uint32_t whole = last ? G - 1 - g : A.gs;  // full groups of the stage
-                const uint32_t a_bytes = (whole * A.Lr.group_bytes + (last ? A.Lr.last_bytes : 0u)) * np;
-                const uint32_t b_bytes = whole * A.Lq.group_bytes + (last ? A.Lq.last_bytes : 0u);
+                const uint32_t ng = min(A.gs, G - g), nc = min(4 * ng, A.Lr.cols - 4 * g);  // groups and columns
+                const uint32_t as = ng * A.Lr.scale_bytes, ac = nc * A.Lr.col_bytes, bc = nc * A.Lq.col_bytes;
+                const uint32_t z = g + ng == G && pad ? A.Lq.col_bytes : 0u;
+                const uint32_t a_bytes = A.pb > 1 ? np * (uint32_t)A.Lr.panel_bytes : np * (as + ac);
+                // query panels of the tile that exist: their scales all come, the codes of this CTA's
+                const uint32_t nq = min(CTAS, A.qpanels - t.q * CTAS);
+                const uint32_t b_bytes = nq * as + (qp < A.qpanels ? bc + z : 0u);
                 if (elect_one()) {
-                    mbar_arrive_expect_tx(bar, a_bytes + b_bytes + (last ? pad : 0u) + A.extra_tx);
-                    bulk_g2s(stg, src_r, a_bytes, bar);
-                    bulk_g2s(stg + A.b_off, src_q, b_bytes, bar);
-                    if (last && pad) bulk_g2s(stg + A.b_off + b_bytes, g_zero, pad, bar);
+                    mbar_arrive_expect_tx(bar, a_bytes + b_bytes + A.extra_tx);
+                    if (A.pb > 1) {  // whole panels
+                        bulk_g2s(stg, A.r + A.Lr.scales_at(p0, 0), a_bytes, bar);
+                    } else if (np) {
+                        bulk_g2s(stg, A.r + A.Lr.scales_at(p0, g), as, bar);
+                        bulk_g2s(stg + A.gs * A.Lr.scale_bytes, A.r + A.Lr.col_at(p0, 4 * g), ac, bar);
+                    }
+                    bulk_g2s(stg + A.b_off, A.q + A.Lq.scales_at(t.q * CTAS, g), as, bar);
+                    if (CTAS == 2 && nq == 2)
+                        bulk_g2s(stg + A.b_off + A.gs * A.Lq.scale_bytes, A.q + A.Lq.scales_at(t.q * CTAS + 1, g), as, bar);
+                    if (qp < A.qpanels) {
+                        bulk_g2s(stg + A.bc_off, A.q + A.Lq.col_at(qp, 4 * g), bc, bar);
+                        if (z) bulk_g2s(stg + A.bc_off + bc, g_zero, z, bar);
+                    }
                 }
                 __syncwarp();
-                src_r += a_bytes;
-                src_q += b_bytes;
             }
         }
         if (!ok) *stop = 1u;
@@ -233,79 +310,107 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
             for (uint32_t st = 0; st < A.stages && st < filled; ++st) {
                 const uint32_t use = (uint32_t)((filled - 1 - st) / A.stages);  // the slot's last
                 uint32_t p = 0;
-                while (!mbar_try_wait(&full[st], use & 1u, 1000) && ++p < A.polls) {
+                while (!mbar_try(&full[st], use & 1u) && ++p < A.polls) {
                 }
             }
         __syncwarp();
+    } else if (warp == 1 && rank != 0) {
+        // ------------------------- the other CTA of a pair: tells CTA 0 which of its stages are full
+        bool ok = true;
+        Ring ring;
+        for (Tiles t(worker, workers, A.batches, A.qtiles); ok && t.more(); t.next())
+            for (uint32_t g = 0; g < G; g += A.gs, ring.next(A.stages)) {
+                if (!(ok = __all_sync(kFull, bwait(&full[ring.i], ring.par, stop, A.polls)))) break;
+                if (lane == 0) arrive_at_leader(&pfull[ring.i]);
+                __syncwarp();
+            }
+        if (!ok) *stop = 1u;
+        // CTA 0's last commit, which follows all its others, has arrived here before this CTA can exit
+        uint32_t p = 0;
+        while (!mbar_try(drain, 0) && ++p < A.polls) {
+        }
+        __syncwarp();
     } else if (warp == 1) {
         // -------------------------------------------------------------- MMA warp
-        // E2M1 x E2M1, K-major, N = nt, M = 128, scales UE8M0 (block 32) or UE4M3 (block 16)
-        const uint32_t idesc = (1u << 7) | (1u << 10) | ((A.nt >> 3) << 17) | ((BLOCK == 32 ? 1u : 0u) << 23) | ((128u >> 4) << 24);
+        // E2M1 x E2M1, K-major, N = nt (256 for a pair), M = 128 (256), scales UE8M0 (block 32) or UE4M3 (block 16)
+        const uint32_t idesc = (1u << 7) | (1u << 10) | ((A.nt >> 3) << 17) | ((BLOCK == 32 ? 1u : 0u) << 23) |
+                               ((CTAS * 128u >> 4) << 24);
         const uint32_t acc_cols = A.pb * A.nt, sf0 = tmem + A.acc * acc_cols;
         // everything below in 16-byte units of shared memory, added to a descriptor's address field
-        constexpr uint32_t kScales = kSub * kFp4ScaleSub / 16;
-        const uint32_t a_item = (A.pb > 1 ? (uint32_t)A.Lr.panel_bytes : A.Lr.group_bytes) / 16, b_item = A.Lq.group_bytes / 16;
-        const uint32_t a_step = A.Lr.col_bytes / 8, b_step = A.Lq.col_bytes / 8;
+        constexpr uint32_t kScales = kSub * kFp4ScaleSub / 16;  // a group's scales
+        const uint32_t a_item = (uint32_t)A.Lr.panel_bytes / 16;
+        const uint32_t a_step = A.Lr.col_bytes / 8, b_step = A.Lq.col_bytes / 8;  // two columns
         const uint32_t sm0 = smem_u32(sm) / 16, st16 = A.stage_bytes / 16, b_off = A.b_off / 16;
-        const uint64_t ad0 = smem_desc(0, A.Lr.col_bytes, 128) + kScales, bd0 = smem_desc(0, A.Lq.col_bytes, 128) + kScales;
+        const uint64_t ad0 = smem_desc(0, A.Lr.col_bytes, 128) + A.gs * kScales;
+        const uint64_t bd0 = smem_desc(0, A.Lq.col_bytes, 128) + A.bc_off / 16;
         const uint64_t cd0 = smem_desc(0, 128, 128);
-        const uint32_t sfb_off = A.pb * A.gs * 4 * kSub;
+        const uint32_t sfb_off = A.pb * A.gs * 4 * kSub, q2 = A.gs * kScales;
         bool ok = true;
         Ring ring, accs;
-        for (Tiles t(A.batches, A.qtiles); t.more(); t.next(), accs.next(A.acc)) {
-            const uint32_t np = min(A.pb, A.panels - t.p * A.pb);
+        for (Tiles t(worker, workers, A.batches, A.qtiles); t.more(); t.next(), accs.next(A.acc)) {
+            const uint32_t np = CTAS == 2 ? 1u : min(A.pb, A.panels - t.p * A.pb);
             const uint32_t d0 = tmem + accs.i * acc_cols;
             if (!(ok = __all_sync(kFull, bwait(&tempty[accs.i], accs.par ^ 1u, stop, A.polls)))) break;
             tc_fence_after();
             for (uint32_t g = 0; g < G; g += A.gs, ring.next(A.stages)) {
-                if (!(ok = __all_sync(kFull, bwait(&full[ring.i], ring.par, stop, A.polls)))) break;
+                ok = bwait(&full[ring.i], ring.par, stop, A.polls);
+                if (CTAS == 2) ok = ok && bwait(&pfull[ring.i], ring.par, stop, A.polls);
+                if (!(ok = __all_sync(kFull, ok))) break;
                 tc_fence_after();
-                const uint32_t as = sm0 + ring.i * st16, bs = as + b_off;
+                const uint32_t st = sm0 + ring.i * st16;
                 // this stage's scales; their slot was last read by MMAs that the stage's empty barrier covers
                 const uint32_t sfa = sf0 + ring.i * A.sf_cols, sfb = sfa + sfb_off;
-                const bool last = g + A.gs >= G;
-                const uint32_t items = A.pb > 1 ? np : min(A.gs, G - g);
-                // (panel, group) pair x of the stage: its scales, and its MMA step s of 64 elements
-                auto scales = [&](uint32_t x, bool q) {
+                const uint32_t ng = min(A.gs, G - g), steps = min(2 * ng, (A.Lr.cols - 4 * g + 1) / 2);
+                // scales of panel x's group y, and of the query panels' group y
+                auto row_scales = [&](uint32_t x, uint32_t y) {
 #pragma unroll
-                    for (uint32_t h = 0; h < kSub; ++h) {
-                        scales_to_tmem(sfa + (x * kSub + h) * 4, cd0 + (as + x * a_item + h * (kFp4ScaleSub / 16)));
-                        if (q) scales_to_tmem(sfb + (x * kSub + h) * 4, cd0 + (bs + x * b_item + h * (kFp4ScaleSub / 16)));
-                    }
+                    for (uint32_t h = 0; h < kSub; ++h)
+                        scales_to_tmem<CTAS>(sfa + ((x * A.gs + y) * kSub + h) * 4, cd0 + (st + x * a_item + (y * kSub + h) * 32));
                 };
-                auto step = [&](uint32_t x, uint32_t s, uint32_t gx, uint32_t d, uint32_t acc) {
-                    // block 16: step s uses sub-block s; block 32: bytes 2s, 2s + 1 of the one sub-block
-                    const uint32_t h = BLOCK == 16 ? s * 4 : 0;
-                    mma_fp4<BLOCK>(d, ad0 + (as + x * a_item + s * a_step), bd0 + (bs + gx * b_item + s * b_step),
-                                   BLOCK == 16 ? idesc : idesc | (2 * s) << 4 | (2 * s) << 29, sfa + x * 4 * kSub + h,
-                                   sfb + gx * 4 * kSub + h, acc);
+                auto query_scales = [&](uint32_t y) {
+#pragma unroll
+                    for (uint32_t h = 0; h < kSub; ++h)
+#pragma unroll
+                        for (uint32_t j = 0; j < CTAS; ++j)
+                            scales_to_tmem<CTAS>(sfb + ((y * kSub + h) * CTAS + j) * 4, cd0 + (st + b_off + j * q2 + (y * kSub + h) * 32));
+                };
+                // MMA step s of 64 elements of panel x (two steps to a group)
+                auto step = [&](uint32_t x, uint32_t s, uint32_t acc) {
+                    // block 16: a step has its own sub-block; block 32: bytes 2s, 2s + 1 of the group's
+                    const uint32_t sub = BLOCK == 16 ? s : s / 2, byte = BLOCK == 16 ? 0u : 2 * (s & 1u);
+                    mma_fp4<BLOCK, CTAS>(d0 + x * A.nt, ad0 + (st + x * a_item + s * a_step), bd0 + (st + s * b_step),
+                                         idesc | byte << 4 | byte << 29, sfa + (x * A.gs * kSub + sub) * 4,
+                                         sfb + sub * CTAS * 4, acc);
                 };
                 if (elect_one()) {
-                    if (A.pb == 1 && (!last || (items == 2 && A.Lr.last_cols > 2))) {  // two groups, both steps
-                        scales(0, true);
-                        scales(1, true);
-                        step(0, 0, 0, d0, g);
-                        step(0, 1, 0, d0, 1);
-                        step(1, 0, 1, d0, 1);
-                        step(1, 1, 1, d0, 1);
-                    } else if (items == 4 && A.Lr.last_cols > 2) {  // four panels, both steps
+                    // the usual full stages as straight code: kGs groups of a panel, one group of four panels
+                    if (np == 1 && steps == 2 * kGs) {
 #pragma unroll
-                        for (uint32_t x = 0; x < 4; ++x) scales(x, x == 0);
+                        for (uint32_t y = 0; y < kGs; ++y) {
+                            row_scales(0, y);
+                            query_scales(y);
+                        }
+                        step(0, 0, g);
+#pragma unroll
+                        for (uint32_t s = 1; s < 2 * kGs; ++s) step(0, s, 1);
+                    } else if (np == 4 && steps == 2) {
+                        query_scales(0);
+#pragma unroll
+                        for (uint32_t x = 0; x < 4; ++x) row_scales(x, 0);
 #pragma unroll
                         for (uint32_t x = 0; x < 4; ++x) {
-                            step(x, 0, 0, d0 + x * A.nt, 0);
-                            step(x, 1, 0, d0 + x * A.nt, 1);
+                            step(x, 0, 0);
+                            step(x, 1, 1);
                         }
                     } else {
-                        for (uint32_t x = 0; x < items; ++x) {
-                            const uint32_t gx = A.pb > 1 ? 0 : x, d = A.pb > 1 ? d0 + x * A.nt : d0;
-                            scales(x, x == 0 || A.pb == 1);
-                            step(x, 0, gx, d, g + gx);
-                            if (g + gx + 1 < G || A.Lr.last_cols > 2) step(x, 1, gx, d, 1);
+                        for (uint32_t y = 0; y < ng; ++y) query_scales(y);
+                        for (uint32_t x = 0; x < np; ++x) {
+                            for (uint32_t y = 0; y < ng; ++y) row_scales(x, y);
+                            for (uint32_t s = 0; s < steps; ++s) step(x, s, g | s);
                         }
                     }
-                    mma_commit(&empty[ring.i]);  // the stage is free once these MMAs have read it
-                    if (last) mma_commit(&tfull[accs.i]);
+                    mma_commit<CTAS>(&empty[ring.i]);  // the stage is free once these MMAs have read it
+                    if (g + ng == G) mma_commit<CTAS>(&tfull[accs.i]);
                 }
                 __syncwarp();
             }
@@ -313,27 +418,27 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         }
         if (!ok) *stop = 1u;
         // every MMA has completed before TMEM is released
-        if (elect_one()) mma_commit(drain);
+        if (elect_one()) mma_commit<CTAS>(drain);
         __syncwarp();
         uint32_t p = 0;
-        while (!mbar_try_wait(drain, 0, 1000) && ++p < A.polls) {
+        while (!mbar_try(drain, 0) && ++p < A.polls) {
         }
-        if (p >= A.polls) *stop = 1u;
         __syncwarp();
     } else {
         // -------------------------------------------------------------- epilogue warps
-        constexpr uint32_t kBatch = 4;  // chunks read before any is stored
+        constexpr uint32_t kBatch = CTAS == 2 ? 8 : 4;  // chunks read before any is stored
         const uint32_t qq = warp & 3u, h = (warp - 2) >> 2;  // lane quarter, half
         const uint32_t acc_cols = A.pb * A.nt;
         T* out = static_cast<T*>(A.out);
         bool ok = true;
         uint32_t u = 0;
         Ring accs;
-        for (Tiles t(A.batches, A.qtiles); t.more(); t.next(), ++u, accs.next(A.acc)) {
+        for (Tiles t(worker, workers, A.batches, A.qtiles); t.more(); t.next(), ++u, accs.next(A.acc)) {
             if (!split && (u & 1u) != h) continue;
-            const uint32_t p0 = t.p * A.pb, q0 = t.q * A.nt;
+            const uint32_t p0 = t.p * A.pb * CTAS + rank, q0 = t.q * A.nt;
+            const uint32_t np = CTAS == 2 ? 1u : min(A.pb, A.panels - p0);
             const uint32_t rows = min(A.nt, A.m - q0);
-            const uint32_t chunks = min(A.pb, A.panels - p0) * cpp, x0 = split ? h : 0, dx = split ? 2 : 1;
+            const uint32_t chunks = np * cpp, x0 = split ? h : 0, dx = split ? 2 : 1;
             const uint32_t addr = tmem + (qq * 32 << 16) + accs.i * acc_cols;
             if (ok) {
                 ok = __all_sync(kFull, bwait(&tfull[accs.i], accs.par, stop, A.polls));
@@ -351,14 +456,19 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
                     if (x + kBatch * dx >= chunks) {  // the accumulator's last read by this warp
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&tempty[accs.i]);
+                        if (lane == 0) {
+                            if (rank == 0)
+                                mbar_arrive(&tempty[accs.i]);
+                            else
+                                arrive_at_leader(&tempty[accs.i]);
+                        }
                     }
                 }
 #pragma unroll
                 for (uint32_t y = 0; y < kBatch; ++y) {
                     const uint32_t xy = x + y * dx;
                     if (xy >= chunks) break;
-                    const uint32_t p = xy / cpp, c = (xy - p * cpp) * 16;
+                    const uint32_t p = CTAS == 2 ? 0u : xy / cpp, c = (xy - p * cpp) * 16;
                     const uint64_t j = (uint64_t)(p0 + p) * kFp4Rows + qq * 32 + lane;
                     T* dst = out + (uint64_t)(q0 + c) * A.ld + j;
                     if (j < A.n)
@@ -371,17 +481,24 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         }
         if (!ok) *stop = 1u;
     }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+    sync_all<CTAS>();
+    if (warp == 0) tmem_free<CTAS>(tmem);
 }
 
-template <typename T, uint32_t BLOCK>
-gf_status launch_product(ProdArgs A, uint32_t grid, uint32_t smem, cudaStream_t s) {
-    GF_CUDA(cudaFuncSetAttribute(fp4_product_kernel<T, BLOCK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    fp4_product_kernel<T, BLOCK><<<grid, kThreads, smem, s>>>(A);
-    GF_CUDA(cudaGetLastError());
+template <typename T, uint32_t BLOCK, uint32_t CTAS>
+gf_status launch_product(const ProdArgs& A, uint32_t grid, uint32_t smem, cudaStream_t s) {
+    GF_CUDA(cudaFuncSetAttribute(fp4_product_kernel<T, BLOCK, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {CTAS, 1, 1};
+    cfg.attrs = at;
+    cfg.numAttrs = CTAS > 1 ? 1 : 0;
+    GF_CUDA(cudaLaunchKernelEx(&cfg, fp4_product_kernel<T, BLOCK, CTAS>, A));
     return GF_OK;
 }
 
@@ -398,32 +515,40 @@ gf_status product(const void* q, uint32_t m, const void* r, uint32_t n, uint32_t
     A.m = m;
     A.n = n;
     A.panels = fp4_panels(n);
-    A.qtiles = fp4_panels(m);
+    A.qpanels = fp4_panels(m);
     A.out = out;
     A.ld = ld;
     A.scale = scale;
     A.polls = test_wait ? test_wait : kPolls;
     A.extra_tx = test_wait ? 16u : 0u;
-    A.nt = A.Lq.col_bytes / 16;
-    A.pb = A.gs = 1;
-    if (A.Lr.groups > 1)
-        A.gs = 2;
-    else  // several panels to a tile while two accumulators fit and every SM still has a tile
-        while (A.pb < 4 && 2 * A.pb * A.nt <= 128 && (uint64_t)A.panels * A.qtiles >= 2ull * A.pb * sms) A.pb *= 2;
-    const uint32_t sub = block == 16 ? 2 : 1;
-    A.batches = (A.panels + A.pb - 1) / A.pb;
-    const uint64_t tiles = (uint64_t)A.batches * A.qtiles;
+    const uint32_t sub = block == 16 ? 2 : 1, group = sub * kFp4ScaleSub + 4 * kFp4ColBytes;
+    // pairs of CTAs once their tiles, of 256 x 256, occupy every SM
+    const uint64_t pair_tiles = ((uint64_t)A.panels + 1) / 2 * ((A.qpanels + 1) / 2);
+    const uint32_t ctas = A.qpanels >= 2 && pair_tiles >= (uint64_t)sms / 2 ? 2 : 1;
+    const uint32_t qcol = A.Lq.col_bytes / 16;
+    A.nt = ctas == 2 ? 256 : qcol;
+    // a stage: up to four groups of a panel, or all groups of several panels while two accumulators fit and
+    // every SM still has a tile
+    A.gs = std::min(A.Lr.groups, stage_groups(block, ctas));
+    A.pb = 1;
+    A.qtiles = (A.qpanels + ctas - 1) / ctas;
+    if (ctas == 1 && A.gs == A.Lr.groups)
+        while (2 * A.pb * A.gs <= 4 && 2 * A.pb * A.nt <= 128 && (uint64_t)A.panels * A.qtiles >= 2ull * A.pb * sms) A.pb *= 2;
+    A.batches = (A.panels + A.pb * ctas - 1) / (A.pb * ctas);
     // the panels' part has room for whole groups: an MMA reads 128 rows of two columns whatever the panel has
-    A.b_off = A.pb * A.gs * (sub * kFp4ScaleSub + kFp4Group / kFp4Col * kFp4ColBytes);
-    A.stage_bytes = A.b_off + A.gs * A.Lq.group_bytes;
-    A.sf_cols = (A.pb + 1) * A.gs * 4 * sub;
-    A.stages = std::min(kMaxStages, (kSmemLimit - 1024) / A.stage_bytes);
+    A.b_off = A.pb * A.gs * group;
+    A.bc_off = A.b_off + ctas * A.gs * sub * kFp4ScaleSub;
+    A.stage_bytes = A.bc_off + A.gs * 4 * A.Lq.col_bytes;
+    A.sf_cols = (A.pb + ctas) * A.gs * 4 * sub;
+    A.stages = std::min({kMaxStages, (kSmemLimit - 1024) / A.stage_bytes, (kTmemCols - A.pb * A.nt) / A.sf_cols});
     A.acc = std::min(kMaxAcc, (kTmemCols - A.stages * A.sf_cols) / (A.pb * A.nt));
-    const uint32_t smem = A.stages * A.stage_bytes + (2 * kMaxStages + 2 * kMaxAcc + 1) * 8 + 16;
-    const uint32_t grid = (uint32_t)std::min<uint64_t>(tiles, (uint64_t)sms);
+    const uint32_t smem = A.stages * A.stage_bytes + (3 * kMaxStages + 2 * kMaxAcc + 1) * 8 + 16;
+    const uint64_t tiles = (uint64_t)A.batches * A.qtiles;
+    const uint32_t grid = ctas * (uint32_t)std::min<uint64_t>(tiles, (uint64_t)sms / ctas);
     auto go = [&](auto tag) {
         using T = decltype(tag);
-        return block == 16 ? launch_product<T, 16>(A, grid, smem, s) : launch_product<T, 32>(A, grid, smem, s);
+        if (ctas == 2) return block == 16 ? launch_product<T, 16, 2>(A, grid, smem, s) : launch_product<T, 32, 2>(A, grid, smem, s);
+        return block == 16 ? launch_product<T, 16, 1>(A, grid, smem, s) : launch_product<T, 32, 1>(A, grid, smem, s);
     };
     return dtype == GF_F32 ? go(float{}) : dtype == GF_F16 ? go(__half{}) : go(__nv_bfloat16{});
 }

@@ -465,11 +465,11 @@ typedef enum { GF_F32 = 0, GF_F16 = 1, GF_BF16 = 2 } gf_dtype;
  * become 0).  A block with an infinity or a NaN after the multiplication is held as NaN.
  *
  * The held form ("packed") is one array of gf_fp4_bytes(n, dim, block) bytes, 16-byte aligned:
- * panels of 128 rows (n < 128: one panel of h = n rounded up to 16 rows), in a panel groups of
- * 128 elements, in a group the scales and then columns of 32 elements (only those the row
- * has, in its last group).
+ * panels of 128 rows (n < 128: one panel of h = n rounded up to 16 rows), in a panel the scales of
+ * each group of 128 elements, then the codes of each column of 32 elements:
  *   scales:  for every 4 blocks 512 bytes; block b (of 4) of row r at (r % 32) * 16 + (r / 32) * 4 + b
- *   column:  16 h bytes (h = 128 in a full panel), row r at r * 16, element 2i in the low half of byte i, 2i + 1 in the high
+ *   column:  16 h bytes (h = 128 in a full panel), row r at r * 16, element 2i in the low half of
+ *            byte i, 2i + 1 in the high
  * r being the row in its panel.  Scales and codes past a row's end are 0; the bytes of rows
  * that the last panel lacks are neither written nor used.  gf_fp4_bytes is 0 for a bad shape
  * (dim = 0, or a block other than 16 and 32).

@@ -90,22 +90,20 @@ def test_packed_positions(block):
     rows = gf.quantize_fp4_host(x, 1.0, block)
     code, s, _ = held(x, 1.0, block)
     sub = 512 * (32 // block)
-    full = sub + 4 * 2048
-    panel = 2 * full + sub + 2 * 2048  # 300 = 128 + 128 + 44: the last group has 2 columns
+    panel = 3 * sub + 10 * 2048  # 300 elements: 3 groups' scales, 10 columns
     assert rows.packed.size == gf.lib().gf_fp4_bytes(n, dim, block) == 2 * panel
     t = e4m3_values()
     for i in (0, 1, 31, 32, 100, 127, 128, 199):
         for k in (0, 1, 15, 16, 31, 32, 97, 127, 128, 255, 256, 299):
-            base = (i // 128) * panel + (k // 128) * full
-            r, kg = i % 128, k % 128
-            byte = rows.packed[base + sub + (kg // 32) * 2048 + r * 16 + (kg % 32) // 2]
+            base, r = (i // 128) * panel, i % 128
+            byte = rows.packed[base + 3 * sub + (k // 32) * 2048 + r * 16 + (k % 32) // 2]
             nib = (byte >> (4 * (k & 1))) & 15
             c = code[i, k]
             assert MAGS[nib & 7] == abs(c) and bool(nib & 8) == bool(np.signbit(c))
-            b = kg // block
+            b = k // block
             s8 = rows.packed[base + (b // 4) * 512 + (r % 32) * 16 + (r // 32) * 4 + b % 4]
             assert (t[s8] if block == 16 else 2.0 ** (int(s8) - 127)) == s[i, k // block]
-    assert not rows.packed[panel + sub + (200 - 128) * 16:panel + sub + 2048].any()  # rows past n
+    assert not rows.packed[panel + 3 * sub + (200 - 128) * 16:panel + 3 * sub + 2048].any()  # rows past n
 
 
 @pytest.mark.parametrize("n,h", [(1, 16), (16, 16), (17, 32), (100, 112), (113, 128), (127, 128)])

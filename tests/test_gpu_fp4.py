@@ -23,12 +23,13 @@ def valid_bytes(packed, n, dim, block):
     at = 0
     for p in range(-(-n // 128)):
         rows = min(128, n - p * 128)
-        for k in range(0, dim, 128):
-            cols = min(4, -(-(dim - k) // 32))
+        for _ in range(0, dim, 128):
             sc = packed[at:at + sub].reshape(-1, 32, 4, 4).transpose(0, 2, 1, 3).reshape(-1, 128, 4)
             out.append(sc[:, :rows].ravel())
-            out.append(packed[at + sub:at + sub + cols * h * 16].reshape(cols, h, 16)[:, :rows].ravel())
-            at += sub + cols * h * 16
+            at += sub
+        cols = -(-dim // 32)
+        out.append(packed[at:at + cols * h * 16].reshape(cols, h, 16)[:, :rows].ravel())
+        at += cols * h * 16
     assert at == packed.size
     return np.concatenate(out)
 

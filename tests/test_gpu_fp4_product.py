@@ -57,9 +57,19 @@ def test_row_counts(n, block):
     check_exact(300, n, 100, block)
 
 
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("m,n,dim", [
+    (129, 19001, 96), (256, 18944, 128), (257, 12801, 32), (300, 20000, 33), (1000, 4993, 200), (2000, 2500, 1000),
+    (384, 9600, 520), (511, 9473, 384), (1500, 3200, 8192), (5000, 700, 640), (20000, 129, 160), (700, 20000, 416),
+])
+def test_pairs_of_ctas(m, n, dim, block):
+    """Enough tiles of 256 x 256 for pairs of CTAs, with odd panel counts on either side."""
+    check_exact(m, n, dim, block)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("block", [16, 32])
-@pytest.mark.parametrize("m,n,dim", [(1, 1000, 300), (20, 333, 128), (100, 100, 1000), (300, 501, 200)])
+@pytest.mark.parametrize("m,n,dim", [(700, 7001, 200), (1, 1000, 300), (20, 333, 128), (100, 100, 1000), (300, 501, 200)])
 def test_output_types(m, n, dim, block, dtype):
     check_exact(m, n, dim, block, dtype)
 
@@ -100,7 +110,7 @@ def test_scales_over_many_binades(block):
 
 
 @pytest.mark.parametrize("block", [16, 32])
-@pytest.mark.parametrize("m,n,dim", [(3, 300, 96), (70, 300, 200)])
+@pytest.mark.parametrize("m,n,dim", [(3, 300, 96), (70, 300, 200), (300, 19100, 168)])
 def test_non_finite_blocks(m, n, dim, block):
     """A NaN or infinity reaches its own row's or column's products and no others."""
     q, r = exact_rows(m, dim, block, 1), exact_rows(n, dim, block, 2)
@@ -123,7 +133,7 @@ def test_zero_rows():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("m,n,gap", [(3, 129, 0), (3, 129, 1), (40, 256, 8), (300, 131, 5), (130, 64, 3)])
+@pytest.mark.parametrize("m,n,gap", [(3, 129, 0), (3, 129, 1), (40, 256, 8), (300, 131, 5), (130, 64, 3), (301, 19003, 2)])
 def test_strided_output(dtype, m, n, gap):
     q, r = exact_rows(m, 96, 32, 1), gf.quantize_fp4(exact_rows(n, 96, 32, 2))
     want = gf.product_fp4(q, r, dtype)
@@ -213,9 +223,10 @@ def test_store_score_read_together():
     assert ((scores.gather(1, top).double() - again).abs() <= 2.0 ** -20 * ref).all()
 
 
-def test_waits_that_run_out():
+@pytest.mark.parametrize("m,n", [(20, 1000), (300, 19000)])
+def test_waits_that_run_out(m, n):
     """The timeout path: outputs owed become NaN, and the next call is sound."""
-    q, r = exact_rows(20, 300, 32, 1), exact_rows(1000, 300, 32, 2)
+    q, r = exact_rows(m, 300, 32, 1), exact_rows(n, 300, 32, 2)
     rows = gf.quantize_fp4(r)
     got = gf.product_fp4(q, rows, test_wait=4)
     assert torch.isnan(got).all()
