@@ -39,6 +39,7 @@ constexpr uint32_t kMaxStages = 8;
 constexpr uint32_t kMaxAcc = 8;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kPolls = 1u << 20;
+constexpr uint64_t kBandBytes = 32u << 20;  // of row panels, a quarter of L2
 constexpr uint32_t kSmemLimit = 227 * 1024;
 
 // Zeros for the second column of an MMA step that the rows' last group lacks: with zero codes on the
@@ -53,6 +54,7 @@ struct ProdArgs {
     const uint8_t *r, *q;
     Fp4Layout Lr, Lq;
     uint32_t m, n, panels, qpanels, batches, qtiles;  // batches: tiles along the rows
+    uint32_t band;                      // tiles along the rows that are walked for every query tile in turn
     uint32_t nt;                        // columns of an accumulator
     uint32_t pb, gs;                    // row panels of a CTA's tile and groups of a stage (pb > 1: gs is all groups)
     uint32_t acc, stages, stage_bytes;
@@ -206,19 +208,31 @@ struct Ring {
     }
 };
 
-// The tiles of worker i of w: i, i + w, ...; query tiles vary fastest.
+// The tiles of worker i of w: i, i + w, ...  The row panels are cut into bands; within a band the panels
+// vary fastest, then the query tiles, so that the tiles in flight write long runs of the same rows of out
+// while a band's panels, read once for every query tile, stay in L2.
 struct Tiles {
-    uint32_t p, q, dp, dq, qtiles, batches;
-    __device__ __forceinline__ Tiles(uint32_t i, uint32_t w, uint32_t batches_, uint32_t qtiles_)
-        : p(i / qtiles_), q(i % qtiles_), dp(w / qtiles_), dq(w % qtiles_), qtiles(qtiles_), batches(batches_) {}
-    __device__ __forceinline__ bool more() const { return p < batches; }
-    __device__ __forceinline__ void next() {
-        p += dp;
-        q += dq;
-        if (q >= qtiles) {
-            q -= qtiles;
-            ++p;
+    uint32_t p, q = 0, w, band, width, batches, qtiles;  // (here p counts from the band's first panel)
+    uint32_t first = 0;
+    __device__ __forceinline__ Tiles(uint32_t i, uint32_t w_, uint32_t band_, uint32_t batches_, uint32_t qtiles_)
+        : p(i), w(w_), band(band_), width(min(band_, batches_)), batches(batches_), qtiles(qtiles_) {
+        settle();
+    }
+    __device__ __forceinline__ void settle() {
+        while (first < batches && p >= width) {
+            p -= width;
+            if (++q == qtiles) {
+                q = 0;
+                first += width;
+                width = min(band, batches - first);
+            }
         }
+    }
+    __device__ __forceinline__ bool more() const { return first < batches; }
+    __device__ __forceinline__ uint32_t batch() const { return first + p; }
+    __device__ __forceinline__ void next() {
+        p += w;
+        settle();
     }
 };
 
@@ -270,8 +284,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         Ring ring;
         uint64_t filled = 0;
         const uint32_t pad = A.Lq.cols & 1u;  // the last group lacks the second column of an MMA step
-        for (Tiles t(worker, workers, A.batches, A.qtiles); ok && t.more(); t.next()) {
-            const uint32_t p0 = t.p * A.pb * CTAS + rank, np = p0 < A.panels ? min(A.pb, A.panels - p0) : 0u;
+        for (Tiles t(worker, workers, A.band, A.batches, A.qtiles); ok && t.more(); t.next()) {
+            const uint32_t p0 = t.batch() * A.pb * CTAS + rank, np = p0 < A.panels ? min(A.pb, A.panels - p0) : 0u;
             const uint32_t qp = t.q * CTAS + rank;
             for (uint32_t g = 0; g < G; g += A.gs, ring.next(A.stages), ++filled) {
                 // (a barrier's first wait, for the use before its first, returns at once)
@@ -318,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         // ------------------------- the other CTA of a pair: tells CTA 0 which of its stages are full
         bool ok = true;
         Ring ring;
-        for (Tiles t(worker, workers, A.batches, A.qtiles); ok && t.more(); t.next())
+        for (Tiles t(worker, workers, A.band, A.batches, A.qtiles); ok && t.more(); t.next())
             for (uint32_t g = 0; g < G; g += A.gs, ring.next(A.stages)) {
                 if (!(ok = __all_sync(kFull, bwait(&full[ring.i], ring.par, stop, A.polls)))) break;
                 if (lane == 0) arrive_at_leader(&pfull[ring.i]);
@@ -347,8 +361,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         const uint32_t sfb_off = A.pb * A.gs * 4 * kSub, q2 = A.gs * kScales;
         bool ok = true;
         Ring ring, accs;
-        for (Tiles t(worker, workers, A.batches, A.qtiles); t.more(); t.next(), accs.next(A.acc)) {
-            const uint32_t np = CTAS == 2 ? 1u : min(A.pb, A.panels - t.p * A.pb);
+        for (Tiles t(worker, workers, A.band, A.batches, A.qtiles); t.more(); t.next(), accs.next(A.acc)) {
+            const uint32_t np = CTAS == 2 ? 1u : min(A.pb, A.panels - t.batch() * A.pb);
             const uint32_t d0 = tmem + accs.i * acc_cols;
             if (!(ok = __all_sync(kFull, bwait(&tempty[accs.i], accs.par ^ 1u, stop, A.polls)))) break;
             tc_fence_after();
@@ -433,9 +447,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         bool ok = true;
         uint32_t u = 0;
         Ring accs;
-        for (Tiles t(worker, workers, A.batches, A.qtiles); t.more(); t.next(), ++u, accs.next(A.acc)) {
+        for (Tiles t(worker, workers, A.band, A.batches, A.qtiles); t.more(); t.next(), ++u, accs.next(A.acc)) {
             if (!split && (u & 1u) != h) continue;
-            const uint32_t p0 = t.p * A.pb * CTAS + rank, q0 = t.q * A.nt;
+            const uint32_t p0 = t.batch() * A.pb * CTAS + rank, q0 = t.q * A.nt;
             const uint32_t np = CTAS == 2 ? 1u : min(A.pb, A.panels - p0);
             const uint32_t rows = min(A.nt, A.m - q0);
             const uint32_t chunks = np * cpp, x0 = split ? h : 0, dx = split ? 2 : 1;
@@ -471,11 +485,18 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
                     const uint32_t p = CTAS == 2 ? 0u : xy / cpp, c = (xy - p * cpp) * 16;
                     const uint64_t j = (uint64_t)(p0 + p) * kFp4Rows + qq * 32 + lane;
                     T* dst = out + (uint64_t)(q0 + c) * A.ld + j;
-                    if (j < A.n)
+                    if (!ok)
 #pragma unroll
-                        for (uint32_t e = 0; e < 16; ++e)
-                            if (c + e < rows)
-                                store(dst + e * A.ld, ok ? __uint_as_float(v[y][e]) * A.scale : __int_as_float(0x7FC00000));
+                        for (uint32_t e = 0; e < 16; ++e) v[y][e] = 0x7FC00000u;
+                    if (j >= A.n) continue;
+                    if (c + 16 <= rows) {
+#pragma unroll
+                        for (uint32_t e = 0; e < 16; ++e, dst += A.ld) store(dst, __uint_as_float(v[y][e]) * A.scale);
+                    } else {
+#pragma unroll
+                        for (uint32_t e = 0; e < 16; ++e, dst += A.ld)
+                            if (c + e < rows) store(dst, __uint_as_float(v[y][e]) * A.scale);
+                    }
                 }
             }
         }
@@ -543,6 +564,7 @@ gf_status product(const void* q, uint32_t m, const void* r, uint32_t n, uint32_t
     A.stages = std::min({kMaxStages, (kSmemLimit - 1024) / A.stage_bytes, (kTmemCols - A.pb * A.nt) / A.sf_cols});
     A.acc = std::min(kMaxAcc, (kTmemCols - A.stages * A.sf_cols) / (A.pb * A.nt));
     const uint32_t smem = A.stages * A.stage_bytes + (3 * kMaxStages + 2 * kMaxAcc + 1) * 8 + 16;
+    A.band = (uint32_t)std::min<uint64_t>(A.batches, std::max<uint64_t>(8, kBandBytes / (A.Lr.panel_bytes * A.pb * ctas)));
     const uint64_t tiles = (uint64_t)A.batches * A.qtiles;
     const uint32_t grid = ctas * (uint32_t)std::min<uint64_t>(tiles, (uint64_t)sms / ctas);
     auto go = [&](auto tag) {
