@@ -569,40 +569,56 @@ def _fp4_need(ok: bool, what: str, msg: str) -> None:
         raise GarfieldError(1, what, msg)
 
 
+_FP4_DTYPES = {}
+
+
 def _fp4_dtype(dtype, what: str) -> int:
-    import torch
-    kinds = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-    _fp4_need(dtype in kinds, what, f"dtype {dtype} is not float32, float16 or bfloat16")
-    return kinds[dtype]
+    if not _FP4_DTYPES:
+        import torch
+        _FP4_DTYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    dt = _FP4_DTYPES.get(dtype)
+    if dt is None:
+        raise GarfieldError(1, what, f"dtype {dtype} is not float32, float16 or bfloat16")
+    return dt
 
 
 def _fp4_matrix(t, what: str, name: str):
     """(rows, columns, row stride) of a CUDA matrix whose rows are each without gaps."""
-    import torch
-    _fp4_need(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2, what, f"{name}: expected a 2-D CUDA tensor")
+    if not getattr(t, "is_cuda", False) or t.dim() != 2:
+        raise GarfieldError(1, what, f"{name}: expected a 2-D CUDA tensor")
     n, dim = t.shape
-    _fp4_need(0 < dim < 2 ** 32 and n < 2 ** 32, what, f"{name}: shape {tuple(t.shape)} out of range")
-    _fp4_need(dim == 1 or n == 0 or t.stride(1) == 1, what, f"{name}: the elements of a row must be adjacent")
-    ld = t.stride(0) if n > 1 else dim
-    _fp4_need(ld >= dim, what, f"{name}: rows overlap (stride {ld} below {dim})")
+    ld, step = t.stride()
+    if n <= 1:
+        ld = dim
+    if not (0 < dim < 2 ** 32 and n < 2 ** 32):
+        raise GarfieldError(1, what, f"{name}: shape {(n, dim)} out of range")
+    if step != 1 and dim > 1 and n > 0:
+        raise GarfieldError(1, what, f"{name}: the elements of a row must be adjacent")
+    if ld < dim:
+        raise GarfieldError(1, what, f"{name}: rows overlap (stride {ld} below {dim})")
     return n, dim, ld
 
 
+def _fp4_size(n: int, dim: int, block: int) -> int:
+    """gf_fp4_bytes: panels of 128 rows, in each the scales of every 128 elements, then columns of 32."""
+    rows = 128 if n >= 128 else -(-n // 16) * 16
+    return -(-n // 128) * (-(-dim // 128) * (16384 // block) + -(-dim // 32) * rows * 16)
+
+
 def _fp4_rows(rows, what: str):
-    import torch
-    _fp4_need(isinstance(rows, Fp4Rows), what, "expected Fp4Rows")
-    p = rows.packed
-    _fp4_need(isinstance(p, torch.Tensor) and p.is_cuda and p.dtype == torch.uint8 and p.is_contiguous(), what,
-              "Fp4Rows.packed: expected a contiguous uint8 CUDA tensor")
-    need = lib().gf_fp4_bytes(rows.n, rows.dim, rows.block)
-    _fp4_need(rows.dim > 0 and rows.block in (16, 32), what, f"dim {rows.dim}, block {rows.block}")
-    _fp4_need(p.numel() >= need, what, f"Fp4Rows.packed holds {p.numel()} bytes, {need} needed")
+    p = getattr(rows, "packed", None)
+    if not isinstance(rows, Fp4Rows) or not getattr(p, "is_cuda", False):
+        raise GarfieldError(1, what, "expected Fp4Rows on a GPU")
+    if rows.block not in (16, 32) or rows.dim <= 0 or rows.n < 0:
+        raise GarfieldError(1, what, f"n {rows.n}, dim {rows.dim}, block {rows.block}")
+    if p.element_size() != 1 or not p.is_contiguous() or p.numel() < _fp4_size(rows.n, rows.dim, rows.block):
+        raise GarfieldError(1, what, f"Fp4Rows.packed: expected {_fp4_size(rows.n, rows.dim, rows.block)} contiguous bytes")
     return p
 
 
 class _on_stream:
-    """Makes a tensor's device current, and the given stream of it (None: the device's current one),
-    so that what is allocated inside belongs to the stream that the kernels run on."""
+    """Makes a device current, and the given stream of it (None: the device's current one), so that
+    what is allocated inside belongs to the stream that the kernels run on."""
 
     def __init__(self, device, stream):
         import torch
@@ -614,39 +630,93 @@ class _on_stream:
     def __enter__(self):
         self.device.__enter__()
         self.ctx.__enter__()
-        return C.c_void_p(self.stream.cuda_stream)
+        return self.stream.cuda_stream
 
     def __exit__(self, *exc):
         self.ctx.__exit__(*exc)
         self.device.__exit__(*exc)
 
 
-def quantize_fp4(data, alpha: float = 1.0, block: int = 32, stream=None) -> Fp4Rows:
-    """gf_quantize_fp4: the rows of a float32, float16 or bfloat16 CUDA matrix, held in 4 bits."""
+def _fp4_run(device, stream, f, *args):
+    """f(raw stream, *args) with the device and the stream current.  The usual case, the current stream
+    of the current device, reads torch's raw handle: entering contexts costs more than a small call."""
+    import torch
+    if stream is None and device.index == torch._C._cuda_getDevice():
+        return f(torch._C._cuda_getCurrentRawStream(device.index), *args)
+    with _on_stream(device, stream) as s:
+        return f(s, *args)
+
+
+def _fp4_quantize(s, data, alpha, block):
     import torch
     what = "gf_quantize_fp4"
     n, dim, ld = _fp4_matrix(data, what, "data")
     dt = _fp4_dtype(data.dtype, what)
-    _fp4_need(block in (16, 32), what, f"block {block} is not 16 or 32")
-    with _on_stream(data.device, stream) as s:
-        packed = torch.empty(lib().gf_fp4_bytes(n, dim, block), dtype=torch.uint8, device=data.device)
-        _check(lib().gf_quantize_fp4(C.c_void_p(data.data_ptr()), dt, ld, n, dim, alpha, block,
-                                     C.c_void_p(packed.data_ptr()), s), what)
+    if block != 32 and block != 16:
+        raise GarfieldError(1, what, f"block {block} is not 16 or 32")
+    packed = torch.empty(_fp4_size(n, dim, block), dtype=torch.uint8, device=data.device)
+    st = lib().gf_quantize_fp4(data.data_ptr(), dt, ld, n, dim, alpha, block, packed.data_ptr(), s)
+    if st:
+        _check(st, what)
     return Fp4Rows(packed, n, dim, block, float(alpha))
+
+
+def quantize_fp4(data, alpha: float = 1.0, block: int = 32, stream=None) -> Fp4Rows:
+    """gf_quantize_fp4: the rows of a float32, float16 or bfloat16 CUDA matrix, held in 4 bits."""
+    if not getattr(data, "is_cuda", False):
+        raise GarfieldError(1, "gf_quantize_fp4", "data: expected a 2-D CUDA tensor")
+    return _fp4_run(data.device, stream, _fp4_quantize, data, alpha, block)
+
+
+def _fp4_out(out, m: int, n: int, dtype, device, what: str):
+    """(out, its row stride): a new m x n tensor, or the caller's, checked."""
+    import torch
+    if out is None:
+        return torch.empty((m, n), dtype=dtype, device=device), n
+    if not getattr(out, "is_cuda", False) or tuple(out.shape) != (m, n) or out.dtype != dtype or out.device != device:
+        raise GarfieldError(1, what, f"out: expected a {dtype} tensor of shape {(m, n)} on {device}")
+    return out, (_fp4_matrix(out, what, "out")[2] if m and n else n)
+
+
+def _fp4_dequantize(s, p, rows, dtype, out):
+    what = "gf_dequantize_fp4"
+    dt = _fp4_dtype(dtype, what)
+    out, ld = _fp4_out(out, rows.n, rows.dim, dtype, p.device, what)
+    st = lib().gf_dequantize_fp4(p.data_ptr(), rows.n, rows.dim, rows.block, rows.alpha, out.data_ptr(), dt, ld, s)
+    if st:
+        _check(st, what)
+    return out
 
 
 def dequantize_fp4(rows: Fp4Rows, dtype=None, out=None, stream=None):
     """gf_dequantize_fp4: the values that rows are held as (n x dim, float32 unless dtype or out say
     otherwise)."""
     import torch
-    what = "gf_dequantize_fp4"
-    p = _fp4_rows(rows, what)
+    p = _fp4_rows(rows, "gf_dequantize_fp4")
     dtype = dtype or (out.dtype if out is not None else torch.float32)
+    return _fp4_run(p.device, stream, _fp4_dequantize, p, rows, dtype, out)
+
+
+def _fp4_product(s, queries, p, rows, dtype, out, query_alpha, test_wait):
+    what = "gf_product_fp4"
     dt = _fp4_dtype(dtype, what)
-    with _on_stream(p.device, stream) as s:
-        out = _fp4_out(out, (rows.n, rows.dim), dtype, p.device, what)
-        _check(lib().gf_dequantize_fp4(C.c_void_p(p.data_ptr()), rows.n, rows.dim, rows.block, rows.alpha,
-                                       C.c_void_p(out.data_ptr()), dt, out.stride(0) if rows.n > 1 else rows.dim, s), what)
+    if not isinstance(queries, Fp4Rows):
+        if getattr(queries, "device", None) != p.device:
+            raise GarfieldError(1, what, f"queries: expected Fp4Rows or a CUDA tensor on {p.device}")
+        queries = _fp4_quantize(s, queries, query_alpha, rows.block)
+        qp = queries.packed
+    else:
+        qp = _fp4_rows(queries, what)
+        if qp.device != p.device:
+            raise GarfieldError(1, what, f"queries on {qp.device}, rows on {p.device}")
+    if queries.dim != rows.dim or queries.block != rows.block:
+        raise GarfieldError(1, what, f"queries of dim {queries.dim}, block {queries.block}; rows of dim {rows.dim}, "
+                                     f"block {rows.block}")
+    out, ld = _fp4_out(out, queries.n, rows.n, dtype, p.device, what)
+    st = lib().gf_product_fp4(qp.data_ptr(), queries.n, p.data_ptr(), rows.n, rows.dim, rows.block,
+                              1.0 / (queries.alpha * rows.alpha), out.data_ptr(), dt, ld, test_wait, s)
+    if st:
+        _check(st, what)
     return out
 
 
@@ -657,34 +727,9 @@ def product_fp4(queries, rows: Fp4Rows, dtype=None, out=None, query_alpha: float
     bfloat16 CUDA matrix, which is held in 4 bits (quantize_fp4 with query_alpha and the rows'
     block) for the call."""
     import torch
-    what = "gf_product_fp4"
-    p = _fp4_rows(rows, what)
+    p = _fp4_rows(rows, "gf_product_fp4")
     dtype = dtype or (out.dtype if out is not None else torch.float32)
-    dt = _fp4_dtype(dtype, what)
-    with _on_stream(p.device, stream) as s:
-        if isinstance(queries, torch.Tensor):
-            _fp4_need(queries.device == p.device, what, f"queries on {queries.device}, rows on {p.device}")
-            queries = quantize_fp4(queries, query_alpha, rows.block)
-        qp = _fp4_rows(queries, what)
-        _fp4_need(qp.device == p.device, what, f"queries on {qp.device}, rows on {p.device}")
-        _fp4_need((queries.dim, queries.block) == (rows.dim, rows.block), what,
-                  f"queries of dim {queries.dim}, block {queries.block}; rows of dim {rows.dim}, block {rows.block}")
-        out = _fp4_out(out, (queries.n, rows.n), dtype, p.device, what)
-        _check(lib().gf_product_fp4(C.c_void_p(qp.data_ptr()), queries.n, C.c_void_p(p.data_ptr()), rows.n, rows.dim,
-                                    rows.block, 1.0 / (queries.alpha * rows.alpha), C.c_void_p(out.data_ptr()), dt,
-                                    out.stride(0) if queries.n > 1 and rows.n else rows.n, test_wait, s), what)
-    return out
-
-
-def _fp4_out(out, shape, dtype, device, what: str):
-    import torch
-    if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    _fp4_need(isinstance(out, torch.Tensor) and out.is_cuda and tuple(out.shape) == shape and out.dtype == dtype
-              and out.device == device, what, f"out: expected a {dtype} tensor of shape {shape} on {device}")
-    if out.numel():
-        _fp4_matrix(out, what, "out")
-    return out
+    return _fp4_run(p.device, stream, _fp4_product, queries, p, rows, dtype, out, query_alpha, test_wait)
 
 
 def quantize_fp4_host(data: np.ndarray, alpha: float = 1.0, block: int = 32) -> Fp4Rows:
@@ -692,7 +737,7 @@ def quantize_fp4_host(data: np.ndarray, alpha: float = 1.0, block: int = 32) -> 
     data = np.ascontiguousarray(data, dtype=np.float32)
     n, dim = data.shape
     _fp4_need(dim > 0 and block in (16, 32), "gf_quantize_fp4_host", f"dim {dim}, block {block}")
-    packed = np.empty(lib().gf_fp4_bytes(n, dim, block), np.uint8)
+    packed = np.empty(_fp4_size(n, dim, block), np.uint8)
     _check(lib().gf_quantize_fp4_host(_np_ptr(data), n, dim, alpha, block, _np_ptr(packed)), "gf_quantize_fp4_host")
     return Fp4Rows(packed, n, dim, block, float(alpha))
 
@@ -703,7 +748,7 @@ def dequantize_fp4_host(rows: Fp4Rows) -> np.ndarray:
     p = rows.packed
     _fp4_need(isinstance(p, np.ndarray) and p.dtype == np.uint8 and p.flags["C_CONTIGUOUS"], what,
               "Fp4Rows.packed: expected a contiguous uint8 array")
-    _fp4_need(p.size >= lib().gf_fp4_bytes(rows.n, rows.dim, rows.block), what, "Fp4Rows.packed is too short")
+    _fp4_need(p.size >= _fp4_size(rows.n, rows.dim, rows.block), what, "Fp4Rows.packed is too short")
     out = np.empty((rows.n, rows.dim), np.float32)
     _check(lib().gf_dequantize_fp4_host(_np_ptr(p), rows.n, rows.dim, rows.block, rows.alpha, _np_ptr(out)), what)
     return out

@@ -150,6 +150,14 @@ def test_empty():
     assert r.packed.size == 0 and gf.dequantize_fp4_host(r).shape == (0, 7)
 
 
+def test_sizes_agree():
+    """The size that Python allocates is gf_fp4_bytes."""
+    for n in (0, 1, 15, 16, 17, 100, 127, 128, 129, 1000, 2 ** 31):
+        for dim in (1, 31, 32, 33, 128, 129, 300, 8192, 100_000):
+            for block in (16, 32):
+                assert gf._fp4_size(n, dim, block) == gf.lib().gf_fp4_bytes(n, dim, block)
+
+
 def test_size_of_bad_shapes():
     L = gf.lib()
     assert L.gf_fp4_bytes(5, 0, 32) == 0 and L.gf_fp4_bytes(5, 8, 8) == 0
