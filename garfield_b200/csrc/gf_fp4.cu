@@ -14,9 +14,19 @@
 // the multiplication by alpha) gets a NaN scale (0xFF, 0x7F) and codes 0, so what is read back
 // and every product with it is NaN.
 //
-// x / s is an IEEE division before the rounding to a code, and that double rounding is harmless:
-// s has at most 4 significant bits and a code boundary at most 3, so x either equals
-// boundary * s or differs from it by at least 2^-24 of its value, which the fp32 quotient keeps.
+// x / s is rounded to fp32 before it is rounded to a code, and that double rounding is harmless: s
+// has at most 4 significant bits and a code boundary at most 3, so x either equals boundary * s or
+// differs from it by at least 2^-24 of its value, which the fp32 quotient keeps.
+//
+// Both directions move 2.5 to 4.5 bytes an element, which leaves some 15 to 27 instructions for one at the
+// HBM rate.  The quantiser's threads take eight consecutive elements: one to four loads, one
+// 4-byte word of codes, and the block maximum in two shuffles (one for blocks of 16).  Four
+// neighbouring lanes hold a row's column of 32 elements and the next lanes the next row, so a warp's
+// codes fill whole 32-byte sectors of the panel.  The reader's threads take what one store
+// holds (16 bytes, or 8, as the rows are aligned; else four elements), so a warp's stores leave no sector
+// half written.  A CTA is short (one group of a panel); six of them on an SM overlap their loads and arithmetic.
+// (2 rows in flight per thread and 6 CTAs: bf16 1M x 128 in 66 us; 4 rows and the 4 CTAs that
+// their registers allow: 74; 8 rows: 86.)
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
@@ -31,8 +41,7 @@ namespace gf {
 namespace {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kWarps = kThreads / 32;
-constexpr uint32_t kColPitch = kFp4ColBytes + 16;  // shared-memory columns, one bank quad apart
+constexpr uint32_t kOct = 8;  // elements of a quantiser's thread
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
@@ -41,16 +50,19 @@ __device__ __forceinline__ void from_f32(float v, float& o) { o = v; }
 __device__ __forceinline__ void from_f32(float v, __half& o) { o = __float2half_rn(v); }
 __device__ __forceinline__ void from_f32(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
 
-// Four consecutive elements in one load or store.
-template <typename T>
-struct alignas(sizeof(T) * 4) Quad {
-    T v[4];
+// W bytes of elements.
+template <typename T, uint32_t W>
+struct alignas(W < 16 ? W : 16) Vec {
+    T v[W / sizeof(T)];
 };
 
-// Two codes from two floats: lo in bits 0-3, hi in bits 4-7 (nearest, ties to even, saturating).
-__device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
+// Eight codes from eight floats, element i in bits 4i .. 4i + 3 (nearest, ties to even, saturating).
+__device__ __forceinline__ uint32_t e2m1x8(const float* x) {
     uint32_t r;
-    asm("{\n .reg .b8 b;\n cvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\n cvt.u32.u8 %0, b;\n}\n" : "=r"(r) : "f"(hi), "f"(lo));
+    asm("{\n .reg .b8 a, b, c, d;\n cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n mov.b32 %0, {a, b, c, d};\n}\n"
+        : "=r"(r)
+        : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]));
     return r;
 }
 // Two floats from a byte of two codes.
@@ -68,149 +80,213 @@ __device__ __forceinline__ float scale_to_f32(uint32_t b, bool block16) {
     return __uint_as_float(b == 255u ? 0x7FC00000u : (b == 0u ? 0x00400000u : b << 23));
 }
 
-// Scale byte of a block from the bits of amax, and the codes of this lane's four elements.
+// max(|a|, |b|), NaN if either is.
+__device__ __forceinline__ float amax2(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return r;
+}
+// Largest magnitude of eight elements, NaN if one is; 16-bit elements are compared in pairs.
+__device__ __forceinline__ float amax8(const float* v) {
+    return amax2(amax2(amax2(v[0], v[1]), amax2(v[2], v[3])), amax2(amax2(v[4], v[5]), amax2(v[6], v[7])));
+}
+__device__ __forceinline__ float amax8(const __half* v) {
+    const __half2* h = reinterpret_cast<const __half2*>(v);
+    const __half2 a = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+    return amax2(__low2float(a), __high2float(a));
+}
+__device__ __forceinline__ float amax8(const __nv_bfloat16* v) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(v);
+    const __nv_bfloat162 a = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+    return amax2(__low2float(a), __high2float(a));
+}
+// x / y correctly rounded, for r = 1 / y correctly rounded and results that are normal: one exact
+// remainder corrects the product (Markstein, IBM J. Res. Dev. 34, 1990).  Results too small for that are far
+// below the first code boundary.  (In this order of signs -0 / y stays -0.)
+__device__ __forceinline__ float div_by(float x, float y, float r) {
+    const float q = __fmul_rn(x, r);
+    return __fmaf_rn(-__fmaf_rn(q, y, -x), r, q);
+}
+
+// Scale byte of a block from its largest magnitude, and the codes of this thread's eight elements.
 template <uint32_t BLOCK>
-__device__ __forceinline__ uint32_t encode4(const float* x, float amax, uint32_t& codes) {
+__device__ __forceinline__ uint32_t encode8(float* x, float amax, uint32_t& codes) {
     const uint32_t ef = __float_as_uint(amax) >> 23;
+    uint32_t s8;
     if (BLOCK == 32) {
-        const uint32_t s8 = ef == 255u ? 255u : (ef >= 2u ? ef - 2u : 0u);
-        if (ef == 255u) {
-            codes = 0;
-            return s8;
+        s8 = ef == 255u ? 255u : max(ef, 2u) - 2u;
+        const float inv = __uint_as_float((254u - min(s8, 253u)) << 23);  // 1 / s, a power of two
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(x[e], inv);
+    } else {
+        s8 = ef == 255u ? 0x7Fu
+                        : (uint32_t)__nv_cvt_float_to_fp8(div_by(amax, 6.0f, 1.0f / 6.0f), __NV_SATFINITE, __NV_E4M3);
+        const float s = e4m3_to_f32(s8), r = __frcp_rn(s);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {  // div_by, two at a time
+            const dev::f2x v = dev::pack2(x[e], x[e + 1]), r2 = dev::pack2(r, r), q = dev::mul2(v, r2);
+            const dev::f2x nr = dev::fma2(q, dev::pack2(s, s), dev::pack2(-x[e], -x[e + 1]));
+            const dev::f2x y = dev::fma2(nr, dev::pack2(-r, -r), q);
+            x[e] = dev::lo2(y);
+            x[e + 1] = dev::hi2(y);
         }
-        const float inv = __uint_as_float((254u - s8) << 23);  // 1 / s, a power of two
-        codes = e2m1x2(x[0] * inv, x[1] * inv) | e2m1x2(x[2] * inv, x[3] * inv) << 8;
-        return s8;
     }
-    const uint32_t s8 = ef == 255u ? 0x7Fu : (uint32_t)__nv_cvt_float_to_fp8(__fdiv_rn(amax, 6.0f), __NV_SATFINITE, __NV_E4M3);
-    if (ef == 255u || s8 == 0u) {
-        codes = 0;
-        return s8;
-    }
-    const float s = e4m3_to_f32(s8);
-    codes = e2m1x2(__fdiv_rn(x[0], s), __fdiv_rn(x[1], s)) | e2m1x2(__fdiv_rn(x[2], s), __fdiv_rn(x[3], s)) << 8;
+    codes = ef == 255u || (BLOCK == 16 && s8 == 0u) ? 0u : e2m1x8(x);
     return s8;
 }
 
-// One group of one panel per block step.  A warp takes a row's 128 elements, four to a lane, so
-// its load is one contiguous run of 512 (fp32) or 256 bytes; the block maximum is a butterfly over the
-// 8 or 4 lanes of the block; codes and scales gather in shared memory in the panel's order and
-// leave as 16-byte pieces.  VEC: rows start on a four-element boundary and dim % 4 == 0.
-template <typename T, uint32_t BLOCK, bool VEC>
-__global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const T* __restrict__ data, uint64_t ld, uint32_t n,
+// Lanes of a row, as a power of two: enough for `cols` columns at `per` lanes each (per a power of two).
+__device__ __forceinline__ uint32_t row_shift(uint32_t cols, uint32_t per) {
+    return 31u - __clz(per) + (cols > 2 ? 2u : cols - 1u);
+}
+
+// One group of one panel.  W: bytes of a load, which rows are aligned to.
+template <typename T, uint32_t BLOCK, uint32_t W>
+__global__ void __launch_bounds__(kThreads, 6) fp4_quantize_kernel(const T* __restrict__ data, uint64_t ld, uint32_t n,
                                                                 uint32_t dim, float alpha, uint8_t* __restrict__ packed,
-                                                                Fp4Layout Lo, uint64_t tiles) {
+                                                                Fp4Layout Lo) {
     constexpr uint32_t kSb = kFp4Group / BLOCK * kFp4Rows;  // scale bytes of a group
-    constexpr int U = 8;                                    // rows in flight per warp
-    __shared__ __align__(16) uint8_t codes_s[4 * kColPitch];
+    constexpr uint32_t kV = W / sizeof(T);                  // elements of a load
+    constexpr uint32_t kBo = BLOCK / kOct;                  // threads of a block
+    constexpr uint32_t kRows = 2;                           // rows in flight per thread: at most 64 * 2 per step
     __shared__ __align__(16) uint8_t scales_s[kSb];
-    const uint32_t lane = dev::lane_id(), warp = threadIdx.x >> 5;
-    for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-        const uint32_t p = (uint32_t)(t / Lo.groups), g = (uint32_t)(t % Lo.groups);
+    const uint32_t p = blockIdx.x;
+    for (uint32_t g = blockIdx.y; g < Lo.groups; g += gridDim.y) {
         const uint32_t row0 = p * kFp4Rows, valid = min(kFp4Rows, n - row0);
-        const uint32_t cols = min(4u, Lo.cols - 4 * g);
-        const uint32_t k = g * kFp4Group + lane * 4;
-        for (uint32_t r0 = warp; r0 < valid; r0 += kWarps * U) {
-            float x[U][4];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const uint32_t r = r0 + u * kWarps;
-                const T* src = data + (uint64_t)(row0 + r) * ld + k;
-                if (VEC) {
-                    Quad<T> q = {};
-                    if (r < valid && k < dim) q = *reinterpret_cast<const Quad<T>*>(src);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[u][e] = __fmul_rn(to_f32(q.v[e]), alpha);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        x[u][e] = r < valid && k + e < dim ? __fmul_rn(to_f32(src[e]), alpha) : 0.0f;
-                }
+        const uint32_t cols = min(4u, Lo.cols - 4 * g), lsh = row_shift(cols, 4);
+        const uint32_t o = threadIdx.x & ((1u << lsh) - 1u), rstep = kThreads >> lsh;
+        const uint32_t k = g * kFp4Group + o * kOct, first = threadIdx.x >> lsh;
+        const uint32_t left = k < dim ? dim - k : 0u;  // elements of the row from k on
+        const T* src = data + (uint64_t)(row0 + first) * ld + k;
+        const uint64_t step = ld * rstep;
+        uint8_t* dst = packed + Lo.col_at(p, 4 * g + (o >> 2)) + (o & 3u) * 4;
+        // scales of blocks in columns that the group lacks are 0
+        if (cols < 4)
+            for (uint32_t i = threadIdx.x; i < kFp4Rows * (128 / BLOCK); i += kThreads) {
+                const uint32_t b = i / kFp4Rows;
+                if (b * BLOCK >= cols * kFp4Col) scales_s[fp4_scale_at(i % kFp4Rows, b)] = 0;
             }
+        typedef Vec<T, W> Oct[kOct / kV];
+        auto encode = [&](const Oct& q, uint32_t r, bool in) {
+            T v[kOct];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const uint32_t r = r0 + u * kWarps;
-                // the bits of |x| order like |x|, with NaN above infinity: an integer maximum
-                // sees every non-finite element
-                uint32_t mb = 0;
+            for (uint32_t e = 0; e < kOct; ++e) v[e] = q[e / kV].v[e % kV];
+            float x[kOct], mx = amax8(v);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mb = max(mb, __float_as_uint(x[u][e]) & 0x7FFFFFFFu);
+            for (uint32_t e = 0; e < kOct; ++e) x[e] = to_f32(v[e]);
+            if (alpha != 1.0f) {  // (rounding keeps order: the largest product is the largest element's)
+                mx = __fmul_rn(mx, alpha);
 #pragma unroll
-                for (int o = BLOCK / 8; o > 0; o >>= 1) mb = max(mb, __shfl_xor_sync(dev::kFull, mb, o));
-                uint32_t c;
-                const uint32_t s8 = encode4<BLOCK>(x[u], __uint_as_float(mb), c);
-                if (r < valid) {
-                    *reinterpret_cast<uint16_t*>(codes_s + (lane >> 3) * kColPitch + r * 16 + (lane & 7u) * 2) = (uint16_t)c;
-                    if (lane % (BLOCK / 4) == 0) scales_s[fp4_scale_at(r, lane / (BLOCK / 4))] = (uint8_t)s8;
+                for (uint32_t e = 0; e < kOct; ++e) x[e] = __fmul_rn(x[e], alpha);
+            }
+            if (BLOCK == 32) mx = amax2(mx, __shfl_xor_sync(dev::kFull, mx, 2));
+            mx = amax2(mx, __shfl_xor_sync(dev::kFull, mx, 1));
+            uint32_t c;
+            const uint32_t s8 = encode8<BLOCK>(x, mx, c);
+            if (in) {
+                *reinterpret_cast<uint32_t*>(dst + r * 16) = c;
+                if (o % kBo == 0) scales_s[fp4_scale_at(r, o / kBo)] = (uint8_t)s8;  // (0 for a block past the row's end)
+            }
+        };
+        if (valid == kFp4Rows && dim % kOct == 0) {  // every thread has eight elements or none, in every row
+            for (uint32_t r0 = 0; r0 < kFp4Rows; r0 += rstep * kRows) {
+                Oct q[kRows] = {};
+                if (left) {
+#pragma unroll
+                    for (uint32_t u = 0; u < kRows; ++u)
+#pragma unroll
+                        for (uint32_t w = 0; w < kOct / kV; ++w)
+                            q[u][w] = *reinterpret_cast<const Vec<T, W>*>(src + u * step + w * kV);
                 }
+                src += step * kRows;
+#pragma unroll
+                for (uint32_t u = 0; u < kRows; ++u) encode(q[u], r0 + first + u * rstep, o < 4 * cols);
+            }
+        } else {
+            for (uint32_t r0 = 0; r0 < valid; r0 += rstep, src += step) {
+                const uint32_t r = r0 + first;
+                Oct q = {};
+                if (r < valid && left >= kOct) {
+#pragma unroll
+                    for (uint32_t w = 0; w < kOct / kV; ++w) q[w] = *reinterpret_cast<const Vec<T, W>*>(src + w * kV);
+                } else if (r < valid) {
+#pragma unroll
+                    for (uint32_t e = 0; e < kOct; ++e)
+                        if (e < left) q[e / kV].v[e % kV] = src[e];
+                }
+                encode(q, r, r < valid && o < 4 * cols);
             }
         }
         __syncthreads();
         uint32_t* dst_s = reinterpret_cast<uint32_t*>(packed + Lo.scales_at(p, g));
-        uint8_t* dst = packed + Lo.col_at(p, 4 * g);
         for (uint32_t i = threadIdx.x; i < kSb / 4; i += kThreads) {
             const uint32_t r = (i & 3u) * 32 + ((i >> 2) & 31u);
             if (r < valid) dst_s[i] = reinterpret_cast<const uint32_t*>(scales_s)[i];
-        }
-        for (uint32_t i = threadIdx.x; i < cols * kFp4Rows; i += kThreads) {
-            const uint32_t c = i / kFp4Rows, r = i % kFp4Rows;
-            if (r < valid)
-                *reinterpret_cast<uint4*>(dst + c * Lo.col_bytes + r * 16) =
-                    *reinterpret_cast<const uint4*>(codes_s + c * kColPitch + r * 16);
         }
         __syncthreads();
     }
 }
 
-// The reverse: a group's bytes come in as 16-byte pieces, a warp writes a row's 128 elements.
-// The scale is divided by alpha once per block (rounded), and the code times it rounded again: with
-// a power of two as alpha both are exact in fp32, otherwise a value is within 2^-23 of
-// c * s / alpha.
-template <typename T, uint32_t BLOCK, bool VEC>
-__global__ void __launch_bounds__(kThreads) fp4_dequantize_kernel(const uint8_t* __restrict__ packed, uint32_t n,
-                                                                  uint32_t dim, float alpha, T* __restrict__ out,
-                                                                  uint64_t ld, Fp4Layout Lo, uint64_t tiles) {
-    constexpr uint32_t kSb = kFp4Group / BLOCK * kFp4Rows;
-    __shared__ __align__(16) uint8_t codes_s[4 * kColPitch];
-    __shared__ __align__(16) uint8_t scales_s[kSb];
-    const uint32_t lane = dev::lane_id(), warp = threadIdx.x >> 5;
-    for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-        const uint32_t p = (uint32_t)(t / Lo.groups), g = (uint32_t)(t % Lo.groups);
+// The reverse.  W: bytes of a store.  inv is 1 / alpha rounded; the scale is multiplied by it once
+// per thread and the code times that rounded again: with a power of two as alpha all is exact in
+// fp32, otherwise a value is within 3 * 2^-24 of c * s / alpha.
+template <typename T, uint32_t BLOCK, uint32_t W>
+__global__ void __launch_bounds__(kThreads, 6) fp4_dequantize_kernel(const uint8_t* __restrict__ packed, uint32_t n,
+                                                                  uint32_t dim, float inv, T* __restrict__ out,
+                                                                  uint64_t ld, Fp4Layout Lo) {
+    constexpr uint32_t kV = W > sizeof(T) ? W / sizeof(T) : 4;  // elements of a thread: 2, 4 or 8
+    constexpr uint32_t kCb = kV / 2;                            // their bytes of codes
+    constexpr uint32_t kRows = 4;                               // rows in flight per thread
+    const uint32_t p = blockIdx.x;
+    for (uint32_t g = blockIdx.y; g < Lo.groups; g += gridDim.y) {
         const uint32_t row0 = p * kFp4Rows, valid = min(kFp4Rows, n - row0);
-        const uint32_t cols = min(4u, Lo.cols - 4 * g);
-        const uint32_t k = g * kFp4Group + lane * 4;
-        const uint4* src_s = reinterpret_cast<const uint4*>(packed + Lo.scales_at(p, g));
-        const uint8_t* src = packed + Lo.col_at(p, 4 * g);
-        for (uint32_t i = threadIdx.x; i < kSb / 16; i += kThreads) reinterpret_cast<uint4*>(scales_s)[i] = src_s[i];
-        for (uint32_t i = threadIdx.x; i < cols * kFp4Rows; i += kThreads) {
-            const uint32_t c = i / kFp4Rows, r = i % kFp4Rows;
-            if (r < valid)
-                *reinterpret_cast<uint4*>(codes_s + c * kColPitch + r * 16) =
-                    *reinterpret_cast<const uint4*>(src + c * Lo.col_bytes + r * 16);
-        }
-        __syncthreads();
-        if (k < dim) {
-#pragma unroll 4
-            for (uint32_t r = warp; r < valid; r += kWarps) {
-                const uint32_t c = *reinterpret_cast<const uint16_t*>(codes_s + (lane >> 3) * kColPitch + r * 16 + (lane & 7u) * 2);
-                const float s = __fdiv_rn(scale_to_f32(scales_s[fp4_scale_at(r, lane / (BLOCK / 4))], BLOCK == 16), alpha);
-                const float2 a = e2m1x2_to_f32(c & 255u), b = e2m1x2_to_f32(c >> 8);
-                Quad<T> q;
-                from_f32(__fmul_rn(a.x, s), q.v[0]);
-                from_f32(__fmul_rn(a.y, s), q.v[1]);
-                from_f32(__fmul_rn(b.x, s), q.v[2]);
-                from_f32(__fmul_rn(b.y, s), q.v[3]);
-                T* dst = out + (uint64_t)(row0 + r) * ld + k;
-                if (VEC) {
-                    *reinterpret_cast<Quad<T>*>(dst) = q;
-                } else {
+        const uint32_t lsh = row_shift(min(4u, Lo.cols - 4 * g), kFp4Col / kV);
+        const uint32_t k0 = (threadIdx.x & ((1u << lsh) - 1u)) * kV, rstep = kThreads >> lsh;  // element of the group
+        const uint32_t k = g * kFp4Group + k0;
+        if (k >= dim) continue;
+        const uint32_t left = dim - k;
+        const uint8_t* src = packed + Lo.col_at(p, 4 * g + k0 / kFp4Col) + k0 % kFp4Col / 2;
+        const uint8_t* src_s = packed + Lo.scales_at(p, g);
+        uint32_t r = threadIdx.x >> lsh;
+        T* dst = out + (uint64_t)(row0 + r) * ld + k;
+        const uint64_t step = ld * rstep;
+        auto codes_of = [&](uint32_t i) -> uint32_t {
+            return kCb == 4   ? *reinterpret_cast<const uint32_t*>(src + i * 16)
+                   : kCb == 2 ? *reinterpret_cast<const uint16_t*>(src + i * 16)
+                              : src[i * 16];
+        };
+        auto write = [&](uint32_t c, uint32_t s8, bool whole) {
+            const float s = __fmul_rn(scale_to_f32(s8, BLOCK == 16), inv);
+            Vec<T, kV * sizeof(T)> y;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (k + e < dim) dst[e] = q.v[e];
-                }
+            for (uint32_t e = 0; e < kV; e += 2) {
+                const float2 a = e2m1x2_to_f32((c >> (4 * e)) & 255u);
+                from_f32(__fmul_rn(a.x, s), y.v[e]);
+                from_f32(__fmul_rn(a.y, s), y.v[e + 1]);
             }
+            if (W > sizeof(T) && whole) {
+                *reinterpret_cast<decltype(y)*>(dst) = y;
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < kV; ++e)
+                    if (whole || e < left) dst[e] = y.v[e];
+            }
+            dst += step;
+        };
+        if (valid == kFp4Rows && left >= kV && rstep * kRows <= kFp4Rows) {
+            for (; r < kFp4Rows; r += rstep * kRows) {
+                uint32_t c[kRows], s8[kRows];
+#pragma unroll
+                for (uint32_t u = 0; u < kRows; ++u) {
+                    c[u] = codes_of(r + u * rstep);
+                    s8[u] = src_s[fp4_scale_at(r + u * rstep, k0 / BLOCK)];
+                }
+#pragma unroll
+                for (uint32_t u = 0; u < kRows; ++u) write(c[u], s8[u], true);
+            }
+        } else {
+            for (; r < valid; r += rstep) write(codes_of(r), src_s[fp4_scale_at(r, k0 / BLOCK)], left >= kV);
         }
-        __syncthreads();
     }
 }
 
@@ -283,41 +359,51 @@ void quantize_host(const float* data, uint32_t n, uint32_t dim, float alpha, uin
 
 void dequantize_host(const uint8_t* packed, uint32_t n, uint32_t dim, uint32_t block, float alpha, float* out) {
     const Fp4Layout Lo = fp4_layout(n, dim, block);
+    const float inv = 1.0f / alpha;
     for (uint32_t i = 0; i < n; ++i)
         for (uint32_t k = 0; k < dim; ++k) {
             const uint32_t r = i % kFp4Rows, p = i / kFp4Rows;
             const uint32_t c = (packed[Lo.col_at(p, k / kFp4Col) + r * 16 + (k % kFp4Col) / 2] >> (4 * (k & 1u))) & 15u;
             const uint32_t s8 = packed[Lo.scales_at(p, k / kFp4Group) + fp4_scale_at(r, k % kFp4Group / block)];
-            const float s = scale_host(s8, block) / alpha;
+            const float s = scale_host(s8, block) * inv;
             out[(uint64_t)i * dim + k] = (c & 8u ? -kMags[c & 7u] : kMags[c & 7u]) * s;
         }
 }
 
 // ------------------------------------------------------------------ launches
 
-bool good_alpha(float alpha) { return std::isfinite(alpha) && alpha > 0.0f; }
+// (so that 1 / alpha is a normal number too)
+bool good_alpha(float alpha) { return alpha >= 0x1p-126f && alpha <= 0x1p126f; }
 
-unsigned grid_of(uint64_t tiles) { return (unsigned)std::min<uint64_t>(tiles, 0x7FFFFFFFu); }
+
+// A CTA per panel and group (at most 2^25 panels).
+dim3 grid_of(uint32_t n, const Fp4Layout& Lo) { return dim3(fp4_panels(n), std::min(Lo.groups, 65535u)); }
+
+// Bytes that the rows of a matrix are all aligned to: 16, 8 or an element.
+uint32_t row_alignment(const void* p, uint64_t ld, uint32_t esize) {
+    const uint64_t a = reinterpret_cast<uintptr_t>(p) | ld * esize;
+    return a % 16 == 0 ? 16 : a % 8 == 0 ? 8 : esize;
+}
 
 template <typename T, uint32_t BLOCK>
 void launch_quantize(const void* data, uint64_t ld, uint32_t n, uint32_t dim, float alpha, uint8_t* packed, cudaStream_t s) {
     const Fp4Layout Lo = fp4_layout(n, dim, BLOCK);
-    const uint64_t tiles = (uint64_t)fp4_panels(n) * Lo.groups;
     const T* x = static_cast<const T*>(data);
-    if (aligned(data, 4 * sizeof(T)) && ld % 4 == 0 && dim % 4 == 0)
-        fp4_quantize_kernel<T, BLOCK, true><<<grid_of(tiles), kThreads, 0, s>>>(x, ld, n, dim, alpha, packed, Lo, tiles);
-    else
-        fp4_quantize_kernel<T, BLOCK, false><<<grid_of(tiles), kThreads, 0, s>>>(x, ld, n, dim, alpha, packed, Lo, tiles);
+    const uint32_t w = row_alignment(data, ld, sizeof(T));
+    auto* k = w == 16 ? fp4_quantize_kernel<T, BLOCK, 16>
+              : w == 8 ? fp4_quantize_kernel<T, BLOCK, 8>
+                       : fp4_quantize_kernel<T, BLOCK, sizeof(T)>;
+    k<<<grid_of(n, Lo), kThreads, 0, s>>>(x, ld, n, dim, alpha, packed, Lo);
 }
 template <typename T, uint32_t BLOCK>
 void launch_dequantize(const uint8_t* packed, uint32_t n, uint32_t dim, float alpha, void* out, uint64_t ld, cudaStream_t s) {
     const Fp4Layout Lo = fp4_layout(n, dim, BLOCK);
-    const uint64_t tiles = (uint64_t)fp4_panels(n) * Lo.groups;
     T* y = static_cast<T*>(out);
-    if (aligned(out, 4 * sizeof(T)) && ld % 4 == 0 && dim % 4 == 0)
-        fp4_dequantize_kernel<T, BLOCK, true><<<grid_of(tiles), kThreads, 0, s>>>(packed, n, dim, alpha, y, ld, Lo, tiles);
-    else
-        fp4_dequantize_kernel<T, BLOCK, false><<<grid_of(tiles), kThreads, 0, s>>>(packed, n, dim, alpha, y, ld, Lo, tiles);
+    const uint32_t w = row_alignment(out, ld, sizeof(T));
+    auto* k = w == 16 ? fp4_dequantize_kernel<T, BLOCK, 16>
+              : w == 8 ? fp4_dequantize_kernel<T, BLOCK, 8>
+                       : fp4_dequantize_kernel<T, BLOCK, sizeof(T)>;
+    k<<<grid_of(n, Lo), kThreads, 0, s>>>(packed, n, dim, 1.0f / alpha, y, ld, Lo);
 }
 
 }  // namespace
@@ -335,7 +421,7 @@ extern "C" gf_status gf_quantize_fp4(const void* data, uint32_t dtype, uint64_t 
                                      uint32_t block, void* packed_out, void* stream) {
     if (!fp4_shape(dim, block)) return fail(GF_ERR_ARG, "dim must be positive and block 16 or 32");
     if (!dtype_bytes(dtype)) return fail(GF_ERR_ARG, "unknown dtype");
-    if (!good_alpha(alpha)) return fail(GF_ERR_ARG, "alpha must be positive and finite");
+    if (!good_alpha(alpha)) return fail(GF_ERR_ARG, "alpha must lie in [2^-126, 2^126]");
     if (ld < dim) return fail(GF_ERR_ARG, "row stride below dim");
     if (n == 0) return GF_OK;
     if (!data || !packed_out) return fail(GF_ERR_ARG, "null argument");
@@ -363,7 +449,7 @@ extern "C" gf_status gf_dequantize_fp4(const void* packed, uint32_t n, uint32_t 
                                        uint32_t dtype, uint64_t ld, void* stream) {
     if (!fp4_shape(dim, block)) return fail(GF_ERR_ARG, "dim must be positive and block 16 or 32");
     if (!dtype_bytes(dtype)) return fail(GF_ERR_ARG, "unknown dtype");
-    if (!good_alpha(alpha)) return fail(GF_ERR_ARG, "alpha must be positive and finite");
+    if (!good_alpha(alpha)) return fail(GF_ERR_ARG, "alpha must lie in [2^-126, 2^126]");
     if (ld < dim) return fail(GF_ERR_ARG, "row stride below dim");
     if (n == 0) return GF_OK;
     if (!packed || !out) return fail(GF_ERR_ARG, "null argument");
@@ -390,7 +476,7 @@ extern "C" gf_status gf_dequantize_fp4(const void* packed, uint32_t n, uint32_t 
 extern "C" gf_status gf_quantize_fp4_host(const float* data, uint32_t n, uint32_t dim, float alpha, uint32_t block,
                                           void* packed_out) {
     if (!fp4_shape(dim, block)) return fail(GF_ERR_ARG, "dim must be positive and block 16 or 32");
-    if (!good_alpha(alpha)) return fail(GF_ERR_ARG, "alpha must be positive and finite");
+    if (!good_alpha(alpha)) return fail(GF_ERR_ARG, "alpha must lie in [2^-126, 2^126]");
     if (n == 0) return GF_OK;
     if (!data || !packed_out) return fail(GF_ERR_ARG, "null argument");
     quantize_host(data, n, dim, alpha, block, static_cast<uint8_t*>(packed_out));
@@ -400,7 +486,7 @@ extern "C" gf_status gf_quantize_fp4_host(const float* data, uint32_t n, uint32_
 extern "C" gf_status gf_dequantize_fp4_host(const void* packed, uint32_t n, uint32_t dim, uint32_t block, float alpha,
                                             float* out) {
     if (!fp4_shape(dim, block)) return fail(GF_ERR_ARG, "dim must be positive and block 16 or 32");
-    if (!good_alpha(alpha)) return fail(GF_ERR_ARG, "alpha must be positive and finite");
+    if (!good_alpha(alpha)) return fail(GF_ERR_ARG, "alpha must lie in [2^-126, 2^126]");
     if (n == 0) return GF_OK;
     if (!packed || !out) return fail(GF_ERR_ARG, "null argument");
     dequantize_host(static_cast<const uint8_t*>(packed), n, dim, block, alpha, out);

@@ -41,7 +41,8 @@ def same_bytes(rows, ref):
     assert np.array_equal(a, b), np.flatnonzero(a != b)[:10]
 
 
-SHAPES = [(1, 1), (1, 8192), (3, 96), (64, 31), (127, 32), (128, 128), (130, 33), (300, 300), (1000, 65), (513, 1000)]
+SHAPES = [(1, 1), (1, 8192), (3, 96), (64, 31), (127, 32), (128, 128), (130, 33), (300, 300), (1000, 65), (513, 1000),
+          (256, 8), (300, 16), (500, 24), (257, 32), (400, 5), (129, 48), (384, 64), (200, 2056)]
 
 
 @pytest.mark.parametrize("block", [16, 32])
