@@ -125,10 +125,12 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem) {
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// Arrival on the same barrier of the cluster's CTA 0, ordered after this thread's earlier accesses.
+// Arrival on the same barrier of the cluster's CTA 0.  (A release at cluster scope would hold the arrival
+// until this thread's stores to out have landed, and the tile's MMAs with it.  What the arrival reports is
+// done by then: bulk copies that completed on this CTA's barrier, or TMEM reads that were waited for.)
 __device__ __forceinline__ void arrive_at_leader(uint64_t* bar) {
     asm volatile(
-        "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, 0;\n mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n}\n" ::"r"(
+        "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, 0;\n mbarrier.arrive.shared::cluster.b64 _, [a];\n}\n" ::"r"(
             smem_u32(bar))
         : "memory");
 }
@@ -166,12 +168,11 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 // Bounded wait on a phase; false when it ran out or the CTA is stopping.  (The suspending form of
-// the test takes longer to answer than the plain one, so a few of those come first.)  Arrivals may
-// come from the pair's other CTA, hence the cluster scope.
+// the test takes longer to answer than the plain one, so a few of those come first.)
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t par) {
     uint32_t ok;
     asm volatile(
-        "{\n .reg .pred p;\n mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
         : "=r"(ok)
         : "r"(smem_u32(bar)), "r"(par)
         : "memory");
@@ -180,7 +181,7 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t par) {
 __device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t par) {
     uint32_t ok;
     asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, "
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, "
         "p;\n}\n"
         : "=r"(ok)
         : "r"(smem_u32(bar)), "r"(par), "r"(1000u)
