@@ -241,6 +241,43 @@ __device__ __forceinline__ void store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
+// Sixteen columns' values of one j: rows i .. i + 15 of out, the first `rows` of them.  With registers to
+// spare, four addresses step by four rows: one that steps by a row is a chain of 16 dependent 64-bit additions.
+template <typename T, bool SPARE>
+__device__ __forceinline__ void store16(T* d0, uint64_t ld, const uint32_t* v, float scale, uint32_t rows) {
+    if (!SPARE) {
+        if (rows >= 16) {
+#pragma unroll
+            for (uint32_t e = 0; e < 16; ++e, d0 += ld) store(d0, __uint_as_float(v[e]) * scale);
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 16; ++e, d0 += ld)
+                if (e < rows) store(d0, __uint_as_float(v[e]) * scale);
+        }
+        return;
+    }
+    T *d1 = d0 + ld, *d2 = d1 + ld, *d3 = d2 + ld;
+    const uint64_t ld4 = 4 * ld;
+    if (rows >= 16) {
+#pragma unroll
+        for (uint32_t e = 0; e < 16; e += 4, d0 += ld4, d1 += ld4, d2 += ld4, d3 += ld4) {
+            store(d0, __uint_as_float(v[e]) * scale);
+            store(d1, __uint_as_float(v[e + 1]) * scale);
+            store(d2, __uint_as_float(v[e + 2]) * scale);
+            store(d3, __uint_as_float(v[e + 3]) * scale);
+        }
+    } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 16; e += 4, d0 += ld4, d1 += ld4, d2 += ld4, d3 += ld4) {
+            if (e >= rows) break;
+            store(d0, __uint_as_float(v[e]) * scale);
+            if (e + 1 < rows) store(d1, __uint_as_float(v[e + 1]) * scale);
+            if (e + 2 < rows) store(d2, __uint_as_float(v[e + 2]) * scale);
+            if (e + 3 < rows) store(d3, __uint_as_float(v[e + 3]) * scale);
+        }
+    }
+}
+
 template <typename T, uint32_t BLOCK, uint32_t CTAS>
 __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_constant__ ProdArgs A) {
     extern __shared__ __align__(1024) unsigned char sm[];
@@ -459,6 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
                 ok = __all_sync(kFull, bwait(&tfull[accs.i], accs.par, stop, A.polls));
                 tc_fence_after();
             }
+            uint32_t p = CTAS == 1 && cpp == 1 ? x0 : 0, c = cpp == 1 ? 0 : x0 * 16;  // panel and column of chunk x
             for (uint32_t x = x0; x < chunks || x == x0; x += kBatch * dx) {
                 uint32_t v[kBatch][16];
                 __syncwarp();  // tcgen05.ld is warp-collective
@@ -481,22 +519,19 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
                 }
 #pragma unroll
                 for (uint32_t y = 0; y < kBatch; ++y) {
-                    const uint32_t xy = x + y * dx;
-                    if (xy >= chunks) break;
-                    const uint32_t p = CTAS == 2 ? 0u : xy / cpp, c = (xy - p * cpp) * 16;
-                    const uint64_t j = (uint64_t)(p0 + p) * kFp4Rows + qq * 32 + lane;
-                    T* dst = out + (uint64_t)(q0 + c) * A.ld + j;
+                    if (x + y * dx >= chunks) break;
                     if (!ok)
 #pragma unroll
                         for (uint32_t e = 0; e < 16; ++e) v[y][e] = 0x7FC00000u;
-                    if (j >= A.n) continue;
-                    if (c + 16 <= rows) {
-#pragma unroll
-                        for (uint32_t e = 0; e < 16; ++e, dst += A.ld) store(dst, __uint_as_float(v[y][e]) * A.scale);
-                    } else {
-#pragma unroll
-                        for (uint32_t e = 0; e < 16; ++e, dst += A.ld)
-                            if (c + e < rows) store(dst, __uint_as_float(v[y][e]) * A.scale);
+                    if (CTAS == 2) c = (x + y * dx) * 16;
+                    const uint64_t j = (uint64_t)(p0 + p) * kFp4Rows + qq * 32 + lane;
+                    if (j < A.n && c < rows) store16<T, CTAS == 1>(out + (uint64_t)(q0 + c) * A.ld + j, A.ld, v[y], A.scale, rows - c);
+                    if (CTAS == 1) {  // the next chunk of this warp's, perhaps of the next panel
+                        c += 16 * dx;
+                        if (c >= A.nt) {
+                            c -= A.nt;
+                            ++p;
+                        }
                     }
                 }
             }

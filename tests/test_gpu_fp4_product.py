@@ -57,6 +57,19 @@ def test_row_counts(n, block):
     check_exact(300, n, 100, block)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("offset", [0, 1, 2, 3, 7, 15])
+@pytest.mark.parametrize("m,n", [(2, 1), (17, 127), (40, 128), (16, 130), (130, 255), (40, 20000), (270, 19013)])
+def test_rows_of_any_alignment(m, n, offset, dtype):
+    """Rows of out at every offset within a sector; what lies around them is left as it was."""
+    q, r = exact_rows(m, 64, 32, 1), exact_rows(n, 64, 32, 2)
+    buf = torch.full((m, n + offset + 5), 7.0, dtype=dtype, device="cuda")
+    got = gf.product_fp4(q, gf.quantize_fp4(r), out=buf[:, offset:offset + n])
+    assert torch.equal(got, (q.double() @ r.double().t()).float().to(dtype))
+    got.fill_(7.0)
+    assert (buf == 7.0).all()
+
+
 @pytest.mark.parametrize("block", [16, 32])
 @pytest.mark.parametrize("m,n,dim", [
     (129, 19001, 96), (256, 18944, 128), (257, 12801, 32), (300, 20000, 33), (1000, 4993, 200), (2000, 2500, 1000),
