@@ -144,6 +144,8 @@ def lib() -> C.CDLL:
         "gf_quantize_fp4": (C.c_int, [_P, _U32, C.c_uint64, _U32, _U32, C.c_float, _U32, _P, _P]),
         "gf_dequantize_fp4": (C.c_int, [_P, _U32, _U32, _U32, C.c_float, _P, _U32, C.c_uint64, _P]),
         "gf_product_fp4": (C.c_int, [_P, _U32, _P, _U32, _U32, _U32, C.c_float, _P, _U32, C.c_uint64, _U32, _P]),
+        "gf_product_fp4_raw": (C.c_int, [_P, _U32, C.c_uint64, _U32, C.c_float, _P, _U32, _U32, _U32, C.c_float, _P, _U32,
+                                         C.c_uint64, _P, _U32, _P]),
         "gf_quantize_fp4_host": (C.c_int, [_P, _U32, _U32, C.c_float, _U32, _P]),
         "gf_dequantize_fp4_host": (C.c_int, [_P, _U32, _U32, _U32, C.c_float, _P]),
         "gf_write_attrs": (C.c_int, [C.c_char_p, _P, _U32, _U32]),
@@ -698,23 +700,35 @@ def dequantize_fp4(rows: Fp4Rows, dtype=None, out=None, stream=None):
 
 
 def _fp4_product(s, queries, p, rows, dtype, out, query_alpha, test_wait):
+    import torch
     what = "gf_product_fp4"
     dt = _fp4_dtype(dtype, what)
-    if not isinstance(queries, Fp4Rows):
-        if getattr(queries, "device", None) != p.device:
-            raise GarfieldError(1, what, f"queries: expected Fp4Rows or a CUDA tensor on {p.device}")
-        queries = _fp4_quantize(s, queries, query_alpha, rows.block)
-        qp = queries.packed
-    else:
+    device, dim, block = p.device, rows.dim, rows.block
+    if isinstance(queries, Fp4Rows):
         qp = _fp4_rows(queries, what)
-        if qp.device != p.device:
-            raise GarfieldError(1, what, f"queries on {qp.device}, rows on {p.device}")
-    if queries.dim != rows.dim or queries.block != rows.block:
-        raise GarfieldError(1, what, f"queries of dim {queries.dim}, block {queries.block}; rows of dim {rows.dim}, "
-                                     f"block {rows.block}")
-    out, ld = _fp4_out(out, queries.n, rows.n, dtype, p.device, what)
-    st = lib().gf_product_fp4(qp.data_ptr(), queries.n, p.data_ptr(), rows.n, rows.dim, rows.block,
-                              1.0 / (queries.alpha * rows.alpha), out.data_ptr(), dt, ld, test_wait, s)
+        m, qdim = queries.n, queries.dim
+        if queries.block != block:
+            raise GarfieldError(1, what, f"queries of block {queries.block}, rows of block {block}")
+    else:
+        qp = queries
+        m, qdim, qld = _fp4_matrix(queries, what, "queries")
+        qdt = _fp4_dtype(queries.dtype, what)
+    if qp.device != device or qdim != dim:
+        raise GarfieldError(1, what, f"queries of dim {qdim} on {qp.device}, rows of dim {dim} on {device}")
+    out, ld = _fp4_out(out, m, rows.n, dtype, device, what)
+    if qp is queries:
+        # (what the call quantises in passing needs no room)
+        ws = None
+        if not (m <= 16 and dim <= 8192 and m * dim <= 32768):
+            ws = torch.empty(_fp4_size(m, dim, block), dtype=torch.uint8, device=device)
+        if not query_alpha > 0.0:
+            raise GarfieldError(1, what, f"query_alpha {query_alpha} is not positive")
+        st = lib().gf_product_fp4_raw(qp.data_ptr(), qdt, qld, m, query_alpha, p.data_ptr(), rows.n, dim, block,
+                                      1.0 / (query_alpha * rows.alpha), out.data_ptr(), dt, ld,
+                                      None if ws is None else ws.data_ptr(), test_wait, s)
+    else:
+        st = lib().gf_product_fp4(qp.data_ptr(), m, p.data_ptr(), rows.n, dim, block, 1.0 / (queries.alpha * rows.alpha),
+                                  out.data_ptr(), dt, ld, test_wait, s)
     if st:
         _check(st, what)
     return out
@@ -725,9 +739,11 @@ def product_fp4(queries, rows: Fp4Rows, dtype=None, out=None, query_alpha: float
     """gf_product_fp4: the inner products of every query with every row (m x n, float32 unless dtype or
     out say otherwise).  queries: Fp4Rows of the same dim and block, or a float32, float16 or
     bfloat16 CUDA matrix, which is held in 4 bits (quantize_fp4 with query_alpha and the rows'
-    block) for the call."""
+    block) for the call (gf_product_fp4_raw)."""
     import torch
     p = _fp4_rows(rows, "gf_product_fp4")
+    if not isinstance(queries, Fp4Rows) and not getattr(queries, "is_cuda", False):
+        raise GarfieldError(1, "gf_product_fp4", "queries: expected Fp4Rows or a 2-D CUDA tensor")
     dtype = dtype or (out.dtype if out is not None else torch.float32)
     return _fp4_run(p.device, stream, _fp4_product, queries, p, rows, dtype, out, query_alpha, test_wait)
 

@@ -51,6 +51,7 @@ __host__ __device__ inline uint32_t fp4_scale_at(uint32_t r, uint32_t b) {
 }
 
 inline bool fp4_shape(uint32_t dim, uint32_t block) { return dim > 0 && (block == 16 || block == 32); }
+inline bool fp4_alpha(float alpha) { return alpha >= 0x1p-126f && alpha <= 0x1p126f; }  // 1 / alpha is normal too
 inline uint32_t dtype_bytes(uint32_t dtype) { return dtype == GF_F32 ? 4u : dtype == GF_F16 || dtype == GF_BF16 ? 2u : 0u; }
 inline bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 

@@ -1,0 +1,108 @@
+// Device code of the 4-bit block floating-point format (gf_fp4.h): codes and scales from elements and back.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
+#include "gf_device.cuh"
+#include "gf_fp4.h"
+
+namespace gf {
+namespace fp4 {
+
+constexpr uint32_t kOct = 8;  // elements that one thread quantises
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void from_f32(float v, float& o) { o = v; }
+__device__ __forceinline__ void from_f32(float v, __half& o) { o = __float2half_rn(v); }
+__device__ __forceinline__ void from_f32(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
+
+// W bytes of elements.
+template <typename T, uint32_t W>
+struct alignas(W < 16 ? W : 16) Vec {
+    T v[W / sizeof(T)];
+};
+
+// Eight codes from eight floats, element i in bits 4i .. 4i + 3 (nearest, ties to even, saturating).
+__device__ __forceinline__ uint32_t e2m1x8(const float* x) {
+    uint32_t r;
+    asm("{\n .reg .b8 a, b, c, d;\n cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n mov.b32 %0, {a, b, c, d};\n}\n"
+        : "=r"(r)
+        : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]));
+    return r;
+}
+// Two floats from a byte of two codes.
+__device__ __forceinline__ float2 e2m1x2_to_f32(uint32_t b) {
+    uint32_t h;
+    asm("{\n .reg .b8 b;\n cvt.u8.u32 b, %1;\n cvt.rn.f16x2.e2m1x2 %0, b;\n}\n" : "=r"(h) : "r"(b));
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+__device__ __forceinline__ float e4m3_to_f32(uint32_t b) {
+    return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3)));
+}
+__device__ __forceinline__ float scale_to_f32(uint32_t b, bool block16) {
+    if (block16) return e4m3_to_f32(b);
+    // E8M0: 2^(b - 127); 0 stands for 2^-127 (half the smallest normal float), 255 for NaN
+    return __uint_as_float(b == 255u ? 0x7FC00000u : (b == 0u ? 0x00400000u : b << 23));
+}
+
+// max(|a|, |b|), NaN if either is.
+__device__ __forceinline__ float amax2(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return r;
+}
+// Largest magnitude of eight elements, NaN if one is; 16-bit elements are compared in pairs.
+__device__ __forceinline__ float amax8(const float* v) {
+    return amax2(amax2(amax2(v[0], v[1]), amax2(v[2], v[3])), amax2(amax2(v[4], v[5]), amax2(v[6], v[7])));
+}
+__device__ __forceinline__ float amax8(const __half* v) {
+    const __half2* h = reinterpret_cast<const __half2*>(v);
+    const __half2 a = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+    return amax2(__low2float(a), __high2float(a));
+}
+__device__ __forceinline__ float amax8(const __nv_bfloat16* v) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(v);
+    const __nv_bfloat162 a = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+    return amax2(__low2float(a), __high2float(a));
+}
+// x / y correctly rounded, for r = 1 / y correctly rounded and results that are normal: one exact
+// remainder corrects the product (Markstein, IBM J. Res. Dev. 34, 1990).  Results too small for that are far
+// below the first code boundary.  (In this order of signs -0 / y stays -0.)
+__device__ __forceinline__ float div_by(float x, float y, float r) {
+    const float q = __fmul_rn(x, r);
+    return __fmaf_rn(-__fmaf_rn(q, y, -x), r, q);
+}
+
+// Scale byte of a block from its largest magnitude, and the codes of this thread's eight elements.
+template <uint32_t BLOCK>
+__device__ __forceinline__ uint32_t encode8(float* x, float amax, uint32_t& codes) {
+    const uint32_t ef = __float_as_uint(amax) >> 23;
+    uint32_t s8;
+    if (BLOCK == 32) {
+        s8 = ef == 255u ? 255u : max(ef, 2u) - 2u;
+        const float inv = __uint_as_float((254u - min(s8, 253u)) << 23);  // 1 / s, a power of two
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(x[e], inv);
+    } else {
+        s8 = ef == 255u ? 0x7Fu
+                        : (uint32_t)__nv_cvt_float_to_fp8(div_by(amax, 6.0f, 1.0f / 6.0f), __NV_SATFINITE, __NV_E4M3);
+        const float s = e4m3_to_f32(s8), r = __frcp_rn(s);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {  // div_by, two at a time
+            const dev::f2x v = dev::pack2(x[e], x[e + 1]), r2 = dev::pack2(r, r), q = dev::mul2(v, r2);
+            const dev::f2x nr = dev::fma2(q, dev::pack2(s, s), dev::pack2(-x[e], -x[e + 1]));
+            const dev::f2x y = dev::fma2(nr, dev::pack2(-r, -r), q);
+            x[e] = dev::lo2(y);
+            x[e + 1] = dev::hi2(y);
+        }
+    }
+    codes = ef == 255u || (BLOCK == 16 && s8 == 0u) ? 0u : e2m1x8(x);
+    return s8;
+}
+
+}  // namespace fp4
+}  // namespace gf

@@ -7,10 +7,16 @@
 // an accumulator's lanes are consecutive j: a warp's store of one column is a contiguous
 // run of out, whatever the number of queries, and few queries cost few columns.
 //
-// One kernel in two widths.  CTAS = 1: a CTA walks tiles of pb row panels by one query panel (up to
-// 128 queries).  CTAS = 2: a cluster of two CTAs walks tiles of two row panels by two query panels,
-// each CTA holding one of either and the tcgen05.mma of the pair (M = N = 256) reading both, so
-// that a byte copied into shared memory feeds twice the products.  Query tiles vary fastest: a
+// One kernel in three modes.
+//   kRing: a CTA walks tiles of pb row panels by one query panel (up to 128 queries).
+//   kFew:  the same for a single query panel small enough to stay in shared memory; up to 16 queries
+//          may come as they are and are quantised there, which saves a launch.
+//   kPair: a cluster of two CTAs walks tiles of two row panels by two query panels, each CTA holding
+//          one of either and the tcgen05.mma of the pair (M = N = 256) reading both, so that a byte
+//          copied into shared memory feeds twice the products.
+// Tiles too few to occupy the SMs are split along the elements over clusters of up to 8 CTAs (kRing,
+// kFew): each sums its share, the others send theirs to the first through distributed shared
+// memory and it adds them in order.  Query tiles vary slowest within a band of row panels: a
 // panel's bytes leave HBM once.
 //
 // Warp 0 copies scales and codes, one run each, into a ring of stages of up to four groups (of a
@@ -21,18 +27,16 @@
 // MMAs take 128 cycles at N = 128 and its panel's bytes 200 at the HBM rate.
 //
 // Every wait is bounded.  When one runs out the CTA stops and the outputs it still owes become NaN.
-#include <cuda_bf16.h>
-
 #include <algorithm>
 #include <cmath>
 
-#include "gf_device.cuh"
-#include "gf_fp4.h"
+#include "gf_fp4_dev.cuh"
 
 namespace gf {
 namespace {
 
 using namespace dev;
+using namespace fp4;
 
 constexpr uint32_t kThreads = 320;    // producer warp, MMA warp, 8 epilogue warps
 constexpr uint32_t kMaxStages = 8;
@@ -45,6 +49,11 @@ constexpr uint32_t kSmemLimit = 227 * 1024;
 // Zeros for the second column of an MMA step that the rows' last group lacks: with zero codes on the
 // query side, whatever codes stand in the other side's place add nothing.
 __device__ __align__(16) uint8_t g_zero[kFp4ColBytes];
+
+enum Mode : uint32_t { kRing = 0, kFew = 1, kPair = 2 };
+constexpr uint32_t ctas_of(uint32_t mode) { return mode == kPair ? 2 : 1; }
+constexpr uint32_t kResident = 128 * 1024;  // bytes of queries kept in shared memory, at most
+constexpr uint32_t kMaxSplit = 8;           // CTAs of a cluster that share a tile
 
 // Groups of a full stage: four, or three where two query panels' scales of 16-element blocks would leave
 // TMEM no room for a third stage beside an accumulator of 256 columns.
@@ -60,10 +69,16 @@ struct ProdArgs {
     uint32_t acc, stages, stage_bytes;
     uint32_t b_off, bc_off;             // within a stage: the query panels' scales, and the query panel's codes
     uint32_t sf_cols;                   // TMEM columns of one stage's scales
+    uint32_t split, per;                // CTAs that share a tile, and groups of each
+    uint32_t res_off, resc_off;         // kFew: scales and codes of the queries' share
+    const void* raw;                    // kFew: queries as they are (else q), quantised with q_alpha
+    uint64_t raw_ld;
+    uint32_t raw_dtype;
+    float q_alpha;
     void* out;
     uint64_t ld;
     float scale;
-    uint32_t polls, extra_tx;
+    uint32_t dim, bar_off, polls, extra_tx;
 };
 
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -134,6 +149,11 @@ __device__ __forceinline__ void arrive_at_leader(uint64_t* bar) {
             smem_u32(bar))
         : "memory");
 }
+// Every thread of the cluster has arrived; its earlier writes, to other CTAs' shared memory too, are seen.
+__device__ __forceinline__ void sync_cluster() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory");
+}
 // Every thread of the CTA, or of the pair, has arrived.
 template <uint32_t CTAS>
 __device__ __forceinline__ void sync_all() {
@@ -141,8 +161,14 @@ __device__ __forceinline__ void sync_all() {
     if (CTAS == 1)
         __syncthreads();
     else
-        asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory");
+        sync_cluster();
     tc_fence_after();
+}
+// v at the same shared-memory place of the cluster's CTA 0.
+__device__ __forceinline__ void store_at_leader(const void* p, float v) {
+    asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, 0;\n st.shared::cluster.f32 [a], %1;\n}\n" ::"r"(smem_u32(p)),
+                 "f"(v)
+                 : "memory");
 }
 // 16 consecutive TMEM columns of this warp's 32 lanes, and the wait that orders their use.
 __device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* v) {
@@ -278,24 +304,73 @@ __device__ __forceinline__ void store16(T* d0, uint64_t ld, const uint32_t* v, f
     }
 }
 
-template <typename T, uint32_t BLOCK, uint32_t CTAS>
+// Eight elements of a row from index k on, as floats; `left` of them exist.
+template <typename T>
+__device__ __forceinline__ void load8(const void* base, uint64_t at, uint32_t left, float* x) {
+    const T* p = static_cast<const T*>(base) + at;
+#pragma unroll
+    for (uint32_t e = 0; e < kOct; ++e) x[e] = e < left ? to_f32(p[e]) : 0.0f;
+}
+
+// This CTA's share of the queries (groups gb .. ge - 1), quantised into shared memory in the packed
+// panel's form by the epilogue's 256 threads (t: this one's number).
+template <uint32_t BLOCK>
+__device__ __forceinline__ void quantize_queries(const ProdArgs& A, uint32_t gb, uint32_t ge, uint32_t dim, unsigned char* scales,
+                                                 unsigned char* codes, uint32_t t) {
+    const uint32_t octs = (ge - gb) * (kFp4Group / kOct), total = A.m * octs;
+    const uint32_t cols = min(4 * ge, (A.Lq.cols + 1) & ~1u) - 4 * gb;  // with the zeros that complete an MMA step
+    for (uint32_t i0 = t & ~31u; i0 < total; i0 += 256) {
+        const uint32_t i = i0 + (t & 31u);  // (a row's octs are a multiple of 16: a block's threads share a row)
+        const bool in = i < total;
+        const uint32_t row = in ? i / octs : 0, o = in ? i - row * octs : 0;
+        const uint32_t k = gb * kFp4Group + o * kOct, left = in && k < dim ? dim - k : 0u;
+        float x[kOct];
+        const uint64_t at = row * A.raw_ld + k;
+        if (A.raw_dtype == GF_F32)
+            load8<float>(A.raw, at, left, x);
+        else if (A.raw_dtype == GF_F16)
+            load8<__half>(A.raw, at, left, x);
+        else
+            load8<__nv_bfloat16>(A.raw, at, left, x);
+#pragma unroll
+        for (uint32_t e = 0; e < kOct; ++e) x[e] = __fmul_rn(x[e], A.q_alpha);
+        float mx = amax8(x);
+        if (BLOCK == 32) mx = amax2(mx, __shfl_xor_sync(kFull, mx, 2));
+        mx = amax2(mx, __shfl_xor_sync(kFull, mx, 1));
+        uint32_t c;
+        const uint32_t s8 = encode8<BLOCK>(x, mx, c);
+        if (!in) continue;
+        if (o / 4 < cols) *reinterpret_cast<uint32_t*>(codes + (o / 4) * A.Lq.col_bytes + row * 16 + (o & 3u) * 4) = c;
+        if (o % (BLOCK / kOct) == 0)
+            scales[(o / 16) * A.Lq.scale_bytes + fp4_scale_at(row, (o % 16) / (BLOCK / kOct))] = (uint8_t)s8;
+    }
+    fence_proxy_async_smem();  // the MMAs read these through the asynchronous proxy
+    __syncwarp();
+}
+
+template <typename T, uint32_t BLOCK, uint32_t MODE>
 __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_constant__ ProdArgs A) {
     extern __shared__ __align__(1024) unsigned char sm[];
+    constexpr uint32_t CTAS = ctas_of(MODE);
     constexpr uint32_t kSub = BLOCK == 16 ? 2 : 1;  // scale sub-blocks of a group
     constexpr uint32_t kGs = stage_groups(BLOCK, CTAS);
-    uint64_t* full = reinterpret_cast<uint64_t*>(sm + A.stages * A.stage_bytes);
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm + A.bar_off);
     uint64_t* pfull = full + kMaxStages;  // CTA 0 of a pair: the other CTA's stage is full
     uint64_t* empty = pfull + kMaxStages;
     uint64_t* tfull = empty + kMaxStages;
     uint64_t* tempty = tfull + kMaxAcc;
     uint64_t* drain = tempty + kMaxAcc;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    uint64_t* qfull = drain + 1;  // kFew: the queries are in place
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(qfull + 1);
     volatile uint32_t* stop = tmem_slot + 1;
     const uint32_t warp = threadIdx.x >> 5, lane = lane_id();
     const uint32_t rank = CTAS == 2 ? (blockIdx.x & 1u) : 0u;  // in the pair (clusters are consecutive blocks)
-    const uint32_t worker = blockIdx.x / CTAS, workers = gridDim.x / CTAS;
+    const uint32_t share = CTAS == 2 ? 0u : blockIdx.x % A.split;  // of the elements
+    const uint32_t worker = CTAS == 2 ? blockIdx.x / 2 : blockIdx.x / A.split;
+    const uint32_t workers = CTAS == 2 ? gridDim.x / 2 : gridDim.x / A.split;
+    const uint32_t G = A.Lr.groups, gb = share * A.per, ge = min(G, gb + A.per);
     const uint32_t cpp = A.nt / 16;     // 16-column chunks of a panel's accumulator
-    const bool split = A.pb * cpp > 1;  // both epilogue halves share a tile's chunks, else they take alternate tiles
+    const bool halves = A.pb * cpp > 1;  // both epilogue halves share a tile's chunks, else they take alternate tiles
 
     if (warp == 0) tmem_alloc<CTAS>(tmem_slot);
     if (threadIdx.x == 0) {
@@ -306,37 +381,47 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         }
         for (uint32_t i = 0; i < kMaxAcc; ++i) {
             mbar_init(&tfull[i], 1);
-            mbar_init(&tempty[i], (split ? 8 : 4) * CTAS);
+            mbar_init(&tempty[i], (halves ? 8 : 4) * CTAS);
         }
         mbar_init(drain, 1);
+        mbar_init(qfull, A.raw ? 8 : 1);
         *stop = 0;
         fence_mbar_init();
     }
     sync_all<CTAS>();
     const uint32_t tmem = *tmem_slot;
-    const uint32_t G = A.Lr.groups;
 
+    bool done = true;  // epilogue warps of a split tile: the sums are in TMEM
     if (warp == 0) {
         // -------------------------------------------------------------- producer warp
         bool ok = true;
         Ring ring;
         uint64_t filled = 0;
         const uint32_t pad = A.Lq.cols & 1u;  // the last group lacks the second column of an MMA step
+        if (MODE == kFew && !A.raw && elect_one()) {
+            const uint32_t as = (ge - gb) * A.Lq.scale_bytes, bc = min(4 * (ge - gb), A.Lq.cols - 4 * gb) * A.Lq.col_bytes;
+            const uint32_t z = ge == G && pad ? A.Lq.col_bytes : 0u;
+            mbar_arrive_expect_tx(qfull, as + bc + z);
+            bulk_g2s(sm + A.res_off, A.q + A.Lq.scales_at(0, gb), as, qfull);
+            bulk_g2s(sm + A.resc_off, A.q + A.Lq.col_at(0, 4 * gb), bc, qfull);
+            if (z) bulk_g2s(sm + A.resc_off + bc, g_zero, z, qfull);
+        }
+        __syncwarp();
         for (Tiles t(worker, workers, A.band, A.batches, A.qtiles); ok && t.more(); t.next()) {
             const uint32_t p0 = t.batch() * A.pb * CTAS + rank, np = p0 < A.panels ? min(A.pb, A.panels - p0) : 0u;
             const uint32_t qp = t.q * CTAS + rank;
-            for (uint32_t g = 0; g < G; g += A.gs, ring.next(A.stages), ++filled) {
+            for (uint32_t g = gb; g < ge; g += A.gs, ring.next(A.stages), ++filled) {
                 // (a barrier's first wait, for the use before its first, returns at once)
                 if (!(ok = __all_sync(kFull, bwait(&empty[ring.i], ring.par ^ 1u, stop, A.polls)))) break;
                 unsigned char* stg = sm + ring.i * A.stage_bytes;
                 uint64_t* bar = &full[ring.i];
-                const uint32_t ng = min(A.gs, G - g), nc = min(4 * ng, A.Lr.cols - 4 * g);  // groups and columns
+                const uint32_t ng = min(A.gs, ge - g), nc = min(4 * ng, A.Lr.cols - 4 * g);  // groups and columns
                 const uint32_t as = ng * A.Lr.scale_bytes, ac = nc * A.Lr.col_bytes, bc = nc * A.Lq.col_bytes;
                 const uint32_t z = g + ng == G && pad ? A.Lq.col_bytes : 0u;
                 const uint32_t a_bytes = A.pb > 1 ? np * (uint32_t)A.Lr.panel_bytes : np * (as + ac);
                 // query panels of the tile that exist: their scales all come, the codes of this CTA's
-                const uint32_t nq = min(CTAS, A.qpanels - t.q * CTAS);
-                const uint32_t b_bytes = nq * as + (qp < A.qpanels ? bc + z : 0u);
+                const uint32_t nq = MODE == kFew ? 0u : min(CTAS, A.qpanels - t.q * CTAS);
+                const uint32_t b_bytes = MODE == kFew ? 0u : nq * as + (qp < A.qpanels ? bc + z : 0u);
                 if (elect_one()) {
                     mbar_arrive_expect_tx(bar, a_bytes + b_bytes + A.extra_tx);
                     if (A.pb > 1) {  // whole panels
@@ -345,12 +430,14 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
                         bulk_g2s(stg, A.r + A.Lr.scales_at(p0, g), as, bar);
                         bulk_g2s(stg + A.gs * A.Lr.scale_bytes, A.r + A.Lr.col_at(p0, 4 * g), ac, bar);
                     }
-                    bulk_g2s(stg + A.b_off, A.q + A.Lq.scales_at(t.q * CTAS, g), as, bar);
-                    if (CTAS == 2 && nq == 2)
-                        bulk_g2s(stg + A.b_off + A.gs * A.Lq.scale_bytes, A.q + A.Lq.scales_at(t.q * CTAS + 1, g), as, bar);
-                    if (qp < A.qpanels) {
-                        bulk_g2s(stg + A.bc_off, A.q + A.Lq.col_at(qp, 4 * g), bc, bar);
-                        if (z) bulk_g2s(stg + A.bc_off + bc, g_zero, z, bar);
+                    if (MODE != kFew) {
+                        bulk_g2s(stg + A.b_off, A.q + A.Lq.scales_at(t.q * CTAS, g), as, bar);
+                        if (CTAS == 2 && nq == 2)
+                            bulk_g2s(stg + A.b_off + A.gs * A.Lq.scale_bytes, A.q + A.Lq.scales_at(t.q * CTAS + 1, g), as, bar);
+                        if (qp < A.qpanels) {
+                            bulk_g2s(stg + A.bc_off, A.q + A.Lq.col_at(qp, 4 * g), bc, bar);
+                            if (z) bulk_g2s(stg + A.bc_off + bc, g_zero, z, bar);
+                        }
                     }
                 }
                 __syncwarp();
@@ -358,13 +445,17 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         }
         if (!ok) *stop = 1u;
         // every copy issued lands before the CTA exits (in normal operation they completed long ago)
-        if (lane == 0)
+        if (lane == 0) {
             for (uint32_t st = 0; st < A.stages && st < filled; ++st) {
                 const uint32_t use = (uint32_t)((filled - 1 - st) / A.stages);  // the slot's last
                 uint32_t p = 0;
                 while (!mbar_try(&full[st], use & 1u) && ++p < A.polls) {
                 }
             }
+            uint32_t p = 0;
+            while (MODE == kFew && !A.raw && !mbar_try(qfull, 0) && ++p < A.polls) {
+            }
+        }
         __syncwarp();
     } else if (warp == 1 && rank != 0) {
         // ------------------------- the other CTA of a pair: tells CTA 0 which of its stages are full
@@ -388,31 +479,36 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         const uint32_t idesc = (1u << 7) | (1u << 10) | ((A.nt >> 3) << 17) | ((BLOCK == 32 ? 1u : 0u) << 23) |
                                ((CTAS * 128u >> 4) << 24);
         const uint32_t acc_cols = A.pb * A.nt, sf0 = tmem + A.acc * acc_cols;
-        // everything below in 16-byte units of shared memory, added to a descriptor's address field
+        // everything below in 16-byte units of shared memory, added to a descriptor's 14-bit address field (in a
+        // cluster, a shared-memory address has the CTA's rank in its upper bits)
         constexpr uint32_t kScales = kSub * kFp4ScaleSub / 16;  // a group's scales
         const uint32_t a_item = (uint32_t)A.Lr.panel_bytes / 16;
         const uint32_t a_step = A.Lr.col_bytes / 8, b_step = A.Lq.col_bytes / 8;  // two columns
-        const uint32_t sm0 = smem_u32(sm) / 16, st16 = A.stage_bytes / 16, b_off = A.b_off / 16;
+        const uint32_t sm0 = (smem_u32(sm) >> 4) & 0x3FFFu, st16 = A.stage_bytes / 16;
         const uint64_t ad0 = smem_desc(0, A.Lr.col_bytes, 128) + A.gs * kScales;
-        const uint64_t bd0 = smem_desc(0, A.Lq.col_bytes, 128) + A.bc_off / 16;
+        const uint64_t bd0 = smem_desc(0, A.Lq.col_bytes, 128);
         const uint64_t cd0 = smem_desc(0, 128, 128);
         const uint32_t sfb_off = A.pb * A.gs * 4 * kSub, q2 = A.gs * kScales;
-        bool ok = true;
+        bool ok = MODE != kFew || __all_sync(kFull, bwait(qfull, 0, stop, A.polls));
         Ring ring, accs;
-        for (Tiles t(worker, workers, A.band, A.batches, A.qtiles); t.more(); t.next(), accs.next(A.acc)) {
+        for (Tiles t(worker, workers, A.band, A.batches, A.qtiles); ok && t.more(); t.next(), accs.next(A.acc)) {
             const uint32_t np = CTAS == 2 ? 1u : min(A.pb, A.panels - t.batch() * A.pb);
             const uint32_t d0 = tmem + accs.i * acc_cols;
             if (!(ok = __all_sync(kFull, bwait(&tempty[accs.i], accs.par ^ 1u, stop, A.polls)))) break;
             tc_fence_after();
-            for (uint32_t g = 0; g < G; g += A.gs, ring.next(A.stages)) {
+            for (uint32_t g = gb; g < ge; g += A.gs, ring.next(A.stages)) {
                 ok = bwait(&full[ring.i], ring.par, stop, A.polls);
                 if (CTAS == 2) ok = ok && bwait(&pfull[ring.i], ring.par, stop, A.polls);
                 if (!(ok = __all_sync(kFull, ok))) break;
                 tc_fence_after();
                 const uint32_t st = sm0 + ring.i * st16;
+                // the queries' scales and codes of the stage's first group
+                const uint32_t bs = MODE == kFew ? sm0 + A.res_off / 16 + (g - gb) * kScales : st + A.b_off / 16;
+                const uint32_t bc = MODE == kFew ? sm0 + A.resc_off / 16 + (g - gb) * 2 * b_step : st + A.bc_off / 16;
                 // this stage's scales; their slot was last read by MMAs that the stage's empty barrier covers
                 const uint32_t sfa = sf0 + ring.i * A.sf_cols, sfb = sfa + sfb_off;
-                const uint32_t ng = min(A.gs, G - g), steps = min(2 * ng, (A.Lr.cols - 4 * g + 1) / 2);
+                const uint32_t ng = min(A.gs, ge - g), steps = min(2 * ng, (A.Lr.cols - 4 * g + 1) / 2);
+                const uint32_t acc0 = g - gb;
                 // scales of panel x's group y, and of the query panels' group y
                 auto row_scales = [&](uint32_t x, uint32_t y) {
 #pragma unroll
@@ -424,13 +520,13 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
                     for (uint32_t h = 0; h < kSub; ++h)
 #pragma unroll
                         for (uint32_t j = 0; j < CTAS; ++j)
-                            scales_to_tmem<CTAS>(sfb + ((y * kSub + h) * CTAS + j) * 4, cd0 + (st + b_off + j * q2 + (y * kSub + h) * 32));
+                            scales_to_tmem<CTAS>(sfb + ((y * kSub + h) * CTAS + j) * 4, cd0 + (bs + j * q2 + (y * kSub + h) * 32));
                 };
                 // MMA step s of 64 elements of panel x (two steps to a group)
                 auto step = [&](uint32_t x, uint32_t s, uint32_t acc) {
                     // block 16: a step has its own sub-block; block 32: bytes 2s, 2s + 1 of the group's
                     const uint32_t sub = BLOCK == 16 ? s : s / 2, byte = BLOCK == 16 ? 0u : 2 * (s & 1u);
-                    mma_fp4<BLOCK, CTAS>(d0 + x * A.nt, ad0 + (st + x * a_item + s * a_step), bd0 + (st + s * b_step),
+                    mma_fp4<BLOCK, CTAS>(d0 + x * A.nt, ad0 + (st + x * a_item + s * a_step), bd0 + (bc + s * b_step),
                                          idesc | byte << 4 | byte << 29, sfa + (x * A.gs * kSub + sub) * 4,
                                          sfb + sub * CTAS * 4, acc);
                 };
@@ -442,10 +538,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
                             row_scales(0, y);
                             query_scales(y);
                         }
-                        step(0, 0, g);
+                        step(0, 0, acc0);
 #pragma unroll
                         for (uint32_t s = 1; s < 2 * kGs; ++s) step(0, s, 1);
-                    } else if (np == 4 && steps == 2) {
+                    } else if (CTAS == 1 && np == 4 && steps == 2) {
                         query_scales(0);
 #pragma unroll
                         for (uint32_t x = 0; x < 4; ++x) row_scales(x, 0);
@@ -458,11 +554,11 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
                         for (uint32_t y = 0; y < ng; ++y) query_scales(y);
                         for (uint32_t x = 0; x < np; ++x) {
                             for (uint32_t y = 0; y < ng; ++y) row_scales(x, y);
-                            for (uint32_t s = 0; s < steps; ++s) step(x, s, g | s);
+                            for (uint32_t s = 0; s < steps; ++s) step(x, s, acc0 | s);
                         }
                     }
                     mma_commit<CTAS>(&empty[ring.i]);  // the stage is free once these MMAs have read it
-                    if (g + ng == G) mma_commit<CTAS>(&tfull[accs.i]);
+                    if (g + ng == ge) mma_commit<CTAS>(&tfull[accs.i]);
                 }
                 __syncwarp();
             }
@@ -482,15 +578,24 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         const uint32_t qq = warp & 3u, h = (warp - 2) >> 2;  // lane quarter, half
         const uint32_t acc_cols = A.pb * A.nt;
         T* out = static_cast<T*>(A.out);
+        if (MODE == kFew && A.raw) {
+            quantize_queries<BLOCK>(A, gb, ge, A.dim, sm + A.res_off, sm + A.resc_off, threadIdx.x - 64);
+            if (lane == 0) mbar_arrive(qfull);
+        }
         bool ok = true;
         uint32_t u = 0;
         Ring accs;
         for (Tiles t(worker, workers, A.band, A.batches, A.qtiles); t.more(); t.next(), ++u, accs.next(A.acc)) {
-            if (!split && (u & 1u) != h) continue;
+            if (CTAS == 1 && A.split > 1) {  // the cluster's one tile, stored below
+                done = __all_sync(kFull, bwait(&tfull[0], 0, stop, A.polls));
+                ok = done;
+                break;
+            }
+            if (!halves && (u & 1u) != h) continue;
             const uint32_t p0 = t.batch() * A.pb * CTAS + rank, q0 = t.q * A.nt;
             const uint32_t np = CTAS == 2 ? 1u : min(A.pb, A.panels - p0);
             const uint32_t rows = min(A.nt, A.m - q0);
-            const uint32_t chunks = np * cpp, x0 = split ? h : 0, dx = split ? 2 : 1;
+            const uint32_t chunks = np * cpp, x0 = halves ? h : 0, dx = halves ? 2 : 1;
             const uint32_t addr = tmem + (qq * 32 << 16) + accs.i * acc_cols;
             if (ok) {
                 ok = __all_sync(kFull, bwait(&tfull[accs.i], accs.par, stop, A.polls));
@@ -538,13 +643,53 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         }
         if (!ok) *stop = 1u;
     }
+    if (CTAS == 1 && A.split > 1) {
+        // ------------------------------------------- the shares of a tile, added in CTA 0 of the cluster
+        // All of the cluster's MMAs are done, so CTA 0's stages are free: share i > 0 writes its sums there as
+        // [i - 1][column][row] floats.
+        const uint32_t qq = warp & 3u, row = qq * 32 + lane;
+        const uint32_t addr = tmem + (qq * 32 << 16);
+        Tiles t(worker, workers, A.band, A.batches, A.qtiles);
+        const uint32_t q0 = t.q * A.nt, rows = min(A.nt, A.m - q0);
+        float* sums = reinterpret_cast<float*>(sm);
+        tc_fence_before();
+        sync_cluster();
+        tc_fence_after();
+        for (uint32_t pass = 0; pass < 2; ++pass) {
+            if (warp >= 2 && (pass == 0) == (share != 0))
+                for (uint32_t c = ((warp - 2) >> 2) * 16; c < rows; c += 32) {
+                    uint32_t v[16];
+                    __syncwarp();
+                    tmem_ld16(addr + c, v);
+                    tmem_wait_ld16(v);
+                    if (!done)
+#pragma unroll
+                        for (uint32_t e = 0; e < 16; ++e) v[e] = 0x7FC00000u;
+                    if (pass == 0) {
+                        float* dst = sums + ((share - 1) * A.nt + c) * kFp4Rows + row;
+#pragma unroll
+                        for (uint32_t e = 0; e < 16; ++e) store_at_leader(dst + e * kFp4Rows, __uint_as_float(v[e]));
+                    } else {
+                        for (uint32_t i = 1; i < A.split; ++i) {
+                            const float* src = sums + ((i - 1) * A.nt + c) * kFp4Rows + row;
+#pragma unroll
+                            for (uint32_t e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) + src[e * kFp4Rows]);
+                        }
+                        const uint64_t j = (uint64_t)t.batch() * kFp4Rows + row;
+                        if (j < A.n)
+                            store16<T, true>(static_cast<T*>(A.out) + (uint64_t)(q0 + c) * A.ld + j, A.ld, v, A.scale, rows - c);
+                    }
+                }
+            if (pass == 0) sync_cluster();
+        }
+    }
     sync_all<CTAS>();
     if (warp == 0) tmem_free<CTAS>(tmem);
 }
 
-template <typename T, uint32_t BLOCK, uint32_t CTAS>
+template <typename T, uint32_t BLOCK, uint32_t MODE>
 gf_status launch_product(const ProdArgs& A, uint32_t grid, uint32_t smem, cudaStream_t s) {
-    GF_CUDA(cudaFuncSetAttribute(fp4_product_kernel<T, BLOCK, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    GF_CUDA(cudaFuncSetAttribute(fp4_product_kernel<T, BLOCK, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kThreads);
@@ -552,25 +697,29 @@ gf_status launch_product(const ProdArgs& A, uint32_t grid, uint32_t smem, cudaSt
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim = {CTAS, 1, 1};
+    at[0].val.clusterDim = {MODE == kPair ? 2 : A.split, 1, 1};
     cfg.attrs = at;
-    cfg.numAttrs = CTAS > 1 ? 1 : 0;
-    GF_CUDA(cudaLaunchKernelEx(&cfg, fp4_product_kernel<T, BLOCK, CTAS>, A));
+    cfg.numAttrs = at[0].val.clusterDim.x > 1 ? 1 : 0;
+    GF_CUDA(cudaLaunchKernelEx(&cfg, fp4_product_kernel<T, BLOCK, MODE>, A));
     return GF_OK;
 }
 
-gf_status product(const void* q, uint32_t m, const void* r, uint32_t n, uint32_t dim, uint32_t block, float scale, void* out,
-                  uint32_t dtype, uint64_t ld, uint32_t test_wait, cudaStream_t s) {
+// Queries that a product quantises itself (their number and size let every CTA do it in passing).
+bool quantised_in_passing(uint32_t m, uint32_t dim) { return m <= 16 && dim <= 8192 && (uint64_t)m * dim <= 32768; }
+
+// q: packed queries, or NULL with raw ones in A (quantised_in_passing).
+gf_status product(ProdArgs A, const void* q, uint32_t m, const void* r, uint32_t n, uint32_t dim, uint32_t block, float scale,
+                  void* out, uint32_t dtype, uint64_t ld, uint32_t test_wait, cudaStream_t s) {
     int dev = 0, sms = 0;
     GF_CUDA(cudaGetDevice(&dev));
     GF_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    ProdArgs A = {};
     A.r = static_cast<const uint8_t*>(r);
     A.q = static_cast<const uint8_t*>(q);
     A.Lr = fp4_layout(n, dim, block);
     A.Lq = fp4_layout(m, dim, block);
     A.m = m;
     A.n = n;
+    A.dim = dim;
     A.panels = fp4_panels(n);
     A.qpanels = fp4_panels(m);
     A.out = out;
@@ -578,37 +727,74 @@ gf_status product(const void* q, uint32_t m, const void* r, uint32_t n, uint32_t
     A.scale = scale;
     A.polls = test_wait ? test_wait : kPolls;
     A.extra_tx = test_wait ? 16u : 0u;
-    const uint32_t sub = block == 16 ? 2 : 1, group = sub * kFp4ScaleSub + 4 * kFp4ColBytes;
-    // pairs of CTAs once their tiles, of 256 x 256, occupy every SM
+    const uint32_t sub = block == 16 ? 2 : 1, scales = sub * kFp4ScaleSub, group = scales + 4 * kFp4ColBytes, G = A.Lr.groups;
+    // pairs of CTAs once their tiles, of 256 x 256, occupy every SM and the rows are long enough for
+    // their arithmetic to show (8192 x 16384 in bf16: 103 us either way at 1024 elements, 107 against 92 at 128)
     const uint64_t pair_tiles = ((uint64_t)A.panels + 1) / 2 * ((A.qpanels + 1) / 2);
-    const uint32_t ctas = A.qpanels >= 2 && pair_tiles >= (uint64_t)sms / 2 ? 2 : 1;
-    const uint32_t qcol = A.Lq.col_bytes / 16;
-    A.nt = ctas == 2 ? 256 : qcol;
-    // a stage: up to four groups of a panel, or all groups of several panels while two accumulators fit and
-    // every SM still has a tile
-    A.gs = std::min(A.Lr.groups, stage_groups(block, ctas));
+    uint32_t mode = G >= 8 && A.qpanels >= 2 && pair_tiles >= (uint64_t)sms / 2 ? kPair : kRing;
+    const uint32_t ctas = ctas_of(mode);
+    A.nt = mode == kPair ? 256 : A.Lq.col_bytes / 16;
+    A.gs = std::min(G, stage_groups(block, ctas));
     A.pb = 1;
     A.qtiles = (A.qpanels + ctas - 1) / ctas;
-    if (ctas == 1 && A.gs == A.Lr.groups)
-        while (2 * A.pb * A.gs <= 4 && 2 * A.pb * A.nt <= 128 && (uint64_t)A.panels * A.qtiles >= 2ull * A.pb * sms) A.pb *= 2;
+    A.split = 1;
+    if (mode == kRing) {
+        // tiles that leave SMs idle are split along the elements, at least four groups to a share
+        const uint64_t tiles = (uint64_t)A.panels * A.qtiles;
+        uint32_t want = 1;
+        while (want < kMaxSplit && tiles * want * 2 <= (uint64_t)sms && G >= 8 * want) want *= 2;
+        while (want > 1 && (want - 1) * A.nt * kFp4Rows * 4 > 96 * 1024) want /= 2;  // the shares' sums, in CTA 0's stages
+        A.per = (G + want - 1) / want;
+        A.split = (G + A.per - 1) / A.per;
+        const uint32_t resident = A.per * (scales + 4 * A.Lq.col_bytes);
+        if (A.qpanels == 1 && (resident <= kResident / 2 || (A.raw && resident <= kResident))) mode = kFew;
+        // several short panels to a tile, while two accumulators fit and every SM still has a tile
+        if (A.gs == G && A.split == 1)
+            while (2 * A.pb * A.gs <= 4 && 2 * A.pb * A.nt <= 128 && tiles >= 2ull * A.pb * sms) A.pb *= 2;
+    } else {
+        A.per = G;
+    }
+    A.gs = std::min(A.gs, A.per);
     A.batches = (A.panels + A.pb * ctas - 1) / (A.pb * ctas);
-    // the panels' part has room for whole groups: an MMA reads 128 rows of two columns whatever the panel has
-    A.b_off = A.pb * A.gs * group;
-    A.bc_off = A.b_off + ctas * A.gs * sub * kFp4ScaleSub;
-    A.stage_bytes = A.bc_off + A.gs * 4 * A.Lq.col_bytes;
-    A.sf_cols = (A.pb + ctas) * A.gs * 4 * sub;
-    A.stages = std::min({kMaxStages, (kSmemLimit - 1024) / A.stage_bytes, (kTmemCols - A.pb * A.nt) / A.sf_cols});
+    const uint32_t fixed = (3 * kMaxStages + 2 * kMaxAcc + 2) * 8 + 16;
+    const uint32_t resident = mode == kFew ? A.per * (scales + 4 * A.Lq.col_bytes) : 0u;
+    for (;; A.gs /= 2) {
+        // the panels' part has room for whole groups: an MMA reads 128 rows of two columns whatever the panel has
+        A.b_off = A.pb * A.gs * group;
+        A.bc_off = A.b_off + (mode == kFew ? 0u : ctas * A.gs * scales);
+        A.stage_bytes = A.bc_off + (mode == kFew ? 0u : A.gs * 4 * A.Lq.col_bytes);
+        A.sf_cols = (A.pb + ctas) * A.gs * 4 * sub;
+        A.stages = std::min({kMaxStages, (kSmemLimit - fixed - resident) / A.stage_bytes, (kTmemCols - A.pb * A.nt) / A.sf_cols});
+        if (A.stages >= 3 || A.gs == 1 || A.pb > 1) break;
+    }
     A.acc = std::min(kMaxAcc, (kTmemCols - A.stages * A.sf_cols) / (A.pb * A.nt));
-    const uint32_t smem = A.stages * A.stage_bytes + (3 * kMaxStages + 2 * kMaxAcc + 1) * 8 + 16;
+    A.res_off = A.stages * A.stage_bytes;
+    A.resc_off = A.res_off + (resident ? A.per * scales : 0u);
+    A.bar_off = A.res_off + resident;
+    const uint32_t smem = A.bar_off + fixed;
     A.band = (uint32_t)std::min<uint64_t>(A.batches, std::max<uint64_t>(8, kBandBytes / (A.Lr.panel_bytes * A.pb * ctas)));
     const uint64_t tiles = (uint64_t)A.batches * A.qtiles;
-    const uint32_t grid = ctas * (uint32_t)std::min<uint64_t>(tiles, (uint64_t)sms / ctas);
+    const uint32_t per_tile = ctas * A.split;
+    const uint32_t grid = per_tile * (uint32_t)std::min<uint64_t>(tiles, (uint64_t)sms / per_tile);
     auto go = [&](auto tag) {
         using T = decltype(tag);
-        if (ctas == 2) return block == 16 ? launch_product<T, 16, 2>(A, grid, smem, s) : launch_product<T, 32, 2>(A, grid, smem, s);
-        return block == 16 ? launch_product<T, 16, 1>(A, grid, smem, s) : launch_product<T, 32, 1>(A, grid, smem, s);
+        if (mode == kPair) return block == 16 ? launch_product<T, 16, kPair>(A, grid, smem, s) : launch_product<T, 32, kPair>(A, grid, smem, s);
+        if (mode == kFew) return block == 16 ? launch_product<T, 16, kFew>(A, grid, smem, s) : launch_product<T, 32, kFew>(A, grid, smem, s);
+        return block == 16 ? launch_product<T, 16, kRing>(A, grid, smem, s) : launch_product<T, 32, kRing>(A, grid, smem, s);
     };
     return dtype == GF_F32 ? go(float{}) : dtype == GF_F16 ? go(__half{}) : go(__nv_bfloat16{});
+}
+
+gf_status check_product(uint32_t m, const void* r_packed, uint32_t n, uint32_t dim, uint32_t block, float scale, const void* out,
+                        uint32_t dtype, uint64_t ld) {
+    if (!fp4_shape(dim, block)) return fail(GF_ERR_ARG, "dim must be positive and block 16 or 32");
+    if (!dtype_bytes(dtype)) return fail(GF_ERR_ARG, "unknown dtype");
+    if (!std::isfinite(scale)) return fail(GF_ERR_ARG, "scale must be finite");
+    if (ld < n) return fail(GF_ERR_ARG, "row stride below n");
+    if (m == 0 || n == 0) return GF_OK;
+    if (!r_packed || !out) return fail(GF_ERR_ARG, "null argument");
+    if (!aligned(r_packed, 16) || !aligned(out, dtype_bytes(dtype))) return fail(GF_ERR_ARG, "misaligned pointer");
+    return GF_OK;
 }
 
 }  // namespace
@@ -619,13 +805,34 @@ using namespace gf;
 extern "C" gf_status gf_product_fp4(const void* q_packed, uint32_t m, const void* r_packed, uint32_t n, uint32_t dim,
                                     uint32_t block, float scale, void* out, uint32_t dtype, uint64_t ld, uint32_t test_wait,
                                     void* stream) {
-    if (!fp4_shape(dim, block)) return fail(GF_ERR_ARG, "dim must be positive and block 16 or 32");
-    if (!dtype_bytes(dtype)) return fail(GF_ERR_ARG, "unknown dtype");
-    if (!std::isfinite(scale)) return fail(GF_ERR_ARG, "scale must be finite");
-    if (ld < n) return fail(GF_ERR_ARG, "row stride below n");
+    const gf_status st = check_product(m, r_packed, n, dim, block, scale, out, dtype, ld);
+    if (st != GF_OK || m == 0 || n == 0) return st;
+    if (!q_packed) return fail(GF_ERR_ARG, "null argument");
+    if (!aligned(q_packed, 16)) return fail(GF_ERR_ARG, "misaligned pointer");
+    return product(ProdArgs{}, q_packed, m, r_packed, n, dim, block, scale, out, dtype, ld, test_wait, (cudaStream_t)stream);
+}
+
+extern "C" gf_status gf_product_fp4_raw(const void* q, uint32_t q_dtype, uint64_t q_ld, uint32_t m, float q_alpha,
+                                        const void* r_packed, uint32_t n, uint32_t dim, uint32_t block, float scale, void* out,
+                                        uint32_t dtype, uint64_t ld, void* workspace, uint32_t test_wait, void* stream) {
+    const gf_status st = check_product(m, r_packed, n, dim, block, scale, out, dtype, ld);
+    if (st != GF_OK) return st;
+    if (!dtype_bytes(q_dtype)) return fail(GF_ERR_ARG, "unknown dtype");
+    if (!fp4_alpha(q_alpha)) return fail(GF_ERR_ARG, "alpha must lie in [2^-126, 2^126]");
+    if (q_ld < dim) return fail(GF_ERR_ARG, "row stride below dim");
     if (m == 0 || n == 0) return GF_OK;
-    if (!q_packed || !r_packed || !out) return fail(GF_ERR_ARG, "null argument");
-    if (!aligned(q_packed, 16) || !aligned(r_packed, 16) || !aligned(out, dtype_bytes(dtype)))
-        return fail(GF_ERR_ARG, "misaligned pointer");
-    return product(q_packed, m, r_packed, n, dim, block, scale, out, dtype, ld, test_wait, (cudaStream_t)stream);
+    if (!q) return fail(GF_ERR_ARG, "null argument");
+    if (!aligned(q, dtype_bytes(q_dtype))) return fail(GF_ERR_ARG, "misaligned pointer");
+    ProdArgs A = {};
+    if (quantised_in_passing(m, dim)) {
+        A.raw = q;
+        A.raw_ld = q_ld;
+        A.raw_dtype = q_dtype;
+        A.q_alpha = q_alpha;
+        return product(A, nullptr, m, r_packed, n, dim, block, scale, out, dtype, ld, test_wait, (cudaStream_t)stream);
+    }
+    if (!workspace) return fail(GF_ERR_ARG, "null argument: this many queries need a workspace");
+    const gf_status sq = gf_quantize_fp4(q, q_dtype, q_ld, m, dim, q_alpha, block, workspace, stream);
+    if (sq != GF_OK) return sq;
+    return product(A, workspace, m, r_packed, n, dim, block, scale, out, dtype, ld, test_wait, (cudaStream_t)stream);
 }

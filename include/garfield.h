@@ -474,8 +474,8 @@ typedef enum { GF_F32 = 0, GF_F16 = 1, GF_BF16 = 2 } gf_dtype;
  * that the last panel lacks are neither written nor used.  gf_fp4_bytes is 0 for a bad shape
  * (dim = 0, or a block other than 16 and 32).
  *
- * Device calls take device pointers on the current device, enqueue one kernel on `stream`,
- * allocate nothing and can be captured into a graph; n = 0 does nothing.  dtype is a gf_dtype;
+ * Device calls take device pointers on the current device, enqueue kernels on `stream`, allocate
+ * nothing and can be captured into a graph; n = 0 does nothing.  dtype is a gf_dtype;
  * ld is the distance between rows in elements, at least dim.  alpha lies in [2^-126, 2^126].
  * _host: host arrays, fp32 rows without gaps; gf_quantize_fp4_host writes the same bytes as
  * gf_quantize_fp4, and 0 in the rows that the last panel lacks.
@@ -499,10 +499,18 @@ gf_status gf_dequantize_fp4_host(const void* packed, uint32_t n, uint32_t dim, u
  * test_wait: 0 in normal use.  Test hook for the timeout path: every wait of the kernel gives up
  * after test_wait polls and every load expects 16 bytes more than it copies; what a CTA then still
  * owes of out becomes NaN.
+ * gf_product_fp4_raw takes the queries as they are (q_dtype, rows q_ld elements apart) and holds them in 4
+ * bits, with q_alpha and the rows' block, for the call.  workspace (device, 16-byte aligned, of
+ * gf_fp4_bytes(m, dim, block) bytes) receives them; it may be NULL when m <= 16, dim <= 8192 and
+ * m * dim <= 32768, for which the product's own kernel quantises them in passing (one launch
+ * instead of two).  The results are those of gf_quantize_fp4 and gf_product_fp4.
  */
 gf_status gf_product_fp4(const void* q_packed, uint32_t m, const void* r_packed, uint32_t n, uint32_t dim,
                          uint32_t block, float scale, void* out, uint32_t dtype, uint64_t ld, uint32_t test_wait,
                          void* stream);
+gf_status gf_product_fp4_raw(const void* q, uint32_t q_dtype, uint64_t q_ld, uint32_t m, float q_alpha,
+                             const void* r_packed, uint32_t n, uint32_t dim, uint32_t block, float scale, void* out,
+                             uint32_t dtype, uint64_t ld, void* workspace, uint32_t test_wait, void* stream);
 
 /* attrs.bin: uint32 n, uint32 a, n*a int32 (tools.cuh:747-765). */
 gf_status gf_read_attrs(const char* path, int32_t** attrs, uint32_t* n, uint32_t* a);

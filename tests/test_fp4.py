@@ -215,3 +215,22 @@ def test_product_refusals(args, word):
     assert L.gf_product_fp4(P(a["q"]), a["m"], P(a["r"]), a["n"], a["dim"], a["block"], a["scale"], P(a["out"]), a["dtype"],
                             a["ld"], 0, None) == 1
     assert word in L.gf_last_error()
+    if args == dict(q=72):
+        return  # aligned to its elements
+    assert L.gf_product_fp4_raw(P(a["q"]), 0, max(a["dim"], 1), a["m"], 1.0, P(a["r"]), a["n"], a["dim"], a["block"], a["scale"],
+                                P(a["out"]), a["dtype"], a["ld"], None, 0, None) == 1
+    assert word in L.gf_last_error()
+
+
+@pytest.mark.parametrize("args,word", [
+    (dict(q_dtype=3), b"dtype"), (dict(q_ld=7), b"stride"), (dict(q_alpha=0.0), b"alpha"), (dict(q_alpha=1e39), b"alpha"),
+    (dict(q=66), b"misaligned"), (dict(m=17), b"workspace"), (dict(dim=8193, q_ld=8193, m=1), b"workspace"),
+    (dict(m=16, dim=2049, q_ld=2049), b"workspace"), (dict(m=17, workspace=72), b"misaligned"),
+])
+def test_raw_product_refusals(args, word):
+    a = dict(q=64, q_dtype=0, q_ld=8, m=3, q_alpha=1.0, dim=8, workspace=0)
+    a.update(args)
+    L, P = gf.lib(), ctypes.c_void_p
+    assert L.gf_product_fp4_raw(P(a["q"]), a["q_dtype"], a["q_ld"], a["m"], a["q_alpha"], P(64), 5, a["dim"], 32, 1.0, P(64), 0, 5,
+                                P(a["workspace"]), 0, None) == 1
+    assert word in L.gf_last_error()

@@ -74,6 +74,7 @@ def test_rows_of_any_alignment(m, n, offset, dtype):
 @pytest.mark.parametrize("m,n,dim", [
     (129, 19001, 96), (256, 18944, 128), (257, 12801, 32), (300, 20000, 33), (1000, 4993, 200), (2000, 2500, 1000),
     (384, 9600, 520), (511, 9473, 384), (1500, 3200, 8192), (5000, 700, 640), (20000, 129, 160), (700, 20000, 416),
+    (129, 19001, 1024), (257, 12801, 1000), (300, 9999, 1057), (1000, 4993, 1320), (20000, 129, 1200), (2049, 4000, 2080),
 ])
 def test_pairs_of_ctas(m, n, dim, block):
     """Enough tiles of 256 x 256 for pairs of CTAs, with odd panel counts on either side."""
@@ -167,6 +168,32 @@ def test_prepared_queries_and_alpha():
     assert torch.equal(gf.product_fp4(rows, rows).double(), r.double() @ r.double().t())
 
 
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("qdtype", DTYPES)
+@pytest.mark.parametrize("m,dim", [(1, 1), (1, 33), (3, 70), (8, 128), (16, 200), (16, 2048), (4, 8192), (1, 8192), (16, 2049),
+                                   (17, 64), (1, 8193), (100, 300), (5, 1000)])
+def test_raw_queries_equal_prepared_ones(m, dim, qdtype, block):
+    """Queries given as they are, few (quantised in passing) or many, strided, are held as quantize_fp4 holds
+    them: the products are equal bit for bit, for one panel of rows (split over a cluster) and many."""
+    x = torch.from_numpy(data(m, dim + 3, dim, "normal")).to(qdtype).cuda()
+    q = x[:, 3:] if dim % 2 else x[:, :dim]
+    for n in (90, 3000, 40000 if dim <= 200 else 1000):
+        rows = gf.quantize_fp4(torch.from_numpy(data(n, dim, 1, "normal")).cuda(), 4.0, block)
+        for alpha in (1.0, 0.7):
+            a = gf.product_fp4(q, rows, query_alpha=alpha)
+            b = gf.product_fp4(gf.quantize_fp4(q, alpha, block), rows)
+            assert torch.equal(a, b), (n, alpha)
+
+
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("m,n,dim", [(1, 100, 8192), (16, 1000, 8192), (20, 500, 4096), (128, 130, 8192), (100, 129, 3000),
+                                     (300, 256, 8192), (64, 4000, 2000), (1, 128, 1024), (1, 9000, 8000), (200, 128, 1100)])
+def test_tiles_split_along_the_elements(m, n, dim, block):
+    """Few tiles of long rows: shares of the elements in a cluster, added in its first CTA."""
+    check_exact(m, n, dim, block)
+    check_exact(m, n, dim, block, torch.bfloat16)
+
+
 def test_repeats_are_equal():
     q = torch.from_numpy(data(70, 3000, 3, "normal")).cuda()
     rows = gf.quantize_fp4(torch.from_numpy(data(500, 3000, 4, "normal")).cuda())
@@ -236,10 +263,10 @@ def test_store_score_read_together():
     assert ((scores.gather(1, top).double() - again).abs() <= 2.0 ** -20 * ref).all()
 
 
-@pytest.mark.parametrize("m,n", [(20, 1000), (300, 19000)])
-def test_waits_that_run_out(m, n):
+@pytest.mark.parametrize("m,n,dim", [(20, 1000, 300), (300, 19000, 300), (300, 19000, 1100), (1, 500, 4096), (100, 500, 4096)])
+def test_waits_that_run_out(m, n, dim):
     """The timeout path: outputs owed become NaN, and the next call is sound."""
-    q, r = exact_rows(m, 300, 32, 1), exact_rows(n, 300, 32, 2)
+    q, r = exact_rows(m, dim, 32, 1), exact_rows(n, dim, 32, 2)
     rows = gf.quantize_fp4(r)
     got = gf.product_fp4(q, rows, test_wait=4)
     assert torch.isnan(got).all()
