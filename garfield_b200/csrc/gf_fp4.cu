@@ -93,16 +93,14 @@ __global__ void __launch_bounds__(kThreads, 6) fp4_quantize_kernel(const T* __re
                 if (o % kBo == 0) scales_s[fp4_scale_at(r, o / kBo)] = (uint8_t)s8;  // (0 for a block past the row's end)
             }
         };
-        if (valid == kFp4Rows && dim % kOct == 0) {  // every thread has eight elements or none, in every row
+        if (valid == kFp4Rows && dim % kV == 0) {  // a load's elements all exist or none does, the same in every row
             for (uint32_t r0 = 0; r0 < kFp4Rows; r0 += rstep * kRows) {
                 Oct q[kRows] = {};
-                if (left) {
 #pragma unroll
-                    for (uint32_t u = 0; u < kRows; ++u)
+                for (uint32_t u = 0; u < kRows; ++u)
 #pragma unroll
-                        for (uint32_t w = 0; w < kOct / kV; ++w)
-                            q[u][w] = *reinterpret_cast<const Vec<T, W>*>(src + u * step + w * kV);
-                }
+                    for (uint32_t w = 0; w < kOct / kV; ++w)
+                        if (left > w * kV) q[u][w] = *reinterpret_cast<const Vec<T, W>*>(src + u * step + w * kV);
                 src += step * kRows;
 #pragma unroll
                 for (uint32_t u = 0; u < kRows; ++u) encode(q[u], r0 + first + u * rstep, o < 4 * cols);
@@ -178,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 6) fp4_dequantize_kernel(const uint8
             }
             dst += step;
         };
-        if (valid == kFp4Rows && left >= kV && rstep * kRows <= kFp4Rows) {
+        if (valid == kFp4Rows && rstep * kRows <= kFp4Rows) {
             for (; r < kFp4Rows; r += rstep * kRows) {
                 uint32_t c[kRows], s8[kRows];
 #pragma unroll
@@ -187,7 +185,7 @@ __global__ void __launch_bounds__(kThreads, 6) fp4_dequantize_kernel(const uint8
                     s8[u] = src_s[fp4_scale_at(r + u * rstep, k0 / BLOCK)];
                 }
 #pragma unroll
-                for (uint32_t u = 0; u < kRows; ++u) write(c[u], s8[u], true);
+                for (uint32_t u = 0; u < kRows; ++u) write(c[u], s8[u], left >= kV);
             }
         } else {
             for (; r < valid; r += rstep) write(codes_of(r), src_s[fp4_scale_at(r, k0 / BLOCK)], left >= kV);
