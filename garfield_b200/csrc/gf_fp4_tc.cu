@@ -43,7 +43,7 @@ constexpr uint32_t kMaxStages = 8;
 constexpr uint32_t kMaxAcc = 8;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kPolls = 1u << 20;
-constexpr uint64_t kBandBytes = 32u << 20;  // of row panels, a quarter of L2
+constexpr uint64_t kBandBytes = 64u << 20;  // of row panels, half of L2
 constexpr uint32_t kSmemLimit = 227 * 1024;
 
 // Zeros for the second column of an MMA step that the rows' last group lacks: with zero codes on the
@@ -55,9 +55,9 @@ constexpr uint32_t ctas_of(uint32_t mode) { return mode == kPair ? 2 : 1; }
 constexpr uint32_t kResident = 128 * 1024;  // bytes of queries kept in shared memory, at most
 constexpr uint32_t kMaxSplit = 8;           // CTAs of a cluster that share a tile
 
-// Groups of a full stage: four, or three where two query panels' scales of 16-element blocks would leave
-// TMEM no room for a third stage beside an accumulator of 256 columns.
-constexpr uint32_t stage_groups(uint32_t block, uint32_t ctas) { return ctas == 2 && block == 16 ? 3 : 4; }
+// Groups of a full stage: four; three for a pair, whose fourth stage is worth more (8192^3, blocks of 32: 186 us
+// against 191) and whose two query panels' scales of 16-element blocks take most of TMEM.
+constexpr uint32_t stage_groups(uint32_t ctas) { return ctas == 2 ? 3 : 4; }
 
 struct ProdArgs {
     const uint8_t *r, *q;
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
     extern __shared__ __align__(1024) unsigned char sm[];
     constexpr uint32_t CTAS = ctas_of(MODE);
     constexpr uint32_t kSub = BLOCK == 16 ? 2 : 1;  // scale sub-blocks of a group
-    constexpr uint32_t kGs = stage_groups(BLOCK, CTAS);
+    constexpr uint32_t kGs = stage_groups(CTAS);
     uint64_t* full = reinterpret_cast<uint64_t*>(sm + A.bar_off);
     uint64_t* pfull = full + kMaxStages;  // CTA 0 of a pair: the other CTA's stage is full
     uint64_t* empty = pfull + kMaxStages;
@@ -633,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
                     if (j < A.n && c < rows) store16<T, CTAS == 1>(out + (uint64_t)(q0 + c) * A.ld + j, A.ld, v[y], A.scale, rows - c);
                     if (CTAS == 1) {  // the next chunk of this warp's, perhaps of the next panel
                         c += 16 * dx;
-                        if (c >= A.nt) {
+                        while (c >= A.nt) {
                             c -= A.nt;
                             ++p;
                         }
@@ -728,13 +728,20 @@ gf_status product(ProdArgs A, const void* q, uint32_t m, const void* r, uint32_t
     A.polls = test_wait ? test_wait : kPolls;
     A.extra_tx = test_wait ? 16u : 0u;
     const uint32_t sub = block == 16 ? 2 : 1, scales = sub * kFp4ScaleSub, group = scales + 4 * kFp4ColBytes, G = A.Lr.groups;
-    // pairs of CTAs once their tiles, of 256 x 256, occupy every SM and the rows are long enough for
-    // their arithmetic to show (8192 x 16384 in bf16: 103 us either way at 1024 elements, 107 against 92 at 128)
+    // Pairs of CTAs once their tiles, of 256 x 256, occupy every SM, where the rows are long enough for
+    // their arithmetic to show (8192 x 16384 in bf16: 102 us either way at 1024 elements, 126 against 157 at 2048,
+    // 107 against 92 at 128), and where out is far larger than L2 and its rows leave sectors half
+    // written or are fp32: a pair writes twice as long a run of each row at a time (10000 x 99999 x 128
+    // in fp16 808 us against 1226, fp32 1664 against 1879; 10000 x 100000 in fp32 820 against 886, but fp16 805
+    // against 632).
     const uint64_t pair_tiles = ((uint64_t)A.panels + 1) / 2 * ((A.qpanels + 1) / 2);
-    uint32_t mode = G >= 8 && A.qpanels >= 2 && pair_tiles >= (uint64_t)sms / 2 ? kPair : kRing;
+    const uint32_t es = dtype_bytes(dtype);
+    const bool torn = (reinterpret_cast<uintptr_t>(out) | ld * es) % 32 != 0;
+    const bool large = m >= 1024 && (uint64_t)m * n >= (1ull << 30) / es && (torn || es == 4);
+    uint32_t mode = (G >= 8 || large) && A.qpanels >= 2 && pair_tiles >= (uint64_t)sms / 2 ? kPair : kRing;
     const uint32_t ctas = ctas_of(mode);
     A.nt = mode == kPair ? 256 : A.Lq.col_bytes / 16;
-    A.gs = std::min(G, stage_groups(block, ctas));
+    A.gs = std::min(G, stage_groups(ctas));
     A.pb = 1;
     A.qtiles = (A.qpanels + ctas - 1) / ctas;
     A.split = 1;

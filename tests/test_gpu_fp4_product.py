@@ -27,7 +27,8 @@ def exact_rows(n, dim, block, seed):
 
 def check_exact(m, n, dim, block, dtype=torch.float32):
     q, r = exact_rows(m, dim, block, m + dim), exact_rows(n, dim, block, 7 * n + dim)
-    got = gf.product_fp4(q, gf.quantize_fp4(r, 1.0, block), dtype)
+    out = torch.full((m, n), float("nan"), dtype=dtype, device="cuda")  # nothing may be left unwritten
+    got = gf.product_fp4(q, gf.quantize_fp4(r, 1.0, block), out=out)
     want = q.double() @ r.double().t()
     if dtype == torch.float32:
         assert torch.equal(got.double(), want)
@@ -55,6 +56,13 @@ def test_row_counts(n, block):
     check_exact(1, n, 96, block)
     check_exact(40, n, 128, block)
     check_exact(300, n, 100, block)
+
+
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("dim", [32, 96, 128, 256])
+@pytest.mark.parametrize("m,n", [(1, 80_000), (3, 200_001), (16, 100_000), (17, 90_001), (33, 120_000), (64, 81_000), (65, 80_001)])
+def test_several_panels_to_a_tile(m, n, dim, block):
+    check_exact(m, n, dim, block)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
