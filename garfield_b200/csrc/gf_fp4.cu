@@ -56,6 +56,8 @@ __global__ void __launch_bounds__(kThreads, 6) fp4_quantize_kernel(const T* __re
     constexpr uint32_t kRows = 2;                           // rows in flight per thread: at most 64 * 2 per step
     __shared__ __align__(16) uint8_t scales_s[kSb];
     const uint32_t p = blockIdx.x;
+    wait_for_previous();
+    let_next_start();
     for (uint32_t g = blockIdx.y; g < Lo.groups; g += gridDim.y) {
         const uint32_t row0 = p * kFp4Rows, valid = min(kFp4Rows, n - row0);
         const uint32_t cols = min(4u, Lo.cols - 4 * g), lsh = row_shift(cols, 4);
@@ -141,6 +143,7 @@ __global__ void __launch_bounds__(kThreads, 6) fp4_dequantize_kernel(const uint8
     constexpr uint32_t kCb = kV / 2;                            // their bytes of codes
     constexpr uint32_t kRows = 4;                               // rows in flight per thread
     const uint32_t p = blockIdx.x;
+    wait_for_previous();
     for (uint32_t g = blockIdx.y; g < Lo.groups; g += gridDim.y) {
         const uint32_t row0 = p * kFp4Rows, valid = min(kFp4Rows, n - row0);
         const uint32_t lsh = row_shift(min(4u, Lo.cols - 4 * g), kFp4Col / kV);
@@ -286,25 +289,38 @@ uint32_t row_alignment(const void* p, uint64_t ld, uint32_t esize) {
     return a % 16 == 0 ? 16 : a % 8 == 0 ? 8 : esize;
 }
 
+template <typename... P, typename... A>
+gf_status launch(void (*k)(P...), dim3 grid, cudaStream_t s, A... args) {
+    cudaLaunchAttribute at = early_start();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = s;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    GF_CUDA(cudaLaunchKernelEx(&cfg, k, args...));
+    return GF_OK;
+}
+
 template <typename T, uint32_t BLOCK>
-void launch_quantize(const void* data, uint64_t ld, uint32_t n, uint32_t dim, float alpha, uint8_t* packed, cudaStream_t s) {
+gf_status launch_quantize(const void* data, uint64_t ld, uint32_t n, uint32_t dim, float alpha, uint8_t* packed, cudaStream_t s) {
     const Fp4Layout Lo = fp4_layout(n, dim, BLOCK);
     const T* x = static_cast<const T*>(data);
     const uint32_t w = row_alignment(data, ld, sizeof(T));
     auto* k = w == 16 ? fp4_quantize_kernel<T, BLOCK, 16>
               : w == 8 ? fp4_quantize_kernel<T, BLOCK, 8>
                        : fp4_quantize_kernel<T, BLOCK, sizeof(T)>;
-    k<<<grid_of(n, Lo), kThreads, 0, s>>>(x, ld, n, dim, alpha, packed, Lo);
+    return launch(k, grid_of(n, Lo), s, x, ld, n, dim, alpha, packed, Lo);
 }
 template <typename T, uint32_t BLOCK>
-void launch_dequantize(const uint8_t* packed, uint32_t n, uint32_t dim, float alpha, void* out, uint64_t ld, cudaStream_t s) {
+gf_status launch_dequantize(const uint8_t* packed, uint32_t n, uint32_t dim, float alpha, void* out, uint64_t ld, cudaStream_t s) {
     const Fp4Layout Lo = fp4_layout(n, dim, BLOCK);
     T* y = static_cast<T*>(out);
     const uint32_t w = row_alignment(out, ld, sizeof(T));
     auto* k = w == 16 ? fp4_dequantize_kernel<T, BLOCK, 16>
               : w == 8 ? fp4_dequantize_kernel<T, BLOCK, 8>
                        : fp4_dequantize_kernel<T, BLOCK, sizeof(T)>;
-    k<<<grid_of(n, Lo), kThreads, 0, s>>>(packed, n, dim, 1.0f / alpha, y, ld, Lo);
+    return launch(k, grid_of(n, Lo), s, packed, n, dim, 1.0f / alpha, y, ld, Lo);
 }
 
 }  // namespace
@@ -331,19 +347,10 @@ extern "C" gf_status gf_quantize_fp4(const void* data, uint32_t dtype, uint64_t 
     uint8_t* out = static_cast<uint8_t*>(packed_out);
     auto go = [&](auto tag) {
         using T = decltype(tag);
-        if (block == 16)
-            launch_quantize<T, 16>(data, ld, n, dim, alpha, out, s);
-        else
-            launch_quantize<T, 32>(data, ld, n, dim, alpha, out, s);
+        return block == 16 ? launch_quantize<T, 16>(data, ld, n, dim, alpha, out, s)
+                           : launch_quantize<T, 32>(data, ld, n, dim, alpha, out, s);
     };
-    if (dtype == GF_F32)
-        go(float{});
-    else if (dtype == GF_F16)
-        go(__half{});
-    else
-        go(__nv_bfloat16{});
-    GF_CUDA(cudaGetLastError());
-    return GF_OK;
+    return dtype == GF_F32 ? go(float{}) : dtype == GF_F16 ? go(__half{}) : go(__nv_bfloat16{});
 }
 
 extern "C" gf_status gf_dequantize_fp4(const void* packed, uint32_t n, uint32_t dim, uint32_t block, float alpha, void* out,
@@ -359,19 +366,10 @@ extern "C" gf_status gf_dequantize_fp4(const void* packed, uint32_t n, uint32_t 
     const uint8_t* in = static_cast<const uint8_t*>(packed);
     auto go = [&](auto tag) {
         using T = decltype(tag);
-        if (block == 16)
-            launch_dequantize<T, 16>(in, n, dim, alpha, out, ld, s);
-        else
-            launch_dequantize<T, 32>(in, n, dim, alpha, out, ld, s);
+        return block == 16 ? launch_dequantize<T, 16>(in, n, dim, alpha, out, ld, s)
+                           : launch_dequantize<T, 32>(in, n, dim, alpha, out, ld, s);
     };
-    if (dtype == GF_F32)
-        go(float{});
-    else if (dtype == GF_F16)
-        go(__half{});
-    else
-        go(__nv_bfloat16{});
-    GF_CUDA(cudaGetLastError());
-    return GF_OK;
+    return dtype == GF_F32 ? go(float{}) : dtype == GF_F16 ? go(__half{}) : go(__nv_bfloat16{});
 }
 
 extern "C" gf_status gf_quantize_fp4_host(const float* data, uint32_t n, uint32_t dim, float alpha, uint32_t block,

@@ -12,6 +12,12 @@ namespace fp4 {
 
 constexpr uint32_t kOct = 8;  // elements that one thread quantises
 
+// The format's kernels may start while the kernel before them on the stream still runs, and wait for its end
+// before they touch memory: what overlaps is their launch and set-up.  The quantiser lets the next kernel
+// start at once; the others leave that to their end.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -102,6 +108,14 @@ __device__ __forceinline__ uint32_t encode8(float* x, float amax, uint32_t& code
     }
     codes = ef == 255u || (BLOCK == 16 && s8 == 0u) ? 0u : e2m1x8(x);
     return s8;
+}
+
+// Launch attribute of a kernel that begins with wait_for_previous.
+inline cudaLaunchAttribute early_start() {
+    cudaLaunchAttribute a = {};
+    a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a.val.programmaticStreamSerializationAllowed = 1;
+    return a;
 }
 
 }  // namespace fp4

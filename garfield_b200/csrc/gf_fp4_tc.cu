@@ -390,6 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
     }
     sync_all<CTAS>();
     const uint32_t tmem = *tmem_slot;
+    wait_for_previous();  // (nothing above touches global memory)
 
     bool done = true;  // epilogue warps of a split tile: the sums are in TMEM
     if (warp == 0) {
@@ -695,11 +696,12 @@ gf_status launch_product(const ProdArgs& A, uint32_t grid, uint32_t smem, cudaSt
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim = {MODE == kPair ? 2 : A.split, 1, 1};
+    cudaLaunchAttribute at[2];
+    at[0] = early_start();
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim = {MODE == kPair ? 2 : A.split, 1, 1};
     cfg.attrs = at;
-    cfg.numAttrs = at[0].val.clusterDim.x > 1 ? 1 : 0;
+    cfg.numAttrs = at[1].val.clusterDim.x > 1 ? 2 : 1;
     GF_CUDA(cudaLaunchKernelEx(&cfg, fp4_product_kernel<T, BLOCK, MODE>, A));
     return GF_OK;
 }
@@ -753,7 +755,7 @@ gf_status product(ProdArgs A, const void* q, uint32_t m, const void* r, uint32_t
         while (want > 1 && (want - 1) * A.nt * kFp4Rows * 4 > 96 * 1024) want /= 2;  // the shares' sums, in CTA 0's stages
         A.per = (G + want - 1) / want;
         A.split = (G + A.per - 1) / A.per;
-        const uint32_t resident = A.per * (scales + 4 * A.Lq.col_bytes);
+        const uint64_t resident = (uint64_t)A.per * (scales + 4 * A.Lq.col_bytes);
         if (A.qpanels == 1 && (resident <= kResident / 2 || (A.raw && resident <= kResident))) mode = kFew;
         // several short panels to a tile, while two accumulators fit and every SM still has a tile
         if (A.gs == G && A.split == 1)
