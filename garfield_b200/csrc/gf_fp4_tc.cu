@@ -21,7 +21,7 @@
 //
 // Warp 0 copies scales and codes, one run each, into a ring of stages of up to four groups (of a
 // panel, or of several panels that fit whole); warp 1 spreads the stage's scales into TMEM
-// (tcgen05.cp) and issues two MMAs of 64 elements per panel and group; eight warps read
+// (tcgen05.cp) and issues two MMAs of 64 elements per panel and group; the other warps read
 // finished accumulators and write out.  The stages are this long because a warp pays some 450
 // cycles a stage whatever it holds (waiting, committing, the first instruction's way), while a group's
 // MMAs take 128 cycles at N = 128 and its panel's bytes 200 at the HBM rate.
@@ -38,7 +38,13 @@ namespace {
 using namespace dev;
 using namespace fp4;
 
-constexpr uint32_t kThreads = 320;    // producer warp, MMA warp, 8 epilogue warps
+// Epilogue groups of four warps, one per TMEM lane quarter.  A pair's two share a tile's columns: its one
+// accumulator is free sooner.  Otherwise they take tiles in turn, so that one stores while another waits and
+// reads (10000 x 100000 x 128 in fp16: 643 us when two shared each tile, 593 with two and 490 with three in
+// turn).  A group that waits for a tile has seen the one before its last, so with as many
+// accumulators as groups it has seen that accumulator's previous use, and a phase's parity is unambiguous.
+constexpr uint32_t epi_groups(uint32_t ctas) { return ctas == 2 ? 2 : 3; }
+constexpr uint32_t threads_of(uint32_t ctas) { return 64 + 128 * epi_groups(ctas); }  // and a producer and an MMA warp
 constexpr uint32_t kMaxStages = 8;
 constexpr uint32_t kMaxAcc = 8;
 constexpr uint32_t kTmemCols = 512;
@@ -313,13 +319,13 @@ __device__ __forceinline__ void load8(const void* base, uint64_t at, uint32_t le
 }
 
 // This CTA's share of the queries (groups gb .. ge - 1), quantised into shared memory in the packed
-// panel's form by the epilogue's 256 threads (t: this one's number).
-template <uint32_t BLOCK>
+// panel's form by the epilogue's threads (t: this one's number).
+template <uint32_t BLOCK, uint32_t THREADS>
 __device__ __forceinline__ void quantize_queries(const ProdArgs& A, uint32_t gb, uint32_t ge, uint32_t dim, unsigned char* scales,
                                                  unsigned char* codes, uint32_t t) {
     const uint32_t octs = (ge - gb) * (kFp4Group / kOct), total = A.m * octs;
     const uint32_t cols = min(4 * ge, (A.Lq.cols + 1) & ~1u) - 4 * gb;  // with the zeros that complete an MMA step
-    for (uint32_t i0 = t & ~31u; i0 < total; i0 += 256) {
+    for (uint32_t i0 = t & ~31u; i0 < total; i0 += THREADS) {
         const uint32_t i = i0 + (t & 31u);  // (a row's octs are a multiple of 16: a block's threads share a row)
         const bool in = i < total;
         const uint32_t row = in ? i / octs : 0, o = in ? i - row * octs : 0;
@@ -349,7 +355,7 @@ __device__ __forceinline__ void quantize_queries(const ProdArgs& A, uint32_t gb,
 }
 
 template <typename T, uint32_t BLOCK, uint32_t MODE>
-__global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_constant__ ProdArgs A) {
+__global__ void __launch_bounds__(threads_of(ctas_of(MODE)), 1) fp4_product_kernel(const __grid_constant__ ProdArgs A) {
     extern __shared__ __align__(1024) unsigned char sm[];
     constexpr uint32_t CTAS = ctas_of(MODE);
     constexpr uint32_t kSub = BLOCK == 16 ? 2 : 1;  // scale sub-blocks of a group
@@ -370,7 +376,6 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
     const uint32_t workers = CTAS == 2 ? gridDim.x / 2 : gridDim.x / A.split;
     const uint32_t G = A.Lr.groups, gb = share * A.per, ge = min(G, gb + A.per);
     const uint32_t cpp = A.nt / 16;     // 16-column chunks of a panel's accumulator
-    const bool halves = A.pb * cpp > 1;  // both epilogue halves share a tile's chunks, else they take alternate tiles
 
     if (warp == 0) tmem_alloc<CTAS>(tmem_slot);
     if (threadIdx.x == 0) {
@@ -381,10 +386,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         }
         for (uint32_t i = 0; i < kMaxAcc; ++i) {
             mbar_init(&tfull[i], 1);
-            mbar_init(&tempty[i], (halves ? 8 : 4) * CTAS);
+            mbar_init(&tempty[i], CTAS == 2 ? 4 * 2 * epi_groups(2) : 4);
         }
         mbar_init(drain, 1);
-        mbar_init(qfull, A.raw ? 8 : 1);
+        mbar_init(qfull, A.raw ? 4 * epi_groups(CTAS) : 1);
         *stop = 0;
         fence_mbar_init();
     }
@@ -575,34 +580,38 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         __syncwarp();
     } else {
         // -------------------------------------------------------------- epilogue warps
-        constexpr uint32_t kBatch = CTAS == 2 ? 8 : 4;  // chunks read before any is stored
-        const uint32_t qq = warp & 3u, h = (warp - 2) >> 2;  // lane quarter, half
+        constexpr uint32_t kBatch = CTAS == 2 ? 8 : 2;  // chunks read before any is stored
+        const uint32_t qq = warp & 3u, h = (warp - 2) >> 2;  // lane quarter, group
         const uint32_t acc_cols = A.pb * A.nt;
         T* out = static_cast<T*>(A.out);
         if (MODE == kFew && A.raw) {
-            quantize_queries<BLOCK>(A, gb, ge, A.dim, sm + A.res_off, sm + A.resc_off, threadIdx.x - 64);
+            quantize_queries<BLOCK, 128 * epi_groups(CTAS)>(A, gb, ge, A.dim, sm + A.res_off, sm + A.resc_off, threadIdx.x - 64);
             if (lane == 0) mbar_arrive(qfull);
         }
         bool ok = true;
         uint32_t u = 0;
         Ring accs;
-        for (Tiles t(worker, workers, A.band, A.batches, A.qtiles); t.more(); t.next(), ++u, accs.next(A.acc)) {
+        for (Tiles t(worker, workers, A.band, A.batches, A.qtiles); t.more(); t.next(), accs.next(A.acc)) {
             if (CTAS == 1 && A.split > 1) {  // the cluster's one tile, stored below
                 done = __all_sync(kFull, bwait(&tfull[0], 0, stop, A.polls));
                 ok = done;
                 break;
             }
-            if (!halves && (u & 1u) != h) continue;
+            if (CTAS == 1) {  // the groups take tiles in turn
+                const bool mine = u == h;
+                u = u + 1 == epi_groups(CTAS) ? 0 : u + 1;
+                if (!mine) continue;
+            }
             const uint32_t p0 = t.batch() * A.pb * CTAS + rank, q0 = t.q * A.nt;
             const uint32_t np = CTAS == 2 ? 1u : min(A.pb, A.panels - p0);
             const uint32_t rows = min(A.nt, A.m - q0);
-            const uint32_t chunks = np * cpp, x0 = halves ? h : 0, dx = halves ? 2 : 1;
+            const uint32_t chunks = np * cpp, x0 = CTAS == 2 ? h : 0, dx = CTAS == 2 ? epi_groups(2) : 1;
             const uint32_t addr = tmem + (qq * 32 << 16) + accs.i * acc_cols;
             if (ok) {
                 ok = __all_sync(kFull, bwait(&tfull[accs.i], accs.par, stop, A.polls));
                 tc_fence_after();
             }
-            uint32_t p = CTAS == 1 && cpp == 1 ? x0 : 0, c = cpp == 1 ? 0 : x0 * 16;  // panel and column of chunk x
+            uint32_t p = 0, c = x0 * 16;  // panel and column of chunk x
             for (uint32_t x = x0; x < chunks || x == x0; x += kBatch * dx) {
                 uint32_t v[kBatch][16];
                 __syncwarp();  // tcgen05.ld is warp-collective
@@ -633,9 +642,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
                     const uint64_t j = (uint64_t)(p0 + p) * kFp4Rows + qq * 32 + lane;
                     if (j < A.n && c < rows) store16<T, CTAS == 1>(out + (uint64_t)(q0 + c) * A.ld + j, A.ld, v[y], A.scale, rows - c);
                     if (CTAS == 1) {  // the next chunk of this warp's, perhaps of the next panel
-                        c += 16 * dx;
-                        while (c >= A.nt) {
-                            c -= A.nt;
+                        c += 16;
+                        if (c == A.nt) {
+                            c = 0;
                             ++p;
                         }
                     }
@@ -658,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_product_kernel(const __grid_c
         tc_fence_after();
         for (uint32_t pass = 0; pass < 2; ++pass) {
             if (warp >= 2 && (pass == 0) == (share != 0))
-                for (uint32_t c = ((warp - 2) >> 2) * 16; c < rows; c += 32) {
+                for (uint32_t c = ((warp - 2) >> 2) * 16; c < rows; c += 16 * epi_groups(CTAS)) {
                     uint32_t v[16];
                     __syncwarp();
                     tmem_ld16(addr + c, v);
@@ -693,7 +702,7 @@ gf_status launch_product(const ProdArgs& A, uint32_t grid, uint32_t smem, cudaSt
     GF_CUDA(cudaFuncSetAttribute(fp4_product_kernel<T, BLOCK, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(threads_of(ctas_of(MODE)));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute at[2];
@@ -757,30 +766,43 @@ gf_status product(ProdArgs A, const void* q, uint32_t m, const void* r, uint32_t
         A.split = (G + A.per - 1) / A.per;
         const uint64_t resident = (uint64_t)A.per * (scales + 4 * A.Lq.col_bytes);
         if (A.qpanels == 1 && (resident <= kResident / 2 || (A.raw && resident <= kResident))) mode = kFew;
-        // several short panels to a tile, while two accumulators fit and every SM still has a tile
+        // several short panels to a tile, while every SM still has a tile
         if (A.gs == G && A.split == 1)
             while (2 * A.pb * A.gs <= 4 && 2 * A.pb * A.nt <= 128 && tiles >= 2ull * A.pb * sms) A.pb *= 2;
     } else {
         A.per = G;
     }
     A.gs = std::min(A.gs, A.per);
-    A.batches = (A.panels + A.pb * ctas - 1) / (A.pb * ctas);
     const uint32_t fixed = (3 * kMaxStages + 2 * kMaxAcc + 2) * 8 + 16;
     const uint32_t resident = mode == kFew ? A.per * (scales + 4 * A.Lq.col_bytes) : 0u;
-    for (;; A.gs /= 2) {
+    const uint32_t accs = mode == kPair ? 1 : epi_groups(1);  // accumulators that there have to be
+    for (;;) {
         // the panels' part has room for whole groups: an MMA reads 128 rows of two columns whatever the panel has
         A.b_off = A.pb * A.gs * group;
         A.bc_off = A.b_off + (mode == kFew ? 0u : ctas * A.gs * scales);
         A.stage_bytes = A.bc_off + (mode == kFew ? 0u : A.gs * 4 * A.Lq.col_bytes);
         A.sf_cols = (A.pb + ctas) * A.gs * 4 * sub;
-        A.stages = std::min({kMaxStages, (kSmemLimit - fixed - resident) / A.stage_bytes, (kTmemCols - A.pb * A.nt) / A.sf_cols});
-        if (A.stages >= 3 || A.gs == 1 || A.pb > 1) break;
+        const uint32_t by_smem = (kSmemLimit - fixed - resident) / A.stage_bytes;
+        const uint32_t by_tmem = (kTmemCols - accs * A.pb * A.nt) / A.sf_cols;
+        A.stages = std::min({kMaxStages, by_smem, by_tmem});
+        // two long stages are better than more short ones (8192 x 16384 x 512, blocks of 16: 76 us against 101),
+        // unless it is shared memory that leaves no third: then shorter ones keep more bytes in flight
+        if (A.stages >= 3 || (A.stages == 2 && A.gs >= 3 && by_smem > 2)) break;
+        if (A.pb > 1)  // fewer panels to a tile, else fewer groups to a stage
+            A.pb /= 2;
+        else if (A.gs > 1)
+            A.gs /= 2;
+        else
+            break;
     }
+    A.batches = (A.panels + A.pb * ctas - 1) / (A.pb * ctas);
     A.acc = std::min(kMaxAcc, (kTmemCols - A.stages * A.sf_cols) / (A.pb * A.nt));
     A.res_off = A.stages * A.stage_bytes;
     A.resc_off = A.res_off + (resident ? A.per * scales : 0u);
     A.bar_off = A.res_off + resident;
-    const uint32_t smem = A.bar_off + fixed;
+    // CTAs that wait for others of their cluster hold all of an SM's TMEM meanwhile: more than half of its shared
+    // memory each, so that two never share an SM and no two clusters can hold what the other waits for
+    const uint32_t smem = std::max(A.bar_off + fixed, mode == kPair || A.split > 1 ? 116u * 1024 : 0u);
     A.band = (uint32_t)std::min<uint64_t>(A.batches, std::max<uint64_t>(8, kBandBytes / (A.Lr.panel_bytes * A.pb * ctas)));
     const uint64_t tiles = (uint64_t)A.batches * A.qtiles;
     const uint32_t per_tile = ctas * A.split;
