@@ -84,7 +84,8 @@ struct ProdArgs {
     void* out;
     uint64_t ld;
     float scale;
-    uint32_t dim, bar_off, polls, extra_tx;
+    uint32_t torn;                      // 1: store16_torn, with the groups' buffers at torn_off
+    uint32_t dim, bar_off, torn_off, polls, extra_tx;
 };
 
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -306,6 +307,43 @@ __device__ __forceinline__ void store16(T* d0, uint64_t ld, const uint32_t* v, f
             if (e + 1 < rows) store(d1, __uint_as_float(v[e + 1]) * scale);
             if (e + 2 < rows) store(d2, __uint_as_float(v[e + 2]) * scale);
             if (e + 3 < rows) store(d3, __uint_as_float(v[e + 3]) * scale);
+        }
+    }
+}
+
+// fp32 rows of out that do not start on 32-byte sectors ("torn"): a warp's 32 elements of a row then leave a
+// sector half written at either end, which out of L2 costs twice the time.  A group's four warps gather
+// kTornCols rows' 128 elements in shared memory instead, and a warp writes whole rows, each store within one
+// 128-byte line (10000 x 99977 x 128: 1059 us against 1720; in 16 bits taking words apart costs more than
+// it saves).
+constexpr uint32_t kTornCols = 8;
+constexpr uint32_t kTornPitch = kFp4Rows + 4;                       // floats
+constexpr uint32_t kTornBytes = 2 * kTornCols * kTornPitch * 4;     // of a group: two buffers in turn
+
+// Sixteen columns' values (v: those of this lane's row of the panel) into rows dst, dst + ld, ...; `rows` and n: rows
+// and elements that exist.  All four warps of the group call it alike.
+__device__ __forceinline__ void store16_torn(float* dst, uint64_t ld, const uint32_t* v, float scale, uint32_t rows, uint32_t n,
+                                             float* buf, uint32_t& turn, uint32_t qq, uint32_t lane, uint32_t gid) {
+#pragma unroll
+    for (uint32_t c0 = 0; c0 < 16; c0 += kTornCols) {
+        if (c0 >= rows) break;
+        float* b = buf + turn * (kTornCols * kTornPitch);
+        turn ^= 1u;
+#pragma unroll
+        for (uint32_t e = 0; e < kTornCols; ++e) b[e * kTornPitch + qq * 32 + lane] = __uint_as_float(v[c0 + e]) * scale;
+        __syncwarp();
+        asm volatile("bar.sync %0, 128;" ::"r"(gid + 1) : "memory");
+        // (the buffer's next use follows the next such barrier, which follows these reads)
+#pragma unroll
+        for (uint32_t e = 0; e < kTornCols; e += 4) {
+            if (c0 + e + qq >= rows) continue;
+            float* row = dst + (c0 + e + qq) * ld;
+            const uint32_t skew = (uint32_t)(reinterpret_cast<uintptr_t>(row) >> 2) & 31u;  // elements into the line
+#pragma unroll
+            for (uint32_t k = 0; k < 5; ++k) {
+                const uint32_t w = k * 32 + lane - skew;  // (a large number before the row)
+                if (w < n) row[w] = b[(e + qq) * kTornPitch + w];
+            }
         }
     }
 }
@@ -589,7 +627,7 @@ __global__ void __launch_bounds__(threads_of(ctas_of(MODE)), 1) fp4_product_kern
             if (lane == 0) mbar_arrive(qfull);
         }
         bool ok = true;
-        uint32_t u = 0;
+        uint32_t u = 0, turn = 0;
         Ring accs;
         for (Tiles t(worker, workers, A.band, A.batches, A.qtiles); t.more(); t.next(), accs.next(A.acc)) {
             if (CTAS == 1 && A.split > 1) {  // the cluster's one tile, stored below
@@ -639,8 +677,15 @@ __global__ void __launch_bounds__(threads_of(ctas_of(MODE)), 1) fp4_product_kern
 #pragma unroll
                         for (uint32_t e = 0; e < 16; ++e) v[y][e] = 0x7FC00000u;
                     if (CTAS == 2) c = (x + y * dx) * 16;
-                    const uint64_t j = (uint64_t)(p0 + p) * kFp4Rows + qq * 32 + lane;
-                    if (j < A.n && c < rows) store16<T, CTAS == 1>(out + (uint64_t)(q0 + c) * A.ld + j, A.ld, v[y], A.scale, rows - c);
+                    const uint64_t j0 = (uint64_t)(p0 + p) * kFp4Rows, j = j0 + qq * 32 + lane;
+                    if (CTAS == 1 && sizeof(T) == 4 && A.torn) {
+                        if (c < rows)
+                            store16_torn(reinterpret_cast<float*>(out + (uint64_t)(q0 + c) * A.ld + j0), A.ld, v[y], A.scale, rows - c,
+                                         (uint32_t)min((uint64_t)kFp4Rows, A.n - j0),
+                                         reinterpret_cast<float*>(sm + A.torn_off + h * kTornBytes), turn, qq, lane, h);
+                    } else if (j < A.n && c < rows) {
+                        store16<T, CTAS == 1>(out + (uint64_t)(q0 + c) * A.ld + j, A.ld, v[y], A.scale, rows - c);
+                    }
                     if (CTAS == 1) {  // the next chunk of this warp's, perhaps of the next panel
                         c += 16;
                         if (c == A.nt) {
@@ -740,16 +785,16 @@ gf_status product(ProdArgs A, const void* q, uint32_t m, const void* r, uint32_t
     A.extra_tx = test_wait ? 16u : 0u;
     const uint32_t sub = block == 16 ? 2 : 1, scales = sub * kFp4ScaleSub, group = scales + 4 * kFp4ColBytes, G = A.Lr.groups;
     // Pairs of CTAs once their tiles, of 256 x 256, occupy every SM, where the rows are long enough for
-    // their arithmetic to show (8192 x 16384 in bf16: 102 us either way at 1024 elements, 126 against 157 at 2048,
-    // 107 against 92 at 128), and where out is far larger than L2 and its rows leave sectors half
-    // written or are fp32: a pair writes twice as long a run of each row at a time (10000 x 99999 x 128
-    // in fp16 808 us against 1226, fp32 1664 against 1879; 10000 x 100000 in fp32 820 against 886, but fp16 805
-    // against 632).
+    // their arithmetic to show (8192 x 16384 in bf16: 96 us against 78 at 512 elements, 86 against 97 at 768,
+    // 117 against 151 at 2048), and where out is far larger than L2 and its rows are of 16 bits and torn, or of
+    // 32 and not: a pair writes twice as long a run of each row at a time (10000 x 99999 x 128 in fp16 708 us
+    // against 1059; 20000 x 20000 x 128 in fp32 286 against 310; but 10000 x 100000 x 128 in fp16 704 against
+    // 492, and torn fp32 rows are put together as store16_torn says).
     const uint64_t pair_tiles = ((uint64_t)A.panels + 1) / 2 * ((A.qpanels + 1) / 2);
     const uint32_t es = dtype_bytes(dtype);
-    const bool torn = (reinterpret_cast<uintptr_t>(out) | ld * es) % 32 != 0;
-    const bool large = m >= 1024 && (uint64_t)m * n >= (1ull << 30) / es && (torn || es == 4);
-    uint32_t mode = (G >= 8 || large) && A.qpanels >= 2 && pair_tiles >= (uint64_t)sms / 2 ? kPair : kRing;
+    const bool torn = (reinterpret_cast<uintptr_t>(out) | (m > 1 ? ld * es : 0u)) % 32 != 0;
+    const bool large = m >= 1024 && (uint64_t)m * n >= (1ull << 30) / es && torn == (es == 2);
+    uint32_t mode = (G >= 6 || large) && A.qpanels >= 2 && pair_tiles >= (uint64_t)sms / 2 ? kPair : kRing;
     const uint32_t ctas = ctas_of(mode);
     A.nt = mode == kPair ? 256 : A.Lq.col_bytes / 16;
     A.gs = std::min(G, stage_groups(ctas));
@@ -773,7 +818,9 @@ gf_status product(ProdArgs A, const void* q, uint32_t m, const void* r, uint32_t
         A.per = G;
     }
     A.gs = std::min(A.gs, A.per);
-    const uint32_t fixed = (3 * kMaxStages + 2 * kMaxAcc + 2) * 8 + 16;
+    A.torn = torn && es == 4 && m >= 16 && mode != kPair && A.split == 1;
+    const uint32_t bars = (3 * kMaxStages + 2 * kMaxAcc + 2) * 8 + 16;
+    const uint32_t fixed = bars + (A.torn ? epi_groups(1) * kTornBytes : 0u);
     const uint32_t resident = mode == kFew ? A.per * (scales + 4 * A.Lq.col_bytes) : 0u;
     const uint32_t accs = mode == kPair ? 1 : epi_groups(1);  // accumulators that there have to be
     for (;;) {
@@ -800,6 +847,7 @@ gf_status product(ProdArgs A, const void* q, uint32_t m, const void* r, uint32_t
     A.res_off = A.stages * A.stage_bytes;
     A.resc_off = A.res_off + (resident ? A.per * scales : 0u);
     A.bar_off = A.res_off + resident;
+    A.torn_off = A.bar_off + bars;
     // CTAs that wait for others of their cluster hold all of an SM's TMEM meanwhile: more than half of its shared
     // memory each, so that two never share an SM and no two clusters can hold what the other waits for
     const uint32_t smem = std::max(A.bar_off + fixed, mode == kPair || A.split > 1 ? 116u * 1024 : 0u);

@@ -496,7 +496,7 @@ gf_status gf_dequantize_fp4_host(const void* packed, uint32_t n, uint32_t dim, u
  * are held, summed in fp32 on the tensor cores, multiplied by scale in fp32 and rounded to dtype.
  * scale = 1 / (alpha of q * alpha of r) gives the products of the data; it is finite.  The same
  * call gives the same bits every time.  out must not overlap the inputs.  Rows of out that start
- * on 32-byte boundaries (out and ld) are written faster, up to twice where out is far larger than L2.
+ * on 32-byte boundaries (out and ld) are written faster, by up to a half where out is far larger than L2.
  * Whichever of the two has more rows is best passed as r.
  * test_wait: 0 in normal use.  Test hook for the timeout path: every wait of the kernel gives up
  * after test_wait polls and every load expects 16 bytes more than it copies; what a CTA then still
