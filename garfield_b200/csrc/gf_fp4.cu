@@ -28,6 +28,7 @@
 // (2 rows in flight per thread and 6 CTAs: bf16 1M x 128 in 66 us; 4 rows and the 4 CTAs that
 // their registers allow: 74; 8 rows: 86.)
 #include <algorithm>
+#include <type_traits>
 #include <cmath>
 #include <cstring>
 
@@ -46,7 +47,7 @@ __device__ __forceinline__ uint32_t row_shift(uint32_t cols, uint32_t per) {
 }
 
 // One group of one panel.  W: bytes of a load, which rows are aligned to.
-template <typename T, uint32_t BLOCK, uint32_t W>
+template <typename T, uint32_t BLOCK, uint32_t W, bool FOLD>
 __global__ void __launch_bounds__(kThreads, 6) fp4_quantize_kernel(const T* __restrict__ data, uint64_t ld, uint32_t n,
                                                                 uint32_t dim, float alpha, uint8_t* __restrict__ packed,
                                                                 Fp4Layout Lo) {
@@ -54,7 +55,8 @@ __global__ void __launch_bounds__(kThreads, 6) fp4_quantize_kernel(const T* __re
     constexpr uint32_t kV = W / sizeof(T);                  // elements of a load
     constexpr uint32_t kBo = BLOCK / kOct;                  // threads of a block
     constexpr uint32_t kRows = 2;                           // rows in flight per thread: at most 64 * 2 per step
-    __shared__ __align__(16) uint8_t scales_s[kSb];
+    constexpr uint32_t kB = kFp4Group / BLOCK;              // blocks of a row's group
+    __shared__ __align__(16) uint8_t scales_s[kSb];         // [row][block]
     const uint32_t p = blockIdx.x;
     wait_for_previous();
     let_next_start();
@@ -69,30 +71,23 @@ __global__ void __launch_bounds__(kThreads, 6) fp4_quantize_kernel(const T* __re
         uint8_t* dst = packed + Lo.col_at(p, 4 * g + (o >> 2)) + (o & 3u) * 4;
         // scales of blocks in columns that the group lacks are 0
         if (cols < 4)
-            for (uint32_t i = threadIdx.x; i < kFp4Rows * (128 / BLOCK); i += kThreads) {
-                const uint32_t b = i / kFp4Rows;
-                if (b * BLOCK >= cols * kFp4Col) scales_s[fp4_scale_at(i % kFp4Rows, b)] = 0;
-            }
+            for (uint32_t i = threadIdx.x; i < kSb; i += kThreads)
+                if (i % kB * BLOCK >= cols * kFp4Col) scales_s[i] = 0;
         typedef Vec<T, W> Oct[kOct / kV];
         auto encode = [&](const Oct& q, uint32_t r, bool in) {
             T v[kOct];
 #pragma unroll
             for (uint32_t e = 0; e < kOct; ++e) v[e] = q[e / kV].v[e % kV];
-            float x[kOct], mx = amax8(v);
+            float x[kOct], mx = __fmul_rn(amax8(v), alpha);
 #pragma unroll
             for (uint32_t e = 0; e < kOct; ++e) x[e] = to_f32(v[e]);
-            if (alpha != 1.0f) {  // (rounding keeps order: the largest product is the largest element's)
-                mx = __fmul_rn(mx, alpha);
-#pragma unroll
-                for (uint32_t e = 0; e < kOct; ++e) x[e] = __fmul_rn(x[e], alpha);
-            }
             if (BLOCK == 32) mx = amax2(mx, __shfl_xor_sync(dev::kFull, mx, 2));
             mx = amax2(mx, __shfl_xor_sync(dev::kFull, mx, 1));
             uint32_t c;
-            const uint32_t s8 = encode8<BLOCK>(x, mx, c);
+            const uint32_t s8 = encode8<BLOCK, FOLD>(x, mx, alpha, c);
             if (in) {
                 *reinterpret_cast<uint32_t*>(dst + r * 16) = c;
-                if (o % kBo == 0) scales_s[fp4_scale_at(r, o / kBo)] = (uint8_t)s8;  // (0 for a block past the row's end)
+                if (o % kBo == 0) scales_s[r * kB + o / kBo] = (uint8_t)s8;  // (0 for a block past the row's end)
             }
         };
         if (valid == kFp4Rows && dim % kV == 0) {  // a load's elements all exist or none does, the same in every row
@@ -125,8 +120,8 @@ __global__ void __launch_bounds__(kThreads, 6) fp4_quantize_kernel(const T* __re
         __syncthreads();
         uint32_t* dst_s = reinterpret_cast<uint32_t*>(packed + Lo.scales_at(p, g));
         for (uint32_t i = threadIdx.x; i < kSb / 4; i += kThreads) {
-            const uint32_t r = (i & 3u) * 32 + ((i >> 2) & 31u);
-            if (r < valid) dst_s[i] = reinterpret_cast<const uint32_t*>(scales_s)[i];
+            const uint32_t r = (i & 3u) * 32 + ((i >> 2) & 31u);  // the inverse of fp4_scale_at, four blocks at a time
+            if (r < valid) dst_s[i] = reinterpret_cast<const uint32_t*>(scales_s)[r * (kB / 4) + (i >> 7)];
         }
         __syncthreads();
     }
@@ -307,9 +302,13 @@ gf_status launch_quantize(const void* data, uint64_t ld, uint32_t n, uint32_t di
     const Fp4Layout Lo = fp4_layout(n, dim, BLOCK);
     const T* x = static_cast<const T*>(data);
     const uint32_t w = row_alignment(data, ld, sizeof(T));
-    auto* k = w == 16 ? fp4_quantize_kernel<T, BLOCK, 16>
-              : w == 8 ? fp4_quantize_kernel<T, BLOCK, 8>
-                       : fp4_quantize_kernel<T, BLOCK, sizeof(T)>;
+    auto pick = [&](auto fold) {
+        constexpr bool F = decltype(fold)::value;
+        return w == 16 ? fp4_quantize_kernel<T, BLOCK, 16, F>
+               : w == 8 ? fp4_quantize_kernel<T, BLOCK, 8, F>
+                        : fp4_quantize_kernel<T, BLOCK, sizeof(T), F>;
+    };
+    auto* k = fold_alpha(alpha, BLOCK) ? pick(std::true_type{}) : pick(std::false_type{});
     return launch(k, grid_of(n, Lo), s, x, ld, n, dim, alpha, packed, Lo);
 }
 template <typename T, uint32_t BLOCK>

@@ -4,6 +4,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
+#include <cmath>
+
 #include "gf_device.cuh"
 #include "gf_fp4.h"
 
@@ -55,15 +57,16 @@ __device__ __forceinline__ float scale_to_f32(uint32_t b, bool block16) {
     return __uint_as_float(b == 255u ? 0x7FC00000u : (b == 0u ? 0x00400000u : b << 23));
 }
 
-// max(|a|, |b|), NaN if either is.
+// max(a, b) of magnitudes, NaN if either is.
 __device__ __forceinline__ float amax2(float a, float b) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
 // Largest magnitude of eight elements, NaN if one is; 16-bit elements are compared in pairs.
 __device__ __forceinline__ float amax8(const float* v) {
-    return amax2(amax2(amax2(v[0], v[1]), amax2(v[2], v[3])), amax2(amax2(v[4], v[5]), amax2(v[6], v[7])));
+    return amax2(amax2(amax2(fabsf(v[0]), fabsf(v[1])), amax2(fabsf(v[2]), fabsf(v[3]))),
+                 amax2(amax2(fabsf(v[4]), fabsf(v[5])), amax2(fabsf(v[6]), fabsf(v[7]))));
 }
 __device__ __forceinline__ float amax8(const __half* v) {
     const __half2* h = reinterpret_cast<const __half2*>(v);
@@ -83,23 +86,51 @@ __device__ __forceinline__ float div_by(float x, float y, float r) {
     return __fmaf_rn(-__fmaf_rn(q, y, -x), r, q);
 }
 
-// Scale byte of a block from its largest magnitude, and the codes of this thread's eight elements.
-template <uint32_t BLOCK>
-__device__ __forceinline__ uint32_t encode8(float* x, float amax, uint32_t& codes) {
+// Whether multiplying by alpha can be left to the multiplication by the block's factor: scaling by a power
+// of two commutes with rounding, and in blocks of 32 the factor is one; in blocks of 16 alpha has to be.
+// (Far from the ends of fp32's range, where rounding does not commute; encode8 looks after small blocks.)
+inline bool fold_alpha(float alpha, uint32_t block) {
+    int e = 0;
+    return alpha >= 0x1p-30f && alpha <= 0x1p30f && (block == 32 || std::frexp(alpha, &e) == 0.5f);
+}
+
+// Scale byte of a block and the codes of this thread's eight elements x, which are to be multiplied by alpha.
+// amax: the block's largest magnitude after that multiplication (rounding keeps order: the largest product is
+// the largest element's).  FOLD: fold_alpha.
+template <uint32_t BLOCK, bool FOLD>
+__device__ __forceinline__ uint32_t encode8(float* x, float amax, float alpha, uint32_t& codes) {
     const uint32_t ef = __float_as_uint(amax) >> 23;
+    float f = 1.0f;  // what the elements still have to be multiplied by
+    if (!FOLD) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(x[e], alpha);
+    } else {
+        f = alpha;
+        if (ef < 64u) {  // products may be subnormal, and rounded as such
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(x[e], alpha);
+            f = 1.0f;
+        }
+    }
     uint32_t s8;
     if (BLOCK == 32) {
         s8 = ef == 255u ? 255u : max(ef, 2u) - 2u;
-        const float inv = __uint_as_float((254u - min(s8, 253u)) << 23);  // 1 / s, a power of two
+        f = __fmul_rn(f, __uint_as_float((254u - min(s8, 253u)) << 23));  // f / s, s a power of two
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(x[e], inv);
+        for (int e = 0; e < 8; e += 2) {
+            const dev::f2x y = dev::mul2(dev::pack2(x[e], x[e + 1]), dev::pack2(f, f));
+            x[e] = dev::lo2(y);
+            x[e + 1] = dev::hi2(y);
+        }
     } else {
         s8 = ef == 255u ? 0x7Fu
                         : (uint32_t)__nv_cvt_float_to_fp8(div_by(amax, 6.0f, 1.0f / 6.0f), __NV_SATFINITE, __NV_E4M3);
-        const float s = e4m3_to_f32(s8), r = __frcp_rn(s);
+        // x f / s = x / (s / f) with f a power of two: 1 / f has the exponent 254 - that of f
+        const float sc = e4m3_to_f32(s8), r = __fmul_rn(__frcp_rn(sc), f);
+        const float s = __fmul_rn(sc, __uint_as_float((254u << 23) - __float_as_uint(f)));
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {  // div_by, two at a time
-            const dev::f2x v = dev::pack2(x[e], x[e + 1]), r2 = dev::pack2(r, r), q = dev::mul2(v, r2);
+            const dev::f2x v = dev::pack2(x[e], x[e + 1]), q = dev::mul2(v, dev::pack2(r, r));
             const dev::f2x nr = dev::fma2(q, dev::pack2(s, s), dev::pack2(-x[e], -x[e + 1]));
             const dev::f2x y = dev::fma2(nr, dev::pack2(-r, -r), q);
             x[e] = dev::lo2(y);

@@ -376,13 +376,11 @@ __device__ __forceinline__ void quantize_queries(const ProdArgs& A, uint32_t gb,
             load8<__half>(A.raw, at, left, x);
         else
             load8<__nv_bfloat16>(A.raw, at, left, x);
-#pragma unroll
-        for (uint32_t e = 0; e < kOct; ++e) x[e] = __fmul_rn(x[e], A.q_alpha);
-        float mx = amax8(x);
+        float mx = __fmul_rn(amax8(x), A.q_alpha);
         if (BLOCK == 32) mx = amax2(mx, __shfl_xor_sync(kFull, mx, 2));
         mx = amax2(mx, __shfl_xor_sync(kFull, mx, 1));
         uint32_t c;
-        const uint32_t s8 = encode8<BLOCK>(x, mx, c);
+        const uint32_t s8 = encode8<BLOCK, false>(x, mx, A.q_alpha, c);
         if (!in) continue;
         if (o / 4 < cols) *reinterpret_cast<uint32_t*>(codes + (o / 4) * A.Lq.col_bytes + row * 16 + (o & 3u) * 4) = c;
         if (o % (BLOCK / kOct) == 0)

@@ -49,7 +49,8 @@ SHAPES = [(1, 1), (1, 8192), (3, 96), (64, 31), (127, 32), (128, 128), (130, 33)
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,dim", SHAPES)
 def test_device_matches_host(n, dim, dtype, block):
-    for kind, alpha in (("normal", 16.0), ("wide", 1.0), ("borders", 1.0), ("normal", 0.3)):
+    for kind, alpha in (("normal", 16.0), ("wide", 1.0), ("borders", 1.0), ("normal", 0.3), ("wide", 2.0 ** -100), ("wide", 0.7),
+                        ("borders", 4.0), ("normal", 2.0 ** 20), ("normal", 1e-36)):
         x = torch.from_numpy(data(n, dim, n + dim, kind)).to(dtype)
         same_bytes(gf.quantize_fp4(x.cuda(), alpha, block), gf.quantize_fp4_host(x.float().numpy(), alpha, block))
 
@@ -85,6 +86,18 @@ def test_strided_rows(dtype, dim, offset, gap):
     got = gf.dequantize_fp4(r, out=out[:, offset:offset + dim])
     assert torch.equal(got, gf.dequantize_fp4(r, dtype))
     assert (out[:, :offset] == 7.0).all() and (out[:, offset + dim:] == 7.0).all()
+
+
+@pytest.mark.parametrize("alpha", [1.0, 2.0 ** -30, 2.0 ** 30, 2.0 ** -31, 2.0 ** 100, 0.3, 1e-30])
+@pytest.mark.parametrize("block", [16, 32])
+def test_magnitudes_from_end_to_end(block, alpha):
+    """fp32 data of every binade, subnormal products among them."""
+    rng = np.random.default_rng(7)
+    x = (rng.standard_normal((300, 96)) * 2.0 ** rng.integers(-149, 127, (300, 1))).astype(np.float32)
+    x[::3] *= (2.0 ** rng.integers(-12, 1, (100, 96))).astype(np.float32)
+    x = np.clip(x, -3e38, 3e38)
+    with np.errstate(over="ignore"):
+        same_bytes(gf.quantize_fp4(torch.from_numpy(x).cuda(), alpha, block), gf.quantize_fp4_host(x, alpha, block))
 
 
 @pytest.mark.parametrize("block", [16, 32])
