@@ -11,6 +11,7 @@ CUDA translation unit; the mapping is:
                              + get_partitions_access_order_V2 (gpu_graph.cu:11742)
   Index.search(...)          batch_graph_search_gpu_with_prefilter_and_postfilter (gpu_graph.cu:12464)
   Index.bruteforce(...)      naive_brute_force_with_filter (gpu_graph.cu:10782)
+  quantize_fp4, dequantize_fp4, product_fp4   rows held in 4-bit block floating point (no counterpart)
   read_* / write_*           loaders of tools.cuh / real_dataset_adapter.cuh (formats: Appendix of the docs)
 If the shared library is missing the import still succeeds, but every call that needs
 it raises: there is no CPU fallback.

@@ -320,6 +320,12 @@ constexpr uint32_t kTornCols = 8;
 constexpr uint32_t kTornPitch = kFp4Rows + 4;                       // floats
 constexpr uint32_t kTornBytes = 2 * kTornCols * kTornPitch * 4;     // of a group: two buffers in turn
 
+// The four warps of an epilogue group.
+__device__ __forceinline__ void group_sync(uint32_t gid) {
+    __syncwarp();
+    asm volatile("bar.sync %0, 128;" ::"r"(gid + 1) : "memory");
+}
+
 // Sixteen columns' values (v: those of this lane's row of the panel) into rows dst, dst + ld, ...; `rows` and n: rows
 // and elements that exist.  All four warps of the group call it alike.
 __device__ __forceinline__ void store16_torn(float* dst, uint64_t ld, const uint32_t* v, float scale, uint32_t rows, uint32_t n,
@@ -331,8 +337,7 @@ __device__ __forceinline__ void store16_torn(float* dst, uint64_t ld, const uint
         turn ^= 1u;
 #pragma unroll
         for (uint32_t e = 0; e < kTornCols; ++e) b[e * kTornPitch + qq * 32 + lane] = __uint_as_float(v[c0 + e]) * scale;
-        __syncwarp();
-        asm volatile("bar.sync %0, 128;" ::"r"(gid + 1) : "memory");
+        group_sync(gid);
         // (the buffer's next use follows the next such barrier, which follows these reads)
 #pragma unroll
         for (uint32_t e = 0; e < kTornCols; e += 4) {
@@ -671,6 +676,10 @@ __global__ void __launch_bounds__(threads_of(ctas_of(MODE)), 1) fp4_product_kern
 #pragma unroll
                 for (uint32_t y = 0; y < kBatch; ++y) {
                     if (x + y * dx >= chunks) break;
+                    // in step, the group's warps write the 512 bytes of a row at about the same time, which fp32 rows
+                    // on their way to HBM gain from (10000 x 100000 x 128: 816 us against 845; in fp16 541
+                    // against 500)
+                    if (sizeof(T) == 4 && !(CTAS == 1 && A.torn)) group_sync(h);
                     if (!ok)
 #pragma unroll
                         for (uint32_t e = 0; e < 16; ++e) v[y][e] = 0x7FC00000u;
@@ -785,9 +794,9 @@ gf_status product(ProdArgs A, const void* q, uint32_t m, const void* r, uint32_t
     // Pairs of CTAs once their tiles, of 256 x 256, occupy every SM, where the rows are long enough for
     // their arithmetic to show (8192 x 16384 in bf16: 96 us against 78 at 512 elements, 86 against 97 at 768,
     // 117 against 151 at 2048), and where out is far larger than L2 and its rows are of 16 bits and torn, or of
-    // 32 and not: a pair writes twice as long a run of each row at a time (10000 x 99999 x 128 in fp16 708 us
-    // against 1059; 20000 x 20000 x 128 in fp32 286 against 310; but 10000 x 100000 x 128 in fp16 704 against
-    // 492, and torn fp32 rows are put together as store16_torn says).
+    // 32 and not: a pair writes twice as long a run of each row at a time (10000 x 99999 x 128 in fp16 744 us
+    // against 1066; 10000 x 100000 x 128 in fp32 822 against 848, but in fp16 704 against 492; torn fp32 rows
+    // are put together as store16_torn says).
     const uint64_t pair_tiles = ((uint64_t)A.panels + 1) / 2 * ((A.qpanels + 1) / 2);
     const uint32_t es = dtype_bytes(dtype);
     const bool torn = (reinterpret_cast<uintptr_t>(out) | (m > 1 ? ld * es : 0u)) % 32 != 0;
