@@ -75,12 +75,10 @@ __global__ void __launch_bounds__(kThreads, 6) fp4_quantize_kernel(const T* __re
                 if (i % kB * BLOCK >= cols * kFp4Col) scales_s[i] = 0;
         typedef Vec<T, W> Oct[kOct / kV];
         auto encode = [&](const Oct& q, uint32_t r, bool in) {
-            T v[kOct];
+            float x[kOct];
 #pragma unroll
-            for (uint32_t e = 0; e < kOct; ++e) v[e] = q[e / kV].v[e % kV];
-            float x[kOct], mx = __fmul_rn(amax8(v), alpha);
-#pragma unroll
-            for (uint32_t e = 0; e < kOct; ++e) x[e] = to_f32(v[e]);
+            for (uint32_t e = 0; e < kOct; ++e) x[e] = to_f32(q[e / kV].v[e % kV]);
+            float mx = __fmul_rn(amax8(x), alpha);
             if (BLOCK == 32) mx = amax2(mx, __shfl_xor_sync(dev::kFull, mx, 2));
             mx = amax2(mx, __shfl_xor_sync(dev::kFull, mx, 1));
             uint32_t c;

@@ -63,20 +63,22 @@ __device__ __forceinline__ float amax2(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-// Largest magnitude of eight elements, NaN if one is; 16-bit elements are compared in pairs.
-__device__ __forceinline__ float amax8(const float* v) {
-    return amax2(amax2(amax2(fabsf(v[0]), fabsf(v[1])), amax2(fabsf(v[2]), fabsf(v[3]))),
-                 amax2(amax2(fabsf(v[4]), fabsf(v[5])), amax2(fabsf(v[6]), fabsf(v[7]))));
+// max(|a|, |b|, |c|), NaN if one is.
+__device__ __forceinline__ float amax3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
-__device__ __forceinline__ float amax8(const __half* v) {
-    const __half2* h = reinterpret_cast<const __half2*>(v);
-    const __half2 a = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
-    return amax2(__low2float(a), __high2float(a));
+// Largest magnitude of eight elements, NaN if one is.
+__device__ __forceinline__ float amax8(const float* x) {
+    return amax2(amax3(amax3(x[0], x[1], x[2]), x[6], x[7]), amax3(x[3], x[4], x[5]));
 }
-__device__ __forceinline__ float amax8(const __nv_bfloat16* v) {
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(v);
-    const __nv_bfloat162 a = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
-    return amax2(__low2float(a), __high2float(a));
+// 1 / s correctly rounded for the finite E4M3 values s > 0: one Newton step on the hardware's approximation
+// (a test compares all of them with the division).
+__device__ __forceinline__ float rcp_e4m3(float s) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+    return __fmaf_rn(r, __fmaf_rn(-s, r, 1.0f), r);
 }
 // x / y correctly rounded, for r = 1 / y correctly rounded and results that are normal: one exact
 // remainder corrects the product (Markstein, IBM J. Res. Dev. 34, 1990).  Results too small for that are far
@@ -126,7 +128,7 @@ __device__ __forceinline__ uint32_t encode8(float* x, float amax, float alpha, u
         s8 = ef == 255u ? 0x7Fu
                         : (uint32_t)__nv_cvt_float_to_fp8(div_by(amax, 6.0f, 1.0f / 6.0f), __NV_SATFINITE, __NV_E4M3);
         // x f / s = x / (s / f) with f a power of two: 1 / f has the exponent 254 - that of f
-        const float sc = e4m3_to_f32(s8), r = __fmul_rn(__frcp_rn(sc), f);
+        const float sc = e4m3_to_f32(s8), r = __fmul_rn(rcp_e4m3(sc), f);
         const float s = __fmul_rn(sc, __uint_as_float((254u << 23) - __float_as_uint(f)));
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {  // div_by, two at a time

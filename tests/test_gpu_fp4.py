@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import garfield_b200 as gf
-from test_fp4 import data, held
+from test_fp4 import data, e4m3_values, held
 
 pytestmark = pytest.mark.gpu
 
@@ -86,6 +86,23 @@ def test_strided_rows(dtype, dim, offset, gap):
     got = gf.dequantize_fp4(r, out=out[:, offset:offset + dim])
     assert torch.equal(got, gf.dequantize_fp4(r, dtype))
     assert (out[:, :offset] == 7.0).all() and (out[:, offset + dim:] == 7.0).all()
+
+
+def test_every_e4m3_scale():
+    """Blocks of 16 whose scale takes every E4M3 value, with elements on and next to every code border."""
+    rows = []
+    for s in e4m3_values()[1:]:
+        b = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], np.float64)
+        x = np.concatenate([[6.0 * s], b * s, np.zeros(8)]).astype(np.float32)
+        for step in (0, 1, -1):
+            y = x.copy()
+            if step:
+                y[1:8] = np.nextafter(y[1:8], np.float32(step * 1e9))
+            y[8:] = -y[:8]
+            rows.append(y)
+    x = np.stack(rows)
+    same_bytes(gf.quantize_fp4(torch.from_numpy(x).cuda(), 1.0, 16), gf.quantize_fp4_host(x, 1.0, 16))
+    same_bytes(gf.quantize_fp4(torch.from_numpy(x / 8).cuda(), 8.0, 16), gf.quantize_fp4_host(x, 1.0, 16))
 
 
 @pytest.mark.parametrize("alpha", [1.0, 2.0 ** -30, 2.0 ** 30, 2.0 ** -31, 2.0 ** 100, 0.3, 1e-30])
