@@ -700,6 +700,15 @@ def dequantize_fp4(rows: Fp4Rows, dtype=None, out=None, stream=None):
     return _fp4_run(p.device, stream, _fp4_dequantize, p, rows, dtype, out)
 
 
+def _fp4_scale(query_alpha: float, alpha: float, what: str) -> float:
+    """What the products of the held values are multiplied by.  Outside fp32's normal range it would be rounded
+    to few bits, or to none."""
+    both = query_alpha * alpha
+    if not 2.0 ** -127 <= both <= 2.0 ** 126:
+        raise GarfieldError(1, what, f"query_alpha {query_alpha} * alpha {alpha} must lie in [2^-127, 2^126]")
+    return 1.0 / both
+
+
 def _fp4_product(s, queries, p, rows, dtype, out, query_alpha, test_wait):
     import torch
     what = "gf_product_fp4"
@@ -722,14 +731,12 @@ def _fp4_product(s, queries, p, rows, dtype, out, query_alpha, test_wait):
         ws = None
         if not (m <= 16 and dim <= 8192 and m * dim <= 32768):
             ws = torch.empty(_fp4_size(m, dim, block), dtype=torch.uint8, device=device)
-        if not query_alpha > 0.0:
-            raise GarfieldError(1, what, f"query_alpha {query_alpha} is not positive")
         st = lib().gf_product_fp4_raw(qp.data_ptr(), qdt, qld, m, query_alpha, p.data_ptr(), rows.n, dim, block,
-                                      1.0 / (query_alpha * rows.alpha), out.data_ptr(), dt, ld,
+                                      _fp4_scale(query_alpha, rows.alpha, what), out.data_ptr(), dt, ld,
                                       None if ws is None else ws.data_ptr(), test_wait, s)
     else:
-        st = lib().gf_product_fp4(qp.data_ptr(), m, p.data_ptr(), rows.n, dim, block, 1.0 / (queries.alpha * rows.alpha),
-                                  out.data_ptr(), dt, ld, test_wait, s)
+        st = lib().gf_product_fp4(qp.data_ptr(), m, p.data_ptr(), rows.n, dim, block,
+                                  _fp4_scale(queries.alpha, rows.alpha, what), out.data_ptr(), dt, ld, test_wait, s)
     if st:
         _check(st, what)
     return out
@@ -740,7 +747,7 @@ def product_fp4(queries, rows: Fp4Rows, dtype=None, out=None, query_alpha: float
     """gf_product_fp4: the inner products of every query with every row (m x n, float32 unless dtype or
     out say otherwise).  queries: Fp4Rows of the same dim and block, or a float32, float16 or
     bfloat16 CUDA matrix, which is held in 4 bits (quantize_fp4 with query_alpha and the rows'
-    block) for the call (gf_product_fp4_raw)."""
+    block) for the call (gf_product_fp4_raw).  The product of both alphas lies in [2^-127, 2^126]."""
     import torch
     p = _fp4_rows(rows, "gf_product_fp4")
     if not isinstance(queries, Fp4Rows) and not getattr(queries, "is_cuda", False):

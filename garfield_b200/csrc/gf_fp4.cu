@@ -271,8 +271,6 @@ void dequantize_host(const uint8_t* packed, uint32_t n, uint32_t dim, uint32_t b
 
 // ------------------------------------------------------------------ launches
 
-
-
 // A CTA per panel and group (at most 2^25 panels).
 dim3 grid_of(uint32_t n, const Fp4Layout& Lo) { return dim3(fp4_panels(n), std::min(Lo.groups, 65535u)); }
 

@@ -751,7 +751,8 @@ __global__ void __launch_bounds__(threads_of(ctas_of(MODE)), 1) fp4_product_kern
 
 template <typename T, uint32_t BLOCK, uint32_t MODE>
 gf_status launch_product(const ProdArgs& A, uint32_t grid, uint32_t smem, cudaStream_t s) {
-    GF_CUDA(cudaFuncSetAttribute(fp4_product_kernel<T, BLOCK, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // (the limit, not this call's size: calls of other sizes may be on their way in other threads)
+    GF_CUDA(cudaFuncSetAttribute(fp4_product_kernel<T, BLOCK, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimit));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(threads_of(ctas_of(MODE)));

@@ -234,3 +234,12 @@ def test_raw_product_refusals(args, word):
     assert L.gf_product_fp4_raw(P(a["q"]), a["q_dtype"], a["q_ld"], a["m"], a["q_alpha"], P(64), 5, a["dim"], 32, 1.0, P(64), 0, 5,
                                 P(a["workspace"]), 0, None) == 1
     assert word in L.gf_last_error()
+
+
+def test_product_scale_range():
+    for qa, ra in [(1.0, 1.0), (2.0 ** -64, 2.0 ** -63), (2.0 ** 63, 2.0 ** 63), (0.7, 3.0)]:
+        got = np.float32(gf._fp4_scale(qa, ra, "product"))
+        assert abs(float(got) * qa * ra - 1) <= 2.0 ** -24  # a normal float, rounded once
+    for qa, ra in [(2.0 ** -64, 2.0 ** -64), (2.0 ** 64, 2.0 ** 63), (0.0, 1.0), (-1.0, 1.0), (float("nan"), 1.0), (float("inf"), 1.0)]:
+        with pytest.raises(gf.GarfieldError):
+            gf._fp4_scale(qa, ra, "product")

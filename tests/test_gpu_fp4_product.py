@@ -255,6 +255,77 @@ def test_streams_and_graphs():
         assert torch.equal(o, -w)
 
 
+def test_calls_from_several_threads():
+    """Calls of one kernel that need different amounts of shared memory, each thread on its own stream."""
+    from concurrent.futures import ThreadPoolExecutor
+    shapes = [(20, 3000, 96), (20, 700, 2048), (60, 500, 300), (3, 1000, 96), (16, 1000, 1500)]
+    sets = []
+    for m, n, dim in shapes:
+        q, r = exact_rows(m, dim, 32, m + dim), exact_rows(n, dim, 32, n + dim)
+        sets.append((q, gf.quantize_fp4(r), q.double() @ r.double().t()))
+    torch.cuda.synchronize()
+
+    def work(k):
+        stream = torch.cuda.Stream()
+        wrong = 0
+        for i in range(60):
+            q, rows, want = sets[(i + k) % len(sets)]
+            out = gf.product_fp4(q, rows, stream=stream)
+            stream.synchronize()
+            wrong += not torch.equal(out.double(), want)
+        return wrong
+
+    with ThreadPoolExecutor(4) as pool:
+        assert list(pool.map(work, range(4))) == [0] * 4
+
+
+def test_captured_pipeline():
+    """Quantising, scoring (with and without a workspace) and reading back captured together, behind a copy and
+    beside work on a second stream; two such graphs replayed at once."""
+    def capture(x, y, q):
+        g, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(g):
+            y.copy_(x)
+            rows = gf.quantize_fp4(y, 1.0, 16)
+            side.wait_stream(torch.cuda.current_stream())
+            few = gf.product_fp4(q[:4], rows, stream=side)
+            many = gf.product_fp4(q, rows)
+            torch.cuda.current_stream().wait_stream(side)
+            back = gf.dequantize_fp4(rows)
+            again = gf.product_fp4(gf.quantize_fp4(back, 1.0, 16), rows)
+        return g, few, many, back, again
+
+    xs = [exact_rows(700, 300, 16, 5), exact_rows(900, 300, 16, 6)]
+    q = exact_rows(40, 300, 16, 7)
+    made = [capture(x, torch.empty_like(x), q) for x in xs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for sign in (-1.0, -1.0):
+        for x in xs:
+            x.mul_(sign)
+        torch.cuda.synchronize()
+        for s, (g, *_) in zip(streams, made):
+            with torch.cuda.stream(s):
+                for _ in range(3):
+                    g.replay()
+        torch.cuda.synchronize()
+        for x, (_, few, many, back, again) in zip(xs, made):
+            want = q.double() @ x.double().t()
+            assert torch.equal(few.double(), want[:4]) and torch.equal(many.double(), want)
+            assert torch.equal(back, x) and torch.equal(again.double(), x.double() @ x.double().t())
+
+
+def test_alphas_without_a_scale():
+    """Alphas whose product's inverse fp32 does not hold as a normal number are refused."""
+    r = gf.quantize_fp4(torch.full((20, 64), 2.0 ** -20, device="cuda"), 2.0 ** 64)
+    q = torch.ones(3, 64, device="cuda")
+    for bad in (2.0 ** 63, 0.0, -1.0, float("nan")):
+        with pytest.raises(gf.GarfieldError):
+            gf.product_fp4(q, r, query_alpha=bad)
+    with pytest.raises(gf.GarfieldError):
+        gf.product_fp4(r, r)
+    assert (gf.product_fp4(q, r, query_alpha=2.0 ** 62) == 2.0 ** -14).all()
+
+
 def test_store_score_read_together():
     """A collection held in 4 bits, scored for candidates, read back and re-ranked by the held values."""
     x = torch.from_numpy(data(5000, 96, 11, "normal")).cuda()
