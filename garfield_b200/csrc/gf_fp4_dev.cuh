@@ -73,19 +73,19 @@ __device__ __forceinline__ float amax3(float a, float b, float c) {
 __device__ __forceinline__ float amax8(const float* x) {
     return amax2(amax3(amax3(x[0], x[1], x[2]), x[6], x[7]), amax3(x[3], x[4], x[5]));
 }
-// 1 / s correctly rounded for the finite E4M3 values s > 0: one Newton step on the hardware's approximation
-// (a test compares all of them with the division).
-__device__ __forceinline__ float rcp_e4m3(float s) {
+// A quotient by a number y is held as x hi + x lo, hi + lo being 1 / y within 2^-41 of it and lo >= 0 (so that -0
+// stays -0).  Where x / y is a boundary between codes the sum rounds to it.  Where it is not, it is more than half
+// a last place away from it, by 1/32 of one at least (y and a boundary have few bits), which is far more than
+// this sum errs by before it is rounded.  (Results too small for that are far below the first boundary.)
+__device__ __forceinline__ float times(float x, float hi, float lo) { return __fmaf_rn(x, hi, __fmul_rn(x, lo)); }
+// hi and lo for the finite E4M3 values s > 0: the hardware's approximation, which errs by a last place, taken four
+// down, and what is missing.
+__device__ __forceinline__ float rcp_e4m3(float s, float& lo) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
-    return __fmaf_rn(r, __fmaf_rn(-s, r, 1.0f), r);
-}
-// x / y correctly rounded, for r = 1 / y correctly rounded and results that are normal: one exact
-// remainder corrects the product (Markstein, IBM J. Res. Dev. 34, 1990).  Results too small for that are far
-// below the first code boundary.  (In this order of signs -0 / y stays -0.)
-__device__ __forceinline__ float div_by(float x, float y, float r) {
-    const float q = __fmul_rn(x, r);
-    return __fmaf_rn(-__fmaf_rn(q, y, -x), r, q);
+    r = __uint_as_float(__float_as_uint(r) - 4u);
+    lo = __fmul_rn(r, __fmaf_rn(-s, r, 1.0f));
+    return r;
 }
 
 // Whether multiplying by alpha can be left to the multiplication by the block's factor: scaling by a power
@@ -125,16 +125,15 @@ __device__ __forceinline__ uint32_t encode8(float* x, float amax, float alpha, u
             x[e + 1] = dev::hi2(y);
         }
     } else {
-        s8 = ef == 255u ? 0x7Fu
-                        : (uint32_t)__nv_cvt_float_to_fp8(div_by(amax, 6.0f, 1.0f / 6.0f), __NV_SATFINITE, __NV_E4M3);
-        // x f / s = x / (s / f) with f a power of two: 1 / f has the exponent 254 - that of f
-        const float sc = e4m3_to_f32(s8), r = __fmul_rn(rcp_e4m3(sc), f);
-        const float s = __fmul_rn(sc, __uint_as_float((254u << 23) - __float_as_uint(f)));
+        constexpr float kHi = 0x1.555554p-3f, kLo = (float)(1.0 / 6.0 - (double)kHi);
+        s8 = ef == 255u ? 0x7Fu : (uint32_t)__nv_cvt_float_to_fp8(times(amax, kHi, kLo), __NV_SATFINITE, __NV_E4M3);
+        float lo;
+        const float hi = __fmul_rn(rcp_e4m3(e4m3_to_f32(s8), lo), f);
+        lo = __fmul_rn(lo, f);
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {  // div_by, two at a time
-            const dev::f2x v = dev::pack2(x[e], x[e + 1]), q = dev::mul2(v, dev::pack2(r, r));
-            const dev::f2x nr = dev::fma2(q, dev::pack2(s, s), dev::pack2(-x[e], -x[e + 1]));
-            const dev::f2x y = dev::fma2(nr, dev::pack2(-r, -r), q);
+        for (int e = 0; e < 8; e += 2) {  // times, two at a time
+            const dev::f2x v = dev::pack2(x[e], x[e + 1]);
+            const dev::f2x y = dev::fma2(v, dev::pack2(hi, hi), dev::mul2(v, dev::pack2(lo, lo)));
             x[e] = dev::lo2(y);
             x[e + 1] = dev::hi2(y);
         }

@@ -89,7 +89,8 @@ def test_strided_rows(dtype, dim, offset, gap):
 
 
 def test_every_e4m3_scale():
-    """Blocks of 16 whose scale takes every E4M3 value, with elements on and next to every code border."""
+    """Blocks of 16 whose scale takes every E4M3 value, with elements on and next to every code border, and zeros of
+    either sign."""
     rows = []
     for s in e4m3_values()[1:]:
         b = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], np.float64)
@@ -100,6 +101,7 @@ def test_every_e4m3_scale():
                 y[1:8] = np.nextafter(y[1:8], np.float32(step * 1e9))
             y[8:] = -y[:8]
             rows.append(y)
+        rows.append(np.where(np.arange(16) == 3, x[0], np.copysign(np.zeros(16), np.arange(16) % 2 - 0.5)).astype(np.float32))
     x = np.stack(rows)
     same_bytes(gf.quantize_fp4(torch.from_numpy(x).cuda(), 1.0, 16), gf.quantize_fp4_host(x, 1.0, 16))
     same_bytes(gf.quantize_fp4(torch.from_numpy(x / 8).cuda(), 8.0, 16), gf.quantize_fp4_host(x, 1.0, 16))
