@@ -25,10 +25,12 @@
 // codes fill whole 32-byte sectors of the panel.  The reader's threads take what one store
 // holds (16 bytes, or 8, as the rows are aligned; else four elements), so a warp's stores leave no sector
 // half written.  A CTA is short (one group of a panel); six of them on an SM overlap their loads and arithmetic.
-// (2 rows in flight per thread and 6 CTAs: bf16 1M x 128 in 57 us, bf16 8192 x 8192 in blocks of 16 in
-// 38; 4 rows and the 4 CTAs that their registers allow: 61 and 40; 1 row and 8 CTAs: 65 and 41.)
-// Measured: fp32 1M x 128 6.8 TB/s of the two directions (with part in L2), bf16 5.7 TB/s in blocks of 32,
-// where instructions count as much as bytes, and 4.5 TB/s at 8192 x 8192 in blocks of 16, where they are the bound.
+// Rows in flight per thread: 16-bit data 2, with 6 CTAs on an SM (4 rows and the 4 CTAs that their registers
+// allow win and lose: bf16 1M x 128 57 us against 61, bf16 8192 x 8192 in blocks of 16 35 against 37, fp16 1M x 128
+// in blocks of 16 62 against 57; 1 row and 8 CTAs: 64, 39 and 66), fp32 4 (1M x 128: 83 us against 86, in blocks of
+// 16 84 against 92), but 2 where short rows leave a thread few (1M x 16: 18 us against 22, 1M x 33 36 against 37).
+// fp32 1M x 128 moves 7.0 TB/s both ways (part of it in L2); 16-bit data are bound by instructions as much
+// as by bytes: bf16 1M x 128 5.7 TB/s, 8192 x 8192 in blocks of 16 5.0.
 #include <algorithm>
 #include <type_traits>
 #include <cmath>
@@ -48,15 +50,14 @@ __device__ __forceinline__ uint32_t row_shift(uint32_t cols, uint32_t per) {
     return 31u - __clz(per) + (cols > 2 ? 2u : cols - 1u);
 }
 
-// One group of one panel.  W: bytes of a load, which rows are aligned to.
-template <typename T, uint32_t BLOCK, uint32_t W, bool FOLD>
-__global__ void __launch_bounds__(kThreads, 6) fp4_quantize_kernel(const T* __restrict__ data, uint64_t ld, uint32_t n,
-                                                                uint32_t dim, float alpha, uint8_t* __restrict__ packed,
-                                                                Fp4Layout Lo) {
+// One group of one panel.  W: bytes of a load, which rows are aligned to; kRows: rows in flight per thread.
+template <typename T, uint32_t BLOCK, uint32_t W, bool FOLD, uint32_t kRows>
+__global__ void __launch_bounds__(kThreads, kRows == 4 ? 4 : 6)
+    fp4_quantize_kernel(const T* __restrict__ data, uint64_t ld, uint32_t n, uint32_t dim, float alpha,
+                        uint8_t* __restrict__ packed, Fp4Layout Lo) {
     constexpr uint32_t kSb = kFp4Group / BLOCK * kFp4Rows;  // scale bytes of a group
     constexpr uint32_t kV = W / sizeof(T);                  // elements of a load
     constexpr uint32_t kBo = BLOCK / kOct;                  // threads of a block
-    constexpr uint32_t kRows = 2;                           // rows in flight per thread: at most 64 * 2 per step
     constexpr uint32_t kB = kFp4Group / BLOCK;              // blocks of a row's group
     __shared__ __align__(16) uint8_t scales_s[kSb];         // [row][block]
     const uint32_t p = blockIdx.x;
@@ -93,14 +94,17 @@ __global__ void __launch_bounds__(kThreads, 6) fp4_quantize_kernel(const T* __re
         if (valid == kFp4Rows && dim % kV == 0) {  // a load's elements all exist or none does, the same in every row
             for (uint32_t r0 = 0; r0 < kFp4Rows; r0 += rstep * kRows) {
                 Oct q[kRows] = {};
+                // (short rows step by up to half a panel, of which two fit)
+                auto there = [&](uint32_t u) { return u < 2 || r0 + u * rstep < kFp4Rows; };
 #pragma unroll
                 for (uint32_t u = 0; u < kRows; ++u)
 #pragma unroll
                     for (uint32_t w = 0; w < kOct / kV; ++w)
-                        if (left > w * kV) q[u][w] = *reinterpret_cast<const Vec<T, W>*>(src + u * step + w * kV);
+                        if (there(u) && left > w * kV) q[u][w] = *reinterpret_cast<const Vec<T, W>*>(src + u * step + w * kV);
                 src += step * kRows;
 #pragma unroll
-                for (uint32_t u = 0; u < kRows; ++u) encode(q[u], r0 + first + u * rstep, o < 4 * cols);
+                for (uint32_t u = 0; u < kRows; ++u)
+                    if (there(u)) encode(q[u], r0 + first + u * rstep, o < 4 * cols);
             }
         } else {
             for (uint32_t r0 = 0; r0 < valid; r0 += rstep, src += step) {
@@ -300,13 +304,19 @@ gf_status launch_quantize(const void* data, uint64_t ld, uint32_t n, uint32_t di
     const Fp4Layout Lo = fp4_layout(n, dim, BLOCK);
     const T* x = static_cast<const T*>(data);
     const uint32_t w = row_alignment(data, ld, sizeof(T));
-    auto pick = [&](auto fold) {
+    auto pick = [&](auto fold, auto rows) {
         constexpr bool F = decltype(fold)::value;
-        return w == 16 ? fp4_quantize_kernel<T, BLOCK, 16, F>
-               : w == 8 ? fp4_quantize_kernel<T, BLOCK, 8, F>
-                        : fp4_quantize_kernel<T, BLOCK, sizeof(T), F>;
+        constexpr uint32_t R = decltype(rows)::value;
+        return w == 16 ? fp4_quantize_kernel<T, BLOCK, 16, F, R>
+               : w == 8 ? fp4_quantize_kernel<T, BLOCK, 8, F, R>
+                        : fp4_quantize_kernel<T, BLOCK, sizeof(T), F, R>;
     };
-    auto* k = fold_alpha(alpha, BLOCK) ? pick(std::true_type{}) : pick(std::false_type{});
+    auto pick_rows = [&](auto fold) {
+        if constexpr (sizeof(T) == 4)
+            if (dim > 2 * kFp4Col) return pick(fold, std::integral_constant<uint32_t, 4>{});
+        return pick(fold, std::integral_constant<uint32_t, 2>{});
+    };
+    auto* k = fold_alpha(alpha, BLOCK) ? pick_rows(std::true_type{}) : pick_rows(std::false_type{});
     return launch(k, grid_of(n, Lo), s, x, ld, n, dim, alpha, packed, Lo);
 }
 template <typename T, uint32_t BLOCK>
