@@ -26,7 +26,10 @@
 // cycles a stage whatever it holds (waiting, committing, the first instruction's way), while a group's
 // MMAs take 128 cycles at N = 128 and its panel's bytes 200 at the HBM rate.
 //
-// Every wait is bounded.  When one runs out the CTA stops and the outputs it still owes become NaN.
+// Every wait on a barrier in shared memory is bounded.  When one runs out the CTA stops and the outputs it still
+// owes become NaN.  The waits for TMEM, for the kernel before and at cluster barriers have no bound of their own:
+// the SM's holder of TMEM and the kernel before run to their ends without this CTA, and every CTA of a cluster
+// reaches every one of its barriers.
 #include <algorithm>
 #include <cmath>
 
@@ -85,7 +88,8 @@ struct ProdArgs {
     uint64_t ld;
     float scale;
     uint32_t torn;                      // 1: store16_torn, with the groups' buffers at torn_off
-    uint32_t dim, bar_off, torn_off, polls, extra_tx;
+    uint32_t dim, bar_off, torn_off, polls;
+    uint32_t hold;                      // test hook: 1 keeps every stage from being reported full until its CTA has given up
 };
 
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -229,6 +233,12 @@ __device__ __forceinline__ bool bwait(uint64_t* bar, uint32_t par, const volatil
         if (*stop) return false;
     }
     return false;
+}
+
+// Wait for asynchronous work that is under way (copies, MMAs), before the CTA gives up what it uses.
+__device__ __forceinline__ void land(uint64_t* bar, uint32_t par) {
+    for (uint32_t p = 0; p < kPolls && !mbar_try(bar, par); ++p) {
+    }
 }
 
 // Position in a ring of barriers: slot and the parity of its current use.
@@ -421,7 +431,7 @@ __global__ void __launch_bounds__(threads_of(ctas_of(MODE)), 1) fp4_product_kern
     if (warp == 0) tmem_alloc<CTAS>(tmem_slot);
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kMaxStages; ++i) {
-            mbar_init(&full[i], 1);
+            mbar_init(&full[i], 1 + A.hold);
             mbar_init(&pfull[i], 1);
             mbar_init(&empty[i], 1);
         }
@@ -470,7 +480,7 @@ __global__ void __launch_bounds__(threads_of(ctas_of(MODE)), 1) fp4_product_kern
                 const uint32_t nq = MODE == kFew ? 0u : min(CTAS, A.qpanels - t.q * CTAS);
                 const uint32_t b_bytes = MODE == kFew ? 0u : nq * as + (qp < A.qpanels ? bc + z : 0u);
                 if (elect_one()) {
-                    mbar_arrive_expect_tx(bar, a_bytes + b_bytes + A.extra_tx);
+                    mbar_arrive_expect_tx(bar, a_bytes + b_bytes);
                     if (A.pb > 1) {  // whole panels
                         bulk_g2s(stg, A.r + A.Lr.scales_at(p0, 0), a_bytes, bar);
                     } else if (np) {
@@ -491,17 +501,17 @@ __global__ void __launch_bounds__(threads_of(ctas_of(MODE)), 1) fp4_product_kern
             }
         }
         if (!ok) *stop = 1u;
-        // every copy issued lands before the CTA exits (in normal operation they completed long ago)
+        // Every copy issued lands before the CTA exits (in normal operation they completed long ago), whatever
+        // A.polls is.  With A.hold no stage was emptied, so each was filled once at most; what kept it from being
+        // full arrives once the MMA warp (of a pair, CTA 0's) has given up.
         if (lane == 0) {
+            if (A.hold) land(drain, 0);
             for (uint32_t st = 0; st < A.stages && st < filled; ++st) {
                 const uint32_t use = (uint32_t)((filled - 1 - st) / A.stages);  // the slot's last
-                uint32_t p = 0;
-                while (!mbar_try(&full[st], use & 1u) && ++p < A.polls) {
-                }
+                if (A.hold) mbar_arrive(&full[st]);
+                land(&full[st], use & 1u);
             }
-            uint32_t p = 0;
-            while (MODE == kFew && !A.raw && !mbar_try(qfull, 0) && ++p < A.polls) {
-            }
+            if (MODE == kFew && !A.raw) land(qfull, 0);
         }
         __syncwarp();
     } else if (warp == 1 && rank != 0) {
@@ -516,9 +526,7 @@ __global__ void __launch_bounds__(threads_of(ctas_of(MODE)), 1) fp4_product_kern
             }
         if (!ok) *stop = 1u;
         // CTA 0's last commit, which follows all its others, has arrived here before this CTA can exit
-        uint32_t p = 0;
-        while (!mbar_try(drain, 0) && ++p < A.polls) {
-        }
+        land(drain, 0);
         __syncwarp();
     } else if (warp == 1) {
         // -------------------------------------------------------------- MMA warp
@@ -615,9 +623,7 @@ __global__ void __launch_bounds__(threads_of(ctas_of(MODE)), 1) fp4_product_kern
         // every MMA has completed before TMEM is released
         if (elect_one()) mma_commit<CTAS>(drain);
         __syncwarp();
-        uint32_t p = 0;
-        while (!mbar_try(drain, 0) && ++p < A.polls) {
-        }
+        land(drain, 0);
         __syncwarp();
     } else {
         // -------------------------------------------------------------- epilogue warps
@@ -790,7 +796,7 @@ gf_status product(ProdArgs A, const void* q, uint32_t m, const void* r, uint32_t
     A.ld = ld;
     A.scale = scale;
     A.polls = test_wait ? test_wait : kPolls;
-    A.extra_tx = test_wait ? 16u : 0u;
+    A.hold = test_wait ? 1u : 0u;
     const uint32_t sub = block == 16 ? 2 : 1, scales = sub * kFp4ScaleSub, group = scales + 4 * kFp4ColBytes, G = A.Lr.groups;
     // Pairs of CTAs once their tiles, of 256 x 256, occupy every SM, where the rows are long enough for
     // their arithmetic to show (8192 x 16384 in bf16: 96 us against 78 at 512 elements, 86 against 97 at 768,

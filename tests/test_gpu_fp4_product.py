@@ -350,3 +350,17 @@ def test_waits_that_run_out(m, n, dim):
     got = gf.product_fp4(q, rows, test_wait=4)
     assert torch.isnan(got).all()
     assert torch.equal(gf.product_fp4(q, rows).double(), q.double() @ r.double().t())
+
+
+@pytest.mark.parametrize("m,n,dim", [(300, 19000, 1100), (40, 40000, 1024), (128, 130, 8192), (20, 1000, 300), (40, 90_000, 64)])
+def test_copies_land_when_waits_run_out_at_once(m, n, dim):
+    """Waits of a single poll give up with copies in flight into every SM's shared memory (pairs, rings, shares of a
+    tile, resident queries, several panels to a tile); calls that follow at once use the same shared memory."""
+    q, r = exact_rows(m, dim, 16, 1), exact_rows(n, dim, 16, 2)
+    rows, queries = gf.quantize_fp4(r, 1.0, 16), gf.quantize_fp4(q, 1.0, 16)
+    want = (q.double() @ r.double().t()).float()
+    for _ in range(5):
+        bad = gf.product_fp4(queries, rows, test_wait=1)
+        got = [gf.product_fp4(queries, rows) for _ in range(3)]
+        assert torch.isnan(bad).all()
+        assert all(torch.equal(g, want) for g in got)
