@@ -51,7 +51,7 @@ constexpr uint32_t threads_of(uint32_t ctas) { return 64 + 128 * epi_groups(ctas
 constexpr uint32_t kMaxStages = 8;
 constexpr uint32_t kMaxAcc = 8;
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kPolls = 1u << 20;
+constexpr uint32_t kPolls = 1u << 20;           // of 3.9 us each
 constexpr uint64_t kBandBytes = 64u << 20;  // of row panels, half of L2
 constexpr uint32_t kSmemLimit = 227 * 1024;
 
@@ -879,11 +879,12 @@ gf_status product(ProdArgs A, const void* q, uint32_t m, const void* r, uint32_t
 }
 
 gf_status check_product(uint32_t m, const void* r_packed, uint32_t n, uint32_t dim, uint32_t block, float scale, const void* out,
-                        uint32_t dtype, uint64_t ld) {
+                        uint32_t dtype, uint64_t ld, uint32_t test_wait) {
     if (!fp4_shape(dim, block)) return fail(GF_ERR_ARG, "dim must be positive and block 16 or 32");
     if (!dtype_bytes(dtype)) return fail(GF_ERR_ARG, "unknown dtype");
     if (!std::isfinite(scale)) return fail(GF_ERR_ARG, "scale must be finite");
     if (ld < n) return fail(GF_ERR_ARG, "row stride below n");
+    if (test_wait > kPolls) return fail(GF_ERR_ARG, "test_wait above 2^20");  // (it would hold the GPU for hours)
     if (m == 0 || n == 0) return GF_OK;
     if (!r_packed || !out) return fail(GF_ERR_ARG, "null argument");
     if (!aligned(r_packed, 16) || !aligned(out, dtype_bytes(dtype))) return fail(GF_ERR_ARG, "misaligned pointer");
@@ -898,7 +899,7 @@ using namespace gf;
 extern "C" gf_status gf_product_fp4(const void* q_packed, uint32_t m, const void* r_packed, uint32_t n, uint32_t dim,
                                     uint32_t block, float scale, void* out, uint32_t dtype, uint64_t ld, uint32_t test_wait,
                                     void* stream) {
-    const gf_status st = check_product(m, r_packed, n, dim, block, scale, out, dtype, ld);
+    const gf_status st = check_product(m, r_packed, n, dim, block, scale, out, dtype, ld, test_wait);
     if (st != GF_OK || m == 0 || n == 0) return st;
     if (!q_packed) return fail(GF_ERR_ARG, "null argument");
     if (!aligned(q_packed, 16)) return fail(GF_ERR_ARG, "misaligned pointer");
@@ -908,7 +909,7 @@ extern "C" gf_status gf_product_fp4(const void* q_packed, uint32_t m, const void
 extern "C" gf_status gf_product_fp4_raw(const void* q, uint32_t q_dtype, uint64_t q_ld, uint32_t m, float q_alpha,
                                         const void* r_packed, uint32_t n, uint32_t dim, uint32_t block, float scale, void* out,
                                         uint32_t dtype, uint64_t ld, void* workspace, uint32_t test_wait, void* stream) {
-    const gf_status st = check_product(m, r_packed, n, dim, block, scale, out, dtype, ld);
+    const gf_status st = check_product(m, r_packed, n, dim, block, scale, out, dtype, ld, test_wait);
     if (st != GF_OK) return st;
     if (!dtype_bytes(q_dtype)) return fail(GF_ERR_ARG, "unknown dtype");
     if (!fp4_alpha(q_alpha)) return fail(GF_ERR_ARG, "alpha must lie in [2^-126, 2^126]");

@@ -499,8 +499,9 @@ gf_status gf_dequantize_fp4_host(const void* packed, uint32_t n, uint32_t dim, u
  * on 32-byte boundaries (out and ld) are written faster, by up to a half where out is far larger than L2.
  * Whichever of the two has more rows is best passed as r.
  * test_wait: 0 in normal use.  Test hook for the timeout path: the kernel's waits give up after
- * test_wait polls and no stage of rows is ever reported to be in place, so all of out becomes NaN.  Copies
- * under way are waited for as long as in normal use.
+ * test_wait polls (at most 2^20, which waits in normal use have: some four seconds) and no stage of rows is
+ * ever reported to be in place, so all of out becomes NaN.  Copies under way are waited for as long as in
+ * normal use.
  * gf_product_fp4_raw takes the queries as they are (q_dtype, rows q_ld elements apart) and holds them in 4
  * bits, with q_alpha and the rows' block, for the call.  workspace (device, 16-byte aligned, of
  * gf_fp4_bytes(m, dim, block) bytes) receives them; it may be NULL when m <= 16, dim <= 8192 and

@@ -243,3 +243,13 @@ def test_product_scale_range():
     for qa, ra in [(2.0 ** -64, 2.0 ** -64), (2.0 ** 64, 2.0 ** 63), (0.0, 1.0), (-1.0, 1.0), (float("nan"), 1.0), (float("inf"), 1.0)]:
         with pytest.raises(gf.GarfieldError):
             gf._fp4_scale(qa, ra, "product")
+
+
+@pytest.mark.parametrize("test_wait", [2 ** 20 + 1, 2 ** 32 - 1])
+def test_long_test_waits_are_refused(test_wait):
+    """Waits that cannot succeed are bounded by those of normal use."""
+    L, P = gf.lib(), ctypes.c_void_p
+    assert L.gf_product_fp4(P(64), 3, P(64), 5, 8, 32, 1.0, P(64), 0, 5, test_wait, None) == 1
+    assert b"test_wait" in L.gf_last_error()
+    assert L.gf_product_fp4_raw(P(64), 0, 8, 3, 1.0, P(64), 5, 8, 32, 1.0, P(64), 0, 5, None, test_wait, None) == 1
+    assert b"test_wait" in L.gf_last_error()
