@@ -640,12 +640,15 @@ class _on_stream:
         self.device.__exit__(*exc)
 
 
-def _fp4_run(device, stream, f, *args):
+def _fp4_run(what, device, stream, f, *args):
     """f(raw stream, *args) with the device and the stream current.  The usual case, the current stream
     of the current device, reads torch's raw handle: entering contexts costs more than a small call."""
     import torch
     if stream is None and device.index == torch._C._cuda_getDevice():
         return f(torch._C._cuda_getCurrentRawStream(device.index), *args)
+    other = getattr(stream, "device", device)
+    if isinstance(other, torch.device) and other != device:
+        raise GarfieldError(1, what, f"a stream of {other}, data on {device}")
     with _on_stream(device, stream) as s:
         return f(s, *args)
 
@@ -668,7 +671,7 @@ def quantize_fp4(data, alpha: float = 1.0, block: int = 32, stream=None) -> Fp4R
     """gf_quantize_fp4: the rows of a float32, float16 or bfloat16 CUDA matrix, held in 4 bits."""
     if not getattr(data, "is_cuda", False):
         raise GarfieldError(1, "gf_quantize_fp4", "data: expected a 2-D CUDA tensor")
-    return _fp4_run(data.device, stream, _fp4_quantize, data, alpha, block)
+    return _fp4_run("gf_quantize_fp4", data.device, stream, _fp4_quantize, data, alpha, block)
 
 
 def _fp4_out(out, m: int, n: int, dtype, device, what: str):
@@ -697,7 +700,7 @@ def dequantize_fp4(rows: Fp4Rows, dtype=None, out=None, stream=None):
     import torch
     p = _fp4_rows(rows, "gf_dequantize_fp4")
     dtype = dtype or (out.dtype if out is not None else torch.float32)
-    return _fp4_run(p.device, stream, _fp4_dequantize, p, rows, dtype, out)
+    return _fp4_run("gf_dequantize_fp4", p.device, stream, _fp4_dequantize, p, rows, dtype, out)
 
 
 def _fp4_scale(query_alpha: float, alpha: float, what: str) -> float:
@@ -753,7 +756,7 @@ def product_fp4(queries, rows: Fp4Rows, dtype=None, out=None, query_alpha: float
     if not isinstance(queries, Fp4Rows) and not getattr(queries, "is_cuda", False):
         raise GarfieldError(1, "gf_product_fp4", "queries: expected Fp4Rows or a 2-D CUDA tensor")
     dtype = dtype or (out.dtype if out is not None else torch.float32)
-    return _fp4_run(p.device, stream, _fp4_product, queries, p, rows, dtype, out, query_alpha, test_wait)
+    return _fp4_run("gf_product_fp4", p.device, stream, _fp4_product, queries, p, rows, dtype, out, query_alpha, test_wait)
 
 
 def quantize_fp4_host(data: np.ndarray, alpha: float = 1.0, block: int = 32) -> Fp4Rows:

@@ -253,3 +253,14 @@ def test_long_test_waits_are_refused(test_wait):
     assert b"test_wait" in L.gf_last_error()
     assert L.gf_product_fp4_raw(P(64), 0, 8, 3, 1.0, P(64), 5, 8, 32, 1.0, P(64), 0, 5, None, test_wait, None) == 1
     assert b"test_wait" in L.gf_last_error()
+
+
+def test_streams_of_other_devices_are_refused():
+    """A kernel on another device's stream would follow this device's pointers there."""
+    import torch
+
+    class Stream:
+        device, cuda_stream = torch.device("cuda", 1), 64
+
+    with pytest.raises(gf.GarfieldError, match="gf_product_fp4.*cuda:1.*cuda:0"):
+        gf._fp4_run("gf_product_fp4", torch.device("cuda", 0), Stream(), pytest.fail)

@@ -182,3 +182,15 @@ def test_streams_and_graph():
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, gf.dequantize_fp4(gf.quantize_fp4(x)))
+
+
+def test_stream_of_another_device_is_refused():
+    class Stream:
+        device, cuda_stream = torch.device("cuda", 1), 64
+
+    x = torch.ones(20, 64, device="cuda:0")
+    r = gf.quantize_fp4(x)
+    for call in (lambda: gf.quantize_fp4(x, stream=Stream()), lambda: gf.dequantize_fp4(r, stream=Stream()),
+                 lambda: gf.product_fp4(x, r, stream=Stream())):
+        with pytest.raises(gf.GarfieldError, match="cuda:1"):
+            call()
