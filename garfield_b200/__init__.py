@@ -642,15 +642,25 @@ class _on_stream:
 
 def _fp4_run(what, device, stream, f, *args):
     """f(raw stream, *args) with the device and the stream current.  The usual case, the current stream
-    of the current device, reads torch's raw handle: entering contexts costs more than a small call."""
+    of the current device, reads torch's raw handle: entering contexts costs more than a small call.
+    On another stream than the current one, the allocator is told that the call's tensors are used there,
+    and its result here: either may be dropped while the other stream has still to read it."""
     import torch
     if stream is None and device.index == torch._C._cuda_getDevice():
         return f(torch._C._cuda_getCurrentRawStream(device.index), *args)
     other = getattr(stream, "device", device)
     if isinstance(other, torch.device) and other != device:
         raise GarfieldError(1, what, f"a stream of {other}, data on {device}")
-    with _on_stream(device, stream) as s:
-        return f(s, *args)
+    here, on = torch.cuda.current_stream(device), _on_stream(device, stream)
+    with on as s:
+        result = f(s, *args)
+    if on.stream.cuda_stream != here.cuda_stream:
+        for t in args:
+            t = t.packed if isinstance(t, Fp4Rows) else t
+            if isinstance(t, torch.Tensor):
+                t.record_stream(on.stream)
+        (result.packed if isinstance(result, Fp4Rows) else result).record_stream(here)
+    return result
 
 
 def _fp4_quantize(s, data, alpha, block):
@@ -668,7 +678,10 @@ def _fp4_quantize(s, data, alpha, block):
 
 
 def quantize_fp4(data, alpha: float = 1.0, block: int = 32, stream=None) -> Fp4Rows:
-    """gf_quantize_fp4: the rows of a float32, float16 or bfloat16 CUDA matrix, held in 4 bits."""
+    """gf_quantize_fp4: the rows of a float32, float16 or bfloat16 CUDA matrix, held in 4 bits.
+    stream: where the kernels run (None: the current stream).  As with torch's own streams, the caller orders
+    another stream after the work that makes the inputs and before the work that reads the result; the
+    tensors need not be kept meanwhile."""
     if not getattr(data, "is_cuda", False):
         raise GarfieldError(1, "gf_quantize_fp4", "data: expected a 2-D CUDA tensor")
     return _fp4_run("gf_quantize_fp4", data.device, stream, _fp4_quantize, data, alpha, block)
@@ -696,7 +709,7 @@ def _fp4_dequantize(s, p, rows, dtype, out):
 
 def dequantize_fp4(rows: Fp4Rows, dtype=None, out=None, stream=None):
     """gf_dequantize_fp4: the values that rows are held as (n x dim, float32 unless dtype or out say
-    otherwise)."""
+    otherwise).  out does not overlap rows; stream is as in quantize_fp4."""
     import torch
     p = _fp4_rows(rows, "gf_dequantize_fp4")
     dtype = dtype or (out.dtype if out is not None else torch.float32)
@@ -750,7 +763,8 @@ def product_fp4(queries, rows: Fp4Rows, dtype=None, out=None, query_alpha: float
     """gf_product_fp4: the inner products of every query with every row (m x n, float32 unless dtype or
     out say otherwise).  queries: Fp4Rows of the same dim and block, or a float32, float16 or
     bfloat16 CUDA matrix, which is held in 4 bits (quantize_fp4 with query_alpha and the rows'
-    block) for the call (gf_product_fp4_raw).  The product of both alphas lies in [2^-127, 2^126]."""
+    block) for the call (gf_product_fp4_raw).  The product of both alphas lies in [2^-127, 2^126].
+    out overlaps neither input; stream is as in quantize_fp4; test_wait is a test hook (0 in normal use)."""
     import torch
     p = _fp4_rows(rows, "gf_product_fp4")
     if not isinstance(queries, Fp4Rows) and not getattr(queries, "is_cuda", False):

@@ -2,6 +2,8 @@
 read back against the definition in 64 bits, strides, alignments, streams and graphs."""
 from __future__ import annotations
 
+import weakref
+
 import numpy as np
 import pytest
 
@@ -194,3 +196,59 @@ def test_stream_of_another_device_is_refused():
                  lambda: gf.product_fp4(x, r, stream=Stream())):
         with pytest.raises(gf.GarfieldError, match="cuda:1"):
             call()
+
+
+def test_inputs_dropped_while_a_stream_has_to_read_them():
+    """Packed rows and queries that only the call held, and memory that is handed out and written again at once."""
+    x, q = torch.from_numpy(data(3000, 256, 8, "normal")).cuda(), torch.from_numpy(data(40, 256, 9, "normal")).cuda()
+    want = gf.product_fp4(q, gf.quantize_fp4(x))
+    back = gf.dequantize_fp4(gf.quantize_fp4(x))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def late(call, *make):
+        """call's result, on a stream that is held up until the memory of what `make` makes could have been
+        written again."""
+        made = [m() for m in make]
+        alive = [weakref.ref(t) for t in made]
+        sizes = [(t.packed if isinstance(t, gf.Fp4Rows) else t) for t in made]
+        sizes = [(t.data_ptr(), t.numel(), t.dtype) for t in sizes]
+        room = [torch.empty(n, dtype=dt, device="cuda").fill_(1) for _, n, dt in sizes]
+        del room  # the allocator has room without asking the driver, and the kernels are loaded
+        side.wait_stream(torch.cuda.current_stream())
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(60_000_000)  # some 30 ms
+        result = call(*made)
+        del made
+        assert not any(r() is not None for r in alive)
+        new = [torch.empty(n, dtype=dt, device="cuda").fill_(3) for _, n, dt in sizes]
+        assert not side.query()
+        assert {t.data_ptr() for t in new}.isdisjoint(at for at, _, _ in sizes)
+        side.synchronize()
+        return result
+
+    assert torch.equal(late(lambda r, y: gf.product_fp4(y, r, stream=side), lambda: gf.quantize_fp4(x), q.clone), want)
+    assert torch.equal(late(lambda r: gf.dequantize_fp4(r, stream=side), lambda: gf.quantize_fp4(x)), back)
+    assert torch.equal(gf.dequantize_fp4(late(lambda y: gf.quantize_fp4(y, stream=side.cuda_stream), x.clone)), back)
+
+
+def test_results_dropped_while_the_current_stream_has_to_read_them():
+    """Rows made on a stream, read on the current one and dropped: the stream's next rows get other memory."""
+    x = torch.from_numpy(data(3000, 256, 8, "normal")).cuda()
+    y, want = -x, gf.dequantize_fp4(gf.quantize_fp4(x))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    rows = gf.quantize_fp4(x, stream=side)
+    at = rows.packed.data_ptr()
+    room = gf.quantize_fp4(x, stream=side)
+    del room  # the allocator has room on that stream without asking the driver
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(60_000_000)
+    got = gf.dequantize_fp4(rows)
+    del rows
+    again = gf.quantize_fp4(y, stream=side)
+    assert not torch.cuda.current_stream().query() and again.packed.data_ptr() != at
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(gf.dequantize_fp4(again), -want)
