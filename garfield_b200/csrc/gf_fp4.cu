@@ -44,6 +44,7 @@ namespace {
 using namespace fp4;
 
 constexpr uint32_t kThreads = 256;
+constexpr float kNormal = 0x1p-126f;  // the smallest normal fp32 number
 
 // Lanes of a row, as a power of two: enough for `cols` columns at `per` lanes each (per a power of two).
 __device__ __forceinline__ uint32_t row_shift(uint32_t cols, uint32_t per) {
@@ -133,8 +134,13 @@ __global__ void __launch_bounds__(kThreads, kRows == 4 ? 4 : 6)
 
 // The reverse.  W: bytes of a store.  inv is 1 / alpha rounded; the scale is multiplied by it once
 // per thread and the code times that rounded again: with a power of two as alpha all is exact in
-// fp32, otherwise a value is within 3 * 2^-24 of c * s / alpha.
-template <typename T, uint32_t BLOCK, uint32_t W>
+// fp32, otherwise a value is within 3 * 2^-24 of c * s / alpha.  Where s * inv is below fp32's normal numbers it
+// keeps fewer bits, or none while 6 s inv has some left: there c * s, which is exact, is multiplied by inv.  A
+// value below the normal numbers is off by another half of the smallest number at most, unless fp32 holds it.
+// SMALL: whether that can happen.  In blocks of 32 it can (1M x 96 to fp16 46.5 us without this, 44.4 with it, 1M x 33
+// 36.7 and 37.7, 1M x 128 to fp32 93.0 both; a branch takes 47.7 and 42.4); blocks of 16 have scales of 2^-9
+// and more, so only an alpha above 2^117 brings it about (1M x 128 to bf16 51.7 us without, 58.8 with it).
+template <typename T, uint32_t BLOCK, uint32_t W, bool SMALL>
 __global__ void __launch_bounds__(kThreads, 6) fp4_dequantize_kernel(const uint8_t* __restrict__ packed, uint32_t n,
                                                                   uint32_t dim, float inv, T* __restrict__ out,
                                                                   uint64_t ld, Fp4Layout Lo) {
@@ -161,13 +167,21 @@ __global__ void __launch_bounds__(kThreads, 6) fp4_dequantize_kernel(const uint8
                               : src[i * 16];
         };
         auto write = [&](uint32_t c, uint32_t s8, bool whole) {
-            const float s = __fmul_rn(scale_to_f32(s8, BLOCK == 16), inv);
+            const float held = scale_to_f32(s8, BLOCK == 16), both = __fmul_rn(held, inv);
+            const bool small = SMALL && both < kNormal;
+            const float s = small ? held : both, f = small ? inv : 1.0f;
             Vec<T, kV * sizeof(T)> y;
 #pragma unroll
             for (uint32_t e = 0; e < kV; e += 2) {
-                const float2 a = e2m1x2_to_f32((c >> (4 * e)) & 255u);
-                from_f32(__fmul_rn(a.x, s), y.v[e]);
-                from_f32(__fmul_rn(a.y, s), y.v[e + 1]);
+                const float2 v = e2m1x2_to_f32((c >> (4 * e)) & 255u);
+                if (SMALL) {  // two products of pairs, in place of a branch
+                    const dev::f2x x = dev::mul2(dev::mul2(dev::pack2(v.x, v.y), dev::pack2(s, s)), dev::pack2(f, f));
+                    from_f32(dev::lo2(x), y.v[e]);
+                    from_f32(dev::hi2(x), y.v[e + 1]);
+                } else {
+                    from_f32(__fmul_rn(v.x, s), y.v[e]);
+                    from_f32(__fmul_rn(v.y, s), y.v[e + 1]);
+                }
             }
             if (W > sizeof(T) && whole) {
                 *reinterpret_cast<decltype(y)*>(dst) = y;
@@ -270,8 +284,8 @@ void dequantize_host(const uint8_t* packed, uint32_t n, uint32_t dim, uint32_t b
             const uint32_t r = i % kFp4Rows, p = i / kFp4Rows;
             const uint32_t c = (packed[Lo.col_at(p, k / kFp4Col) + r * 16 + (k % kFp4Col) / 2] >> (4 * (k & 1u))) & 15u;
             const uint32_t s8 = packed[Lo.scales_at(p, k / kFp4Group) + fp4_scale_at(r, k % kFp4Group / block)];
-            const float s = scale_host(s8, block) * inv;
-            out[(uint64_t)i * dim + k] = (c & 8u ? -kMags[c & 7u] : kMags[c & 7u]) * s;
+            const float held = scale_host(s8, block), s = held * inv, v = c & 8u ? -kMags[c & 7u] : kMags[c & 7u];
+            out[(uint64_t)i * dim + k] = s < kNormal ? v * held * inv : v * s;
         }
 }
 
@@ -324,10 +338,17 @@ gf_status launch_dequantize(const uint8_t* packed, uint32_t n, uint32_t dim, flo
     const Fp4Layout Lo = fp4_layout(n, dim, BLOCK);
     T* y = static_cast<T*>(out);
     const uint32_t w = row_alignment(out, ld, sizeof(T));
-    auto* k = w == 16 ? fp4_dequantize_kernel<T, BLOCK, 16>
-              : w == 8 ? fp4_dequantize_kernel<T, BLOCK, 8>
-                       : fp4_dequantize_kernel<T, BLOCK, sizeof(T)>;
-    return launch(k, grid_of(n, Lo), s, packed, n, dim, 1.0f / alpha, y, ld, Lo);
+    const float inv = 1.0f / alpha;
+    auto pick = [&](auto small) {
+        constexpr bool S = decltype(small)::value;
+        return w == 16 ? fp4_dequantize_kernel<T, BLOCK, 16, S>
+               : w == 8 ? fp4_dequantize_kernel<T, BLOCK, 8, S>
+                        : fp4_dequantize_kernel<T, BLOCK, sizeof(T), S>;
+    };
+    auto* k = pick(std::true_type{});
+    if constexpr (BLOCK == 16)
+        if (inv >= 0x1p9f * kNormal) k = pick(std::false_type{});
+    return launch(k, grid_of(n, Lo), s, packed, n, dim, inv, y, ld, Lo);
 }
 
 }  // namespace

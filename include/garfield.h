@@ -479,8 +479,9 @@ typedef enum { GF_F32 = 0, GF_F16 = 1, GF_BF16 = 2 } gf_dtype;
  * ld is the distance between rows in elements, at least dim.  alpha lies in [2^-126, 2^126].
  * _host: host arrays, fp32 rows without gaps; gf_quantize_fp4_host writes the same bytes as
  * gf_quantize_fp4, and 0 in the rows that the last panel lacks.
- * gf_dequantize_fp4 multiplies each code with s * (1 / alpha), rounding to fp32 each time, and rounds to
- * dtype: exact in fp32 when alpha is a power of two, else within 3 * 2^-24 of the held value.
+ * gf_dequantize_fp4 multiplies each code with s * (1 / alpha), rounding to fp32 each time (where that is
+ * below 2^-126: code * s with 1 / alpha), and rounds to dtype.  In fp32 a held value is read back exactly when
+ * alpha is a power of two and fp32 has it, else within 3 * 2^-24 of it, and 2^-150 more below 2^-126.
  */
 uint64_t gf_fp4_bytes(uint32_t n, uint32_t dim, uint32_t block);
 gf_status gf_quantize_fp4(const void* data, uint32_t dtype, uint64_t ld, uint32_t n, uint32_t dim, float alpha,

@@ -264,3 +264,38 @@ def test_streams_of_other_devices_are_refused():
 
     with pytest.raises(gf.GarfieldError, match="gf_product_fp4.*cuda:1.*cuda:0"):
         gf._fp4_run("gf_product_fp4", torch.device("cuda", 0), Stream(), pytest.fail)
+
+
+def small_values(block, seed=1):
+    """fp32 data near its smallest number, in blocks whose codes and scales hold them exactly with a large enough alpha."""
+    rng = np.random.default_rng(seed)
+    n, nb = 150, 96 // block
+    e = rng.integers(-150, -120, (n, nb, 1))
+    x = np.ldexp(MAGS[rng.integers(0, 8, (n, nb, block))] * rng.choice([-1.0, 1.0], (n, nb, block)), e)
+    x[:, :, 0] = np.ldexp(6.0, e[:, :, 0])
+    x = np.where(x == np.ldexp(np.rint(np.ldexp(x, 149)), -149), x, 0.0)  # (no parts of fp32's smallest number)
+    return x.reshape(n, -1).astype(np.float32)
+
+
+@pytest.mark.parametrize("block,alpha", [(32, 2.0 ** 30), (32, 2.0 ** 60), (32, 2.0 ** 100), (32, 2.0 ** 126), (16, 2.0 ** 125),
+                                         (16, 2.0 ** 126), (32, 1.0), (32, 2.0)])
+def test_small_values_are_rounded_once(block, alpha):
+    """Scales whose quotient by a power of two is below fp32's normal numbers, or below all of them: what is read back
+    is the held value, rounded only where fp32 does not have it."""
+    x = small_values(block)
+    want = held(x, alpha, block)[2]
+    if block == 32 and alpha >= 2.0 ** 30:
+        assert np.array_equal(want, x.astype(np.float64))
+    assert np.array_equal(gf.dequantize_fp4_host(gf.quantize_fp4_host(x, alpha, block)), want.astype(np.float32))
+
+
+@pytest.mark.parametrize("alpha", [3e35, 1.7e20, 0.3, 5.0, 8e37])
+def test_small_values_read_back_within_the_bound(alpha):
+    """Other alphas: three roundings of 2^-24 of the value, and half of fp32's smallest number below the normal ones."""
+    rng = np.random.default_rng(3)
+    x = (rng.standard_normal((150, 96)) * 2.0 ** rng.integers(-145, -100, (150, 1))).astype(np.float32)
+    a32 = float(np.float32(alpha))
+    _, _, want = held(x, a32, 32)
+    got = gf.dequantize_fp4_host(gf.quantize_fp4_host(x, alpha, 32)).astype(np.float64)
+    tol = 3 * 2.0 ** -24 * (1 + 2.0 ** -22) * np.abs(want) + np.where(np.abs(want) < 2.0 ** -126, 2.0 ** -150, 0.0)
+    assert np.all(np.abs(got - want) <= tol)

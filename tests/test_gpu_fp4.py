@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 import garfield_b200 as gf
-from test_fp4 import data, e4m3_values, held
+from test_fp4 import data, e4m3_values, held, small_values
 
 pytestmark = pytest.mark.gpu
 
@@ -252,3 +252,18 @@ def test_results_dropped_while_the_current_stream_has_to_read_them():
     assert not torch.cuda.current_stream().query() and again.packed.data_ptr() != at
     torch.cuda.synchronize()
     assert torch.equal(got, want) and torch.equal(gf.dequantize_fp4(again), -want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("block,alpha", [(32, 1.0), (32, 2.0), (32, 2.0 ** 60), (32, 2.0 ** 126), (16, 2.0 ** 126), (32, 3e35), (32, 5.0),
+                                         (16, 8e37)])
+def test_small_values_as_on_the_host(block, alpha, dtype):
+    """Values below fp32's normal numbers, at each width of a store."""
+    x = small_values(block)
+    ref = gf.quantize_fp4_host(x, alpha, block)
+    want = torch.from_numpy(gf.dequantize_fp4_host(ref))
+    assert want.count_nonzero() > 4000
+    r = gf.Fp4Rows(gf.quantize_fp4(torch.from_numpy(x).cuda(), alpha, block).packed, *x.shape, block, alpha)
+    for pad in (0, 1, 4):
+        out = torch.empty(x.shape[0], x.shape[1] + pad, dtype=dtype, device="cuda")[:, :x.shape[1]]
+        assert torch.equal(gf.dequantize_fp4(r, out=out).cpu(), want.to(dtype))
