@@ -558,13 +558,16 @@ def quantize_i8(data, alpha: float = 1.0, stream=None):
 @dataclass
 class Fp4Rows:
     """n x dim rows held in 4 bits (the packed form that include/garfield.h describes): codes with one
-    scale per `block` elements of a row, standing for the data multiplied by alpha.  packed is a uint8
-    CUDA tensor, or a numpy array from quantize_fp4_host."""
+    scale per `block` elements of a row, standing for the data multiplied by alpha (an fp32 number: what is
+    given is rounded to one).  packed is a uint8 CUDA tensor, or a numpy array from quantize_fp4_host."""
     packed: object
     n: int
     dim: int
     block: int
     alpha: float
+
+    def __post_init__(self):
+        self.alpha = C.c_float(self.alpha).value
 
 
 def _fp4_need(ok: bool, what: str, msg: str) -> None:
@@ -674,7 +677,7 @@ def _fp4_quantize(s, data, alpha, block):
     st = lib().gf_quantize_fp4(data.data_ptr(), dt, ld, n, dim, alpha, block, packed.data_ptr(), s)
     if st:
         _check(st, what)
-    return Fp4Rows(packed, n, dim, block, float(alpha))
+    return Fp4Rows(packed, n, dim, block, alpha)
 
 
 def quantize_fp4(data, alpha: float = 1.0, block: int = 32, stream=None) -> Fp4Rows:
@@ -748,7 +751,7 @@ def _fp4_product(s, queries, p, rows, dtype, out, query_alpha, test_wait):
         if not (m <= 16 and dim <= 8192 and m * dim <= 32768):
             ws = torch.empty(_fp4_size(m, dim, block), dtype=torch.uint8, device=device)
         st = lib().gf_product_fp4_raw(qp.data_ptr(), qdt, qld, m, query_alpha, p.data_ptr(), rows.n, dim, block,
-                                      _fp4_scale(query_alpha, rows.alpha, what), out.data_ptr(), dt, ld,
+                                      _fp4_scale(C.c_float(query_alpha).value, rows.alpha, what), out.data_ptr(), dt, ld,
                                       None if ws is None else ws.data_ptr(), test_wait, s)
     else:
         st = lib().gf_product_fp4(qp.data_ptr(), m, p.data_ptr(), rows.n, dim, block,
@@ -780,7 +783,7 @@ def quantize_fp4_host(data: np.ndarray, alpha: float = 1.0, block: int = 32) -> 
     _fp4_need(dim > 0 and block in (16, 32), "gf_quantize_fp4_host", f"dim {dim}, block {block}")
     packed = np.empty(_fp4_size(n, dim, block), np.uint8)
     _check(lib().gf_quantize_fp4_host(_np_ptr(data), n, dim, alpha, block, _np_ptr(packed)), "gf_quantize_fp4_host")
-    return Fp4Rows(packed, n, dim, block, float(alpha))
+    return Fp4Rows(packed, n, dim, block, alpha)
 
 
 def dequantize_fp4_host(rows: Fp4Rows) -> np.ndarray:

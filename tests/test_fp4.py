@@ -299,3 +299,10 @@ def test_small_values_read_back_within_the_bound(alpha):
     got = gf.dequantize_fp4_host(gf.quantize_fp4_host(x, alpha, 32)).astype(np.float64)
     tol = 3 * 2.0 ** -24 * (1 + 2.0 ** -22) * np.abs(want) + np.where(np.abs(want) < 2.0 ** -126, 2.0 ** -150, 0.0)
     assert np.all(np.abs(got - want) <= tol)
+
+
+@pytest.mark.parametrize("alpha", [0.3, 1.0 + 1.9 * 2.0 ** -25, 1, 1e-30])
+def test_alpha_is_one_number(alpha):
+    """What the codec multiplied by is what the products are divided by: alpha in fp32."""
+    assert gf.quantize_fp4_host(np.ones((3, 8), np.float32), alpha).alpha == float(np.float32(alpha))
+    assert gf.Fp4Rows(None, 3, 8, 32, alpha).alpha == float(np.float32(alpha))

@@ -364,3 +364,15 @@ def test_copies_land_when_waits_run_out_at_once(m, n, dim):
         got = [gf.product_fp4(queries, rows) for _ in range(3)]
         assert torch.isnan(bad).all()
         assert all(torch.equal(g, want) for g in got)
+
+
+@pytest.mark.parametrize("m", [3, 40])
+def test_products_use_the_alphas_of_the_codec(m):
+    """An alpha that rounds to 1 in fp32 leaves the products of exactly held rows exact."""
+    alpha = 1.0 + 1.9 * 2.0 ** -25
+    q, r = exact_rows(m, 96, 16, 1), exact_rows(300, 96, 16, 2)
+    want = q.double() @ r.double().t()
+    rows = gf.quantize_fp4(r, alpha, 16)
+    assert torch.equal(gf.product_fp4(q, rows, query_alpha=alpha).double(), want)
+    assert torch.equal(gf.product_fp4(gf.quantize_fp4(q, alpha, 16), rows).double(), want)
+    assert torch.equal(gf.dequantize_fp4(rows), r)
