@@ -29,7 +29,8 @@ __all__ = [
     "GarfieldError", "lib", "lib_path", "SearchParams", "Index", "Plan", "NO_ID", "schedule_batches",
     "read_fvecs", "write_fvecs", "read_attrs", "write_attrs", "read_u32mat", "write_u32mat",
     "read_ranges", "write_ranges", "read_labels", "read_grid",
-    "Fp4Rows", "quantize_fp4", "dequantize_fp4", "product_fp4", "quantize_fp4_host", "dequantize_fp4_host",
+    "Fp4Rows", "quantize_fp4", "dequantize_fp4", "product_fp4", "product_fp4_timeouts", "quantize_fp4_host",
+    "dequantize_fp4_host",
 ]
 
 NO_ID = 0xFFFFFFFF
@@ -147,6 +148,7 @@ def lib() -> C.CDLL:
         "gf_product_fp4": (C.c_int, [_P, _U32, _P, _U32, _U32, _U32, C.c_float, _P, _U32, C.c_uint64, _U32, _P]),
         "gf_product_fp4_raw": (C.c_int, [_P, _U32, C.c_uint64, _U32, C.c_float, _P, _U32, _U32, _U32, C.c_float, _P, _U32,
                                          C.c_uint64, _P, _U32, _P]),
+        "gf_product_fp4_timeouts": (C.c_int, [_PTR(C.c_uint64)]),
         "gf_quantize_fp4_host": (C.c_int, [_P, _U32, _U32, C.c_float, _U32, _P]),
         "gf_dequantize_fp4_host": (C.c_int, [_P, _U32, _U32, _U32, C.c_float, _P]),
         "gf_write_attrs": (C.c_int, [C.c_char_p, _P, _U32, _U32]),
@@ -767,13 +769,25 @@ def product_fp4(queries, rows: Fp4Rows, dtype=None, out=None, query_alpha: float
     out say otherwise).  queries: Fp4Rows of the same dim and block, or a float32, float16 or
     bfloat16 CUDA matrix, which is held in 4 bits (quantize_fp4 with query_alpha and the rows'
     block) for the call (gf_product_fp4_raw).  The product of both alphas lies in [2^-127, 2^126].
-    out overlaps neither input; stream is as in quantize_fp4; test_wait is a test hook (0 in normal use)."""
+    out overlaps neither input; stream is as in quantize_fp4; test_wait is a test hook (0 in normal use).
+    product_fp4_timeouts tells outputs that a wait which ran out left as NaN from those of NaN data."""
     import torch
     p = _fp4_rows(rows, "gf_product_fp4")
     if not isinstance(queries, Fp4Rows) and not getattr(queries, "is_cuda", False):
         raise GarfieldError(1, "gf_product_fp4", "queries: expected Fp4Rows or a 2-D CUDA tensor")
     dtype = dtype or (out.dtype if out is not None else torch.float32)
     return _fp4_run("gf_product_fp4", p.device, stream, _fp4_product, queries, p, rows, dtype, out, query_alpha, test_wait)
+
+
+def product_fp4_timeouts(device=None) -> int:
+    """gf_product_fp4_timeouts: how many thread blocks of product_fp4 stopped on a device (None: the current one)
+    because a wait ran out, each leaving NaN in its outputs.  0 on a sound GPU.  Waits for the device."""
+    import torch
+    with torch.cuda.device(device):
+        torch.cuda.synchronize()
+        count = C.c_uint64()
+        _check(lib().gf_product_fp4_timeouts(C.byref(count)), "gf_product_fp4_timeouts")
+    return count.value
 
 
 def quantize_fp4_host(data: np.ndarray, alpha: float = 1.0, block: int = 32) -> Fp4Rows:

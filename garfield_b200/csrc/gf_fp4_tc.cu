@@ -26,8 +26,8 @@
 // cycles a stage whatever it holds (waiting, committing, the first instruction's way), while a group's
 // MMAs take 128 cycles at N = 128 and its panel's bytes 200 at the HBM rate.
 //
-// Every wait on a barrier in shared memory is bounded.  When one runs out the CTA stops and the outputs it still
-// owes become NaN.  The waits for TMEM, for the kernel before and at cluster barriers have no bound of their own:
+// Every wait on a barrier in shared memory is bounded.  When one runs out the CTA stops, is counted, and the outputs
+// it still owes become NaN.  The waits for TMEM, for the kernel before and at cluster barriers have no bound of their own:
 // the SM's holder of TMEM and the kernel before run to their ends without this CTA, and every CTA of a cluster
 // reaches every one of its barriers.
 #include <algorithm>
@@ -58,6 +58,8 @@ constexpr uint32_t kSmemLimit = 227 * 1024;
 // Zeros for the second column of an MMA step that the rows' last group lacks: with zero codes on the
 // query side, whatever codes stand in the other side's place add nothing.
 __device__ __align__(16) uint8_t g_zero[kFp4ColBytes];
+// CTAs of this device's products that stopped because a wait ran out.
+__device__ unsigned long long g_timeouts;
 
 enum Mode : uint32_t { kRing = 0, kFew = 1, kPair = 2 };
 constexpr uint32_t ctas_of(uint32_t mode) { return mode == kPair ? 2 : 1; }
@@ -752,6 +754,7 @@ __global__ void __launch_bounds__(threads_of(ctas_of(MODE)), 1) fp4_product_kern
         }
     }
     sync_all<CTAS>();
+    if (threadIdx.x == 0 && *stop) atomicAdd(&g_timeouts, 1ull);
     if (warp == 0) tmem_free<CTAS>(tmem);
 }
 
@@ -929,4 +932,12 @@ extern "C" gf_status gf_product_fp4_raw(const void* q, uint32_t q_dtype, uint64_
     const gf_status sq = gf_quantize_fp4(q, q_dtype, q_ld, m, dim, q_alpha, block, workspace, stream);
     if (sq != GF_OK) return sq;
     return product(A, workspace, m, r_packed, n, dim, block, scale, out, dtype, ld, test_wait, (cudaStream_t)stream);
+}
+
+extern "C" gf_status gf_product_fp4_timeouts(uint64_t* count) {
+    if (!count) return fail(GF_ERR_ARG, "null argument");
+    unsigned long long v = 0;
+    GF_CUDA(cudaMemcpyFromSymbol(&v, g_timeouts, sizeof v));
+    *count = v;
+    return GF_OK;
 }

@@ -499,10 +499,13 @@ gf_status gf_dequantize_fp4_host(const void* packed, uint32_t n, uint32_t dim, u
  * call gives the same bits every time.  out must not overlap the inputs.  Rows of out that start
  * on 32-byte boundaries (out and ld) are written faster, by up to a half where out is far larger than L2.
  * Whichever of the two has more rows is best passed as r.
+ * Every wait for a copy or an MMA is bounded (some four seconds).  When one runs out, the CTA stops and what it
+ * still owes of out becomes NaN; gf_product_fp4_timeouts gives the number of CTAs that stopped so on the
+ * current device since the library was loaded, of the calls that have ended (synchronise with them first).
+ * It waits for the device like a copy on the default stream and cannot be captured.
  * test_wait: 0 in normal use.  Test hook for the timeout path: the kernel's waits give up after
- * test_wait polls (at most 2^20, which waits in normal use have: some four seconds) and no stage of rows is
- * ever reported to be in place, so all of out becomes NaN.  Copies under way are waited for as long as in
- * normal use.
+ * test_wait polls (at most 2^20, as in normal use) and no stage of rows is ever reported to be in place, so
+ * all of out becomes NaN.  Copies under way are waited for as long as in normal use.
  * gf_product_fp4_raw takes the queries as they are (q_dtype, rows q_ld elements apart) and holds them in 4
  * bits, with q_alpha and the rows' block, for the call.  workspace (device, 16-byte aligned, of
  * gf_fp4_bytes(m, dim, block) bytes) receives them; it may be NULL when m <= 16, dim <= 8192 and
@@ -515,6 +518,7 @@ gf_status gf_product_fp4(const void* q_packed, uint32_t m, const void* r_packed,
 gf_status gf_product_fp4_raw(const void* q, uint32_t q_dtype, uint64_t q_ld, uint32_t m, float q_alpha,
                              const void* r_packed, uint32_t n, uint32_t dim, uint32_t block, float scale, void* out,
                              uint32_t dtype, uint64_t ld, void* workspace, uint32_t test_wait, void* stream);
+gf_status gf_product_fp4_timeouts(uint64_t* count);
 
 /* attrs.bin: uint32 n, uint32 a, n*a int32 (tools.cuh:747-765). */
 gf_status gf_read_attrs(const char* path, int32_t** attrs, uint32_t* n, uint32_t* a);

@@ -306,3 +306,7 @@ def test_alpha_is_one_number(alpha):
     """What the codec multiplied by is what the products are divided by: alpha in fp32."""
     assert gf.quantize_fp4_host(np.ones((3, 8), np.float32), alpha).alpha == float(np.float32(alpha))
     assert gf.Fp4Rows(None, 3, 8, 32, alpha).alpha == float(np.float32(alpha))
+
+
+def test_timeout_count_refusal():
+    assert gf.lib().gf_product_fp4_timeouts(None) == 1 and b"null" in gf.lib().gf_last_error()

@@ -376,3 +376,18 @@ def test_products_use_the_alphas_of_the_codec(m):
     assert torch.equal(gf.product_fp4(q, rows, query_alpha=alpha).double(), want)
     assert torch.equal(gf.product_fp4(gf.quantize_fp4(q, alpha, 16), rows).double(), want)
     assert torch.equal(gf.dequantize_fp4(rows), r)
+
+
+@pytest.mark.parametrize("m,n,dim", [(300, 19000, 1100), (1, 500, 4096), (40, 1000, 96)])
+def test_waits_that_run_out_are_counted(m, n, dim):
+    """NaN left by a wait that ran out is told from NaN data: pairs, shares of a tile, single CTAs."""
+    q, rows = exact_rows(m, dim, 32, 1), gf.quantize_fp4(exact_rows(n, dim, 32, 2))
+    before = gf.product_fp4_timeouts()
+    q[0] = float("nan")
+    assert torch.isnan(gf.product_fp4(q, rows)[0]).all()
+    assert gf.product_fp4_timeouts() == before
+    gf.product_fp4(q, rows, test_wait=4)
+    after = gf.product_fp4_timeouts(torch.device("cuda", 0))
+    assert before < after <= before + 148
+    gf.product_fp4(q, rows)
+    assert gf.product_fp4_timeouts() == after
