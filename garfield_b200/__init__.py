@@ -591,10 +591,11 @@ def _fp4_dtype(dtype, what: str) -> int:
 
 
 def _fp4_matrix(t, what: str, name: str):
-    """(rows, columns, row stride) of a CUDA matrix whose rows are each without gaps."""
-    if not getattr(t, "is_cuda", False) or t.dim() != 2:
+    """(rows, columns, row stride) of a CUDA tensor, which has to be a matrix whose rows are each without gaps."""
+    shape = t.shape
+    if len(shape) != 2:
         raise GarfieldError(1, what, f"{name}: expected a 2-D CUDA tensor")
-    n, dim = t.shape
+    n, dim = shape
     ld, step = t.stride()
     if n <= 1:
         ld = dim
