@@ -614,12 +614,16 @@ def _fp4_size(n: int, dim: int, block: int) -> int:
     return -(-n // 128) * (-(-dim // 128) * (16384 // block) + -(-dim // 32) * rows * 16)
 
 
+def _fp4_shape(rows, what: str) -> None:
+    if rows.block not in (16, 32) or not (0 < rows.dim < 2 ** 32 and 0 <= rows.n < 2 ** 32):
+        raise GarfieldError(1, what, f"n {rows.n}, dim {rows.dim}, block {rows.block}")
+
+
 def _fp4_rows(rows, what: str):
     p = getattr(rows, "packed", None)
     if not isinstance(rows, Fp4Rows) or not getattr(p, "is_cuda", False):
         raise GarfieldError(1, what, "expected Fp4Rows on a GPU")
-    if rows.block not in (16, 32) or rows.dim <= 0 or rows.n < 0:
-        raise GarfieldError(1, what, f"n {rows.n}, dim {rows.dim}, block {rows.block}")
+    _fp4_shape(rows, what)
     if p.element_size() != 1 or not p.is_contiguous() or p.numel() < _fp4_size(rows.n, rows.dim, rows.block):
         raise GarfieldError(1, what, f"Fp4Rows.packed: expected {_fp4_size(rows.n, rows.dim, rows.block)} contiguous bytes")
     return p
@@ -794,6 +798,7 @@ def product_fp4_timeouts(device=None) -> int:
 def quantize_fp4_host(data: np.ndarray, alpha: float = 1.0, block: int = 32) -> Fp4Rows:
     """gf_quantize_fp4_host on a float32 array: the same bytes as quantize_fp4."""
     data = np.ascontiguousarray(data, dtype=np.float32)
+    _fp4_need(data.ndim == 2, "gf_quantize_fp4_host", "data: expected a 2-D array")
     n, dim = data.shape
     _fp4_need(dim > 0 and block in (16, 32), "gf_quantize_fp4_host", f"dim {dim}, block {block}")
     packed = np.empty(_fp4_size(n, dim, block), np.uint8)
@@ -804,6 +809,8 @@ def quantize_fp4_host(data: np.ndarray, alpha: float = 1.0, block: int = 32) -> 
 def dequantize_fp4_host(rows: Fp4Rows) -> np.ndarray:
     """gf_dequantize_fp4_host: the float32 values that rows with a host array are held as."""
     what = "gf_dequantize_fp4_host"
+    _fp4_need(isinstance(rows, Fp4Rows), what, "expected Fp4Rows")
+    _fp4_shape(rows, what)
     p = rows.packed
     _fp4_need(isinstance(p, np.ndarray) and p.dtype == np.uint8 and p.flags["C_CONTIGUOUS"], what,
               "Fp4Rows.packed: expected a contiguous uint8 array")

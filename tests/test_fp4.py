@@ -310,3 +310,28 @@ def test_alpha_is_one_number(alpha):
 
 def test_timeout_count_refusal():
     assert gf.lib().gf_product_fp4_timeouts(None) == 1 and b"null" in gf.lib().gf_last_error()
+
+
+@pytest.mark.parametrize("field", [dict(block=0), dict(block=8), dict(n=-1), dict(n=2 ** 32 + 4), dict(dim=0), dict(dim=2 ** 32 + 8),
+                                   dict(dim=-8)])
+def test_rows_of_bad_shapes_are_refused(field):
+    """By the host call and before a GPU call (which takes both numbers in 32 bits)."""
+    class Cuda(np.ndarray):
+        is_cuda = True
+
+    rows = gf.quantize_fp4_host(np.ones((4, 8), np.float32))
+    for name, v in field.items():
+        setattr(rows, name, v)
+    with pytest.raises(gf.GarfieldError, match="block"):
+        gf.dequantize_fp4_host(rows)
+    rows.packed = rows.packed.view(Cuda)
+    with pytest.raises(gf.GarfieldError, match="block"):
+        gf._fp4_rows(rows, "gf_dequantize_fp4")
+
+
+def test_host_calls_refuse_other_things():
+    for bad in (np.ones(8, np.float32), np.ones((2, 2, 8), np.float32)):
+        with pytest.raises(gf.GarfieldError, match="2-D"):
+            gf.quantize_fp4_host(bad)
+    with pytest.raises(gf.GarfieldError, match="Fp4Rows"):
+        gf.dequantize_fp4_host(np.ones(8, np.uint8))
