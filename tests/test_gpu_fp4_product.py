@@ -391,3 +391,22 @@ def test_waits_that_run_out_are_counted(m, n, dim):
     assert before < after <= before + 148
     gf.product_fp4(q, rows)
     assert gf.product_fp4_timeouts() == after
+
+
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("m,n,dim", [
+    (1, 100, 4100), (16, 100, 4480), (1, 2000, 5200), (16, 500, 6272),  # 33 to 49 groups of 128 elements: 7 CTAs
+    (1, 128, 7168), (1, 100, 4096), (3, 129, 4608),  # 8
+    (20, 300, 4480), (40, 128, 4225), (20, 300, 8192), (64, 1000, 2049),  # 4
+    (128, 128, 1025),  # 2
+])
+def test_shares_of_every_number(m, n, dim, block):
+    """Rows of long elements, split over clusters of 2, 4, 7 and 8 CTAs with shares that do not come out even."""
+    check_exact(m, n, dim, block)
+
+
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("m,n,dim", [(20_000, 100, 1024), (20_000, 1, 800), (20_000, 128, 1056), (19_201, 33, 1000), (20_000, 300, 768)])
+def test_pairs_of_ctas_with_few_rows(m, n, dim, block):
+    """Many queries against one row panel, short or whole, or three: the second half of some pairs' tiles is empty."""
+    check_exact(m, n, dim, block)
