@@ -614,18 +614,21 @@ def _fp4_size(n: int, dim: int, block: int) -> int:
     return -(-n // 128) * (-(-dim // 128) * (16384 // block) + -(-dim // 32) * rows * 16)
 
 
-def _fp4_shape(rows, what: str) -> None:
-    if rows.block not in (16, 32) or not (0 < rows.dim < 2 ** 32 and 0 <= rows.n < 2 ** 32):
-        raise GarfieldError(1, what, f"n {rows.n}, dim {rows.dim}, block {rows.block}")
+def _fp4_shape(rows, what: str) -> int:
+    """The size of rows, whose shape has to be one that the library takes."""
+    n, dim, block = rows.n, rows.dim, rows.block
+    if block not in (16, 32) or not (0 < dim < 2 ** 32 and 0 <= n < 2 ** 32):
+        raise GarfieldError(1, what, f"n {n}, dim {dim}, block {block}")
+    return _fp4_size(n, dim, block)
 
 
 def _fp4_rows(rows, what: str):
     p = getattr(rows, "packed", None)
     if not isinstance(rows, Fp4Rows) or not getattr(p, "is_cuda", False):
         raise GarfieldError(1, what, "expected Fp4Rows on a GPU")
-    _fp4_shape(rows, what)
-    if p.element_size() != 1 or not p.is_contiguous() or p.numel() < _fp4_size(rows.n, rows.dim, rows.block):
-        raise GarfieldError(1, what, f"Fp4Rows.packed: expected {_fp4_size(rows.n, rows.dim, rows.block)} contiguous bytes")
+    size = _fp4_shape(rows, what)
+    if p.element_size() != 1 or not p.is_contiguous() or p.numel() < size:
+        raise GarfieldError(1, what, f"Fp4Rows.packed: expected {size} contiguous bytes")
     return p
 
 
@@ -722,7 +725,7 @@ def dequantize_fp4(rows: Fp4Rows, dtype=None, out=None, stream=None):
     otherwise).  out does not overlap rows; stream is as in quantize_fp4."""
     import torch
     p = _fp4_rows(rows, "gf_dequantize_fp4")
-    dtype = dtype or (out.dtype if out is not None else torch.float32)
+    dtype = dtype or (torch.float32 if out is None else out.dtype)
     return _fp4_run("gf_dequantize_fp4", p.device, stream, _fp4_dequantize, p, rows, dtype, out)
 
 
@@ -736,7 +739,6 @@ def _fp4_scale(query_alpha: float, alpha: float, what: str) -> float:
 
 
 def _fp4_product(s, queries, p, rows, dtype, out, query_alpha, test_wait):
-    import torch
     what = "gf_product_fp4"
     dt = _fp4_dtype(dtype, what)
     device, dim, block = p.device, rows.dim, rows.block
@@ -756,6 +758,7 @@ def _fp4_product(s, queries, p, rows, dtype, out, query_alpha, test_wait):
         # (what the call quantises in passing needs no room)
         ws = None
         if not (m <= 16 and dim <= 8192 and m * dim <= 32768):
+            import torch
             ws = torch.empty(_fp4_size(m, dim, block), dtype=torch.uint8, device=device)
         st = lib().gf_product_fp4_raw(qp.data_ptr(), qdt, qld, m, query_alpha, p.data_ptr(), rows.n, dim, block,
                                       _fp4_scale(C.c_float(query_alpha).value, rows.alpha, what), out.data_ptr(), dt, ld,
@@ -810,11 +813,11 @@ def dequantize_fp4_host(rows: Fp4Rows) -> np.ndarray:
     """gf_dequantize_fp4_host: the float32 values that rows with a host array are held as."""
     what = "gf_dequantize_fp4_host"
     _fp4_need(isinstance(rows, Fp4Rows), what, "expected Fp4Rows")
-    _fp4_shape(rows, what)
+    size = _fp4_shape(rows, what)
     p = rows.packed
     _fp4_need(isinstance(p, np.ndarray) and p.dtype == np.uint8 and p.flags["C_CONTIGUOUS"], what,
               "Fp4Rows.packed: expected a contiguous uint8 array")
-    _fp4_need(p.size >= _fp4_size(rows.n, rows.dim, rows.block), what, "Fp4Rows.packed is too short")
+    _fp4_need(p.size >= size, what, "Fp4Rows.packed is too short")
     out = np.empty((rows.n, rows.dim), np.float32)
     _check(lib().gf_dequantize_fp4_host(_np_ptr(p), rows.n, rows.dim, rows.block, rows.alpha, _np_ptr(out)), what)
     return out
