@@ -24,7 +24,7 @@
 // neighbouring lanes hold a row's column of 32 elements and the next lanes the next row, so a warp's
 // codes fill whole 32-byte sectors of the panel.  The reader's threads take what one store
 // holds (16 bytes, or 8, as the rows are aligned; else four elements), so a warp's stores leave no sector
-// half written.  A CTA is short (one group of a panel); six of them on an SM overlap their loads and arithmetic.
+// half written.  A CTA is short (one group of a panel); four to six of them on an SM overlap their loads and arithmetic.
 // Rows in flight per thread: 16-bit data 2, with 6 CTAs on an SM (4 rows and the 4 CTAs that their registers
 // allow win and lose: bf16 1M x 128 57 us against 61, bf16 8192 x 8192 in blocks of 16 35 against 37, fp16 1M x 128
 // in blocks of 16 62 against 57; 1 row and 8 CTAs: 64, 39 and 66), fp32 4 (1M x 128: 83 us against 86, in blocks of

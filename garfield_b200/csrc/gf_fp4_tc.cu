@@ -331,10 +331,10 @@ __device__ __forceinline__ void store16(T* d0, uint64_t ld, const uint32_t* v, f
 }
 
 // fp32 rows of out that do not start on 32-byte sectors ("torn"): a warp's 32 elements of a row then leave a
-// sector half written at either end, which out of L2 costs twice the time.  A group's four warps gather
-// kTornCols rows' 128 elements in shared memory instead, and a warp writes whole rows, each store within one
-// 128-byte line (10000 x 99977 x 128: 1059 us against 1720; in 16 bits taking words apart costs more than
-// it saves).
+// sector half written at either end, which costs where they reach HBM so.  Where out is far larger than L2, a group's
+// four warps gather kTornCols rows' 128 elements in shared memory instead, and a warp writes whole rows, each
+// store within one 128-byte line: 10000 x 99977 x 128 1114 us against 1227, 4000 x 99977 x 128 (1.5 GB) 450 against
+// 455, but 2000 x 99977 x 128 229 against 208 and 300 x 77777 x 200 (in L2) 37 against 25.5.
 constexpr uint32_t kTornCols = 8;
 constexpr uint32_t kTornPitch = kFp4Rows + 4;                       // floats
 constexpr uint32_t kTornBytes = 2 * kTornCols * kTornPitch * 4;     // of a group: two buffers in turn
@@ -807,7 +807,8 @@ gf_status product(ProdArgs A, const void* q, uint32_t m, const void* r, uint32_t
     A.polls = test_wait ? test_wait : kPolls;
     A.hold = test_wait ? 1u : 0u;
     const uint32_t sub = block == 16 ? 2 : 1, scales = sub * kFp4ScaleSub, group = scales + 4 * kFp4ColBytes, G = A.Lr.groups;
-    // Pairs of CTAs once their tiles, of 256 x 256, occupy every SM, where the rows are long enough for
+    // Pairs of CTAs once their tiles, of 256 x 256, occupy every SM (of one row panel, or the last of an odd number,
+    // half a tile is empty and counts all the same), where the rows are long enough for
     // their arithmetic to show (8192 x 16384 in bf16: 96 us against 78 at 512 elements, 86 against 97 at 768,
     // 117 against 151 at 2048), and where out is far larger than L2 and its rows are of 16 bits and torn, or of
     // 32 and not: a pair writes twice as long a run of each row at a time (10000 x 99999 x 128 in fp16 744 us
@@ -816,7 +817,8 @@ gf_status product(ProdArgs A, const void* q, uint32_t m, const void* r, uint32_t
     const uint64_t pair_tiles = ((uint64_t)A.panels + 1) / 2 * ((A.qpanels + 1) / 2);
     const uint32_t es = dtype_bytes(dtype);
     const bool torn = (reinterpret_cast<uintptr_t>(out) | (m > 1 ? ld * es : 0u)) % 32 != 0;
-    const bool large = m >= 1024 && (uint64_t)m * n >= (1ull << 30) / es && torn == (es == 2);
+    const bool past_l2 = (uint64_t)m * n >= (1ull << 30) / es;
+    const bool large = m >= 1024 && past_l2 && torn == (es == 2);
     uint32_t mode = (G >= 6 || large) && A.qpanels >= 2 && pair_tiles >= (uint64_t)sms / 2 ? kPair : kRing;
     const uint32_t ctas = ctas_of(mode);
     A.nt = mode == kPair ? 256 : A.Lq.col_bytes / 16;
@@ -841,7 +843,7 @@ gf_status product(ProdArgs A, const void* q, uint32_t m, const void* r, uint32_t
         A.per = G;
     }
     A.gs = std::min(A.gs, A.per);
-    A.torn = torn && es == 4 && m >= 16 && mode != kPair && A.split == 1;
+    A.torn = torn && es == 4 && past_l2 && m >= 16 && mode != kPair && A.split == 1;
     const uint32_t bars = (3 * kMaxStages + 2 * kMaxAcc + 2) * 8 + 16;
     const uint32_t fixed = bars + (A.torn ? epi_groups(1) * kTornBytes : 0u);
     const uint32_t resident = mode == kFew ? A.per * (scales + 4 * A.Lq.col_bytes) : 0u;
