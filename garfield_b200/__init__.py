@@ -590,6 +590,11 @@ def _fp4_dtype(dtype, what: str) -> int:
     return dt
 
 
+def _fp4_float32():
+    import torch
+    return torch.float32
+
+
 def _fp4_matrix(t, what: str, name: str):
     """(rows, columns, row stride) of a CUDA tensor, which has to be a matrix whose rows are each without gaps."""
     shape = t.shape
@@ -627,7 +632,7 @@ def _fp4_rows(rows, what: str):
     if not isinstance(rows, Fp4Rows) or not getattr(p, "is_cuda", False):
         raise GarfieldError(1, what, "expected Fp4Rows on a GPU")
     size = _fp4_shape(rows, what)
-    if p.element_size() != 1 or not p.is_contiguous() or p.numel() < size:
+    if p.numel() < size or p.element_size() != 1 or not p.is_contiguous():
         raise GarfieldError(1, what, f"Fp4Rows.packed: expected {size} contiguous bytes")
     return p
 
@@ -723,9 +728,9 @@ def _fp4_dequantize(s, p, rows, dtype, out):
 def dequantize_fp4(rows: Fp4Rows, dtype=None, out=None, stream=None):
     """gf_dequantize_fp4: the values that rows are held as (n x dim, float32 unless dtype or out say
     otherwise).  out does not overlap rows; stream is as in quantize_fp4."""
-    import torch
     p = _fp4_rows(rows, "gf_dequantize_fp4")
-    dtype = dtype or (torch.float32 if out is None else out.dtype)
+    if dtype is None:
+        dtype = _fp4_float32() if out is None else out.dtype
     return _fp4_run("gf_dequantize_fp4", p.device, stream, _fp4_dequantize, p, rows, dtype, out)
 
 
@@ -779,11 +784,11 @@ def product_fp4(queries, rows: Fp4Rows, dtype=None, out=None, query_alpha: float
     block) for the call (gf_product_fp4_raw).  The product of both alphas lies in [2^-127, 2^126].
     out overlaps neither input; stream is as in quantize_fp4; test_wait is a test hook (0 in normal use).
     product_fp4_timeouts tells outputs that a wait which ran out left as NaN from those of NaN data."""
-    import torch
     p = _fp4_rows(rows, "gf_product_fp4")
     if not isinstance(queries, Fp4Rows) and not getattr(queries, "is_cuda", False):
         raise GarfieldError(1, "gf_product_fp4", "queries: expected Fp4Rows or a 2-D CUDA tensor")
-    dtype = dtype or (out.dtype if out is not None else torch.float32)
+    if dtype is None:
+        dtype = _fp4_float32() if out is None else out.dtype
     return _fp4_run("gf_product_fp4", p.device, stream, _fp4_product, queries, p, rows, dtype, out, query_alpha, test_wait)
 
 
